@@ -1,0 +1,477 @@
+"""Operator cases: group norm with an activation, and products in 8 bits.
+
+Residual blocks of image decoders and U-Nets normalise a channels-last map over
+groups of channels, apply an activation and convolve the result.  The cases
+below are those steps, with their inputs and outputs in device memory:
+
+  norm    group norm and an activation of a map, f16 or f32 in and out
+  norm8   the same with its result in 8 bits (e4m3 with a power-of-two scale
+          for each 128 channels of a pixel), read back as f16
+  quant   rows in 8 bits, read back as f32
+  rows8   a product of rows in 8 bits with weights in 8 bits
+  conv8   a 3 x 3 convolution of a map in 8 bits with weights in 8 bits
+  block   x + conv8(norm8(conv8(norm8(x)))): the four steps of a residual block
+
+A row of k values in 8 bits is ceil(k / 128) blocks of 128 e4m3 bytes (zeros
+past k) and a byte of scale a block: the block's values are e4m3 x 2^(byte -
+127), with the smallest exponent that keeps the largest magnitude at most 448.
+The scales of a row are padded to whole groups of four bytes.  Weights have a
+scale for each 128 input channels of a tap and output.
+"""
+
+import functools
+import importlib
+import math
+
+import torch
+
+own = False
+
+DEVICE = "cuda:0"
+EPS = 1e-5
+BLOCK = 128
+TYPES = {"f16": torch.float16, "f32": torch.float32}
+
+
+def listed():
+    return [
+        # The innermost map of a U-Net: latency.
+        dict(name="norm_16x16_512", kind="norm", images=1, height=16, width=16, c=512, groups=32, extra=0,
+             act="silu", into="f16", outof="f16"),
+        # Two ragged maps, the normalised channels a part of each pixel's.
+        dict(name="norm_85x125_384", kind="norm", images=2, height=85, width=125, c=384, groups=24, extra=128,
+             act="none", into="f16", outof="f32"),
+        # A decoder's last, full-size map.
+        dict(name="norm_512x768_128", kind="norm", images=1, height=512, width=768, c=128, groups=32, extra=0,
+             act="silu", into="f16", outof="f16"),
+        # A middle map on its way into an 8-bit convolution.
+        dict(name="norm8_64x96_640", kind="norm8", images=1, height=64, width=96, c=640, groups=32, extra=0,
+             act="silu", into="f16"),
+        # The tokens of a text or class condition.
+        dict(name="quant_77_768", kind="quant", rows=77, k=768, extra=0, into="f16"),
+        # A full-size map of 512 channels that was accumulated in f32.
+        dict(name="quant_98304_512", kind="quant", rows=98304, k=512, extra=0, into="f32"),
+        # A time embedding's layer: one row.
+        dict(name="rows8_1_1280_5120", kind="rows8", rows=1, k=1280, n=5120, extra=0, act="silu", add=False,
+             outof="f16"),
+        # The first layer of a transformer stage's MLP.
+        dict(name="rows8_4096_384_1536", kind="rows8", rows=4096, k=384, n=1536, extra=0, act="gelu", add=False,
+             outof="f16"),
+        # A wide MLP over the tokens of four 1024 x 1024 images.
+        dict(name="rows8_16384_2048_8192", kind="rows8", rows=16384, k=2048, n=8192, extra=0, act="none",
+             add=False, outof="f16"),
+        # A local convolution on the ragged map of an editor's photograph.
+        dict(name="conv8_85x125_512_128", kind="conv8", images=1, height=85, width=125, step=1, cin=512, cout=128,
+             extra=0, act="relu", add=False, outof="f16"),
+        # A decoder's convolution at 384 x 256, accumulated onto the map.
+        dict(name="conv8_256x384_256_256", kind="conv8", images=1, height=256, width=384, step=1, cin=256,
+             cout=256, extra=0, act="none", add=True, outof="f16"),
+        # A residual block in the middle of a decoder.
+        dict(name="block_64x64_512", kind="block", images=1, height=64, width=64, c=512, groups=32),
+    ]
+
+
+def _log_int(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def _sides(rng, low, high, area):
+    """Two sides spread over their logarithm, their product at most `area`."""
+    while True:
+        h, w = _log_int(rng, low, high), _log_int(rng, low, high)
+        if h * w <= area:
+            return h, w
+
+
+def draw(rng):
+    kind = rng.choice(("norm", "norm", "norm8", "quant", "rows8", "rows8", "conv8", "conv8", "block"))
+    if kind in ("norm", "norm8"):
+        per = rng.choice((1, 3, 4, 7, 8, 12, 16, 20, 32))  # channels a group
+        groups = rng.choice((1, 4, 8, 24, 32, 32, 32))
+        images = rng.choice((1, 1, 2, 3))
+        h, w = _sides(rng, 1, 700, 48 * (1 << 20) // (per * groups * images))
+        case = dict(kind=kind, images=images, height=h, width=w, c=per * groups, groups=groups,
+                    extra=rng.choice((0, 0, 8, 13)), act=rng.choice(("silu", "silu", "none", "relu", "gelu")),
+                    into=rng.choice(("f16", "f16", "f32")))
+        if kind == "norm":
+            case["outof"] = rng.choice(("f16", "f16", "f32"))
+        return case
+    if kind == "quant":
+        k = rng.choice((_log_int(rng, 1, 4096), 128 * rng.randint(1, 16)))
+        return dict(kind=kind, rows=_log_int(rng, 1, 50 * 10**6 // (BLOCK * _blocks(k))), k=k, extra=rng.choice((0, 0, 8, 5)),
+                    into=rng.choice(("f16", "f32")))
+    if kind == "rows8":
+        while True:
+            k = rng.choice((_log_int(rng, 16, 8192), 64 * rng.randint(1, 40)))
+            n = rng.choice((_log_int(rng, 1, 8192), 64 * rng.randint(1, 64)))
+            rows = _log_int(rng, 1, 65536)
+            if 2.0 * rows * k * n <= 5e11 and rows * max(k, n) <= 1 << 27:
+                break
+        return dict(kind=kind, rows=rows, k=k, n=n, extra=rng.choice((0, 0, 8, 3)),
+                    act=rng.choice(("none", "none", "gelu", "silu", "relu")), add=rng.random() < 0.3,
+                    outof=rng.choice(("f16", "f16", "f32")))
+    if kind == "conv8":
+        while True:
+            cin = rng.choice((36, 64, 128, 256, 320, 512))
+            cout = rng.choice((3, 48, 64, 128, 256, 320, 512))
+            images = rng.choice((1, 1, 2))
+            h, w = _sides(rng, 1, 512, 512 * 512)
+            if images * h * w * max(9 * cin, cout) <= 1 << 28:
+                break
+        return dict(kind=kind, images=images, height=h, width=w, step=rng.choice((1, 1, 2)), cin=cin, cout=cout,
+                    extra=rng.choice((0, 0, 8, 3)), act=rng.choice(("none", "relu", "silu")),
+                    add=rng.random() < 0.4, outof=rng.choice(("f16", "f16", "f32")))
+    c = rng.choice((64, 128, 256, 320, 512))
+    h, w = _sides(rng, 8, 256, (1 << 28) // (9 * c))
+    return dict(kind=kind, images=rng.choice((1, 2)) if h * w * c < 1 << 23 else 1, height=h, width=w, c=c,
+                groups=rng.choice((8, 16, 32)))
+
+
+# ---- rows in 8 bits, in elementary operations ------------------------------------
+
+
+def _blocks(k):
+    return -(-k // BLOCK)
+
+
+def _power(e):
+    """2^e for whole e in -126 .. 127."""
+    return ((e + 127) << 23).to(torch.int32).view(torch.float32)
+
+
+def _quantize(x):
+    """f32 rows [r, k] as e4m3 [r, blocks, 128] and exponents [r, blocks]."""
+    r, k = x.shape
+    x = torch.cat([x, x.new_zeros(r, _blocks(k) * BLOCK - k)], 1).reshape(r, -1, BLOCK)
+    largest = x.abs().amax(2)
+    m, e = torch.frexp(largest)  # m in 1/2 .. 1; 448 = 7/8 x 2^9
+    e = torch.where(largest > 0, e.to(torch.int32) - 9 + (m > 0.875), 0)
+    return (x * _power(-e)[:, :, None]).to(torch.float8_e4m3fn), e
+
+
+def _values(q, e, k):
+    """The f32 rows that _quantize's result stands for."""
+    return (q.float() * _power(e)[:, :, None]).reshape(q.shape[0], -1)[:, :k]
+
+
+def _laid_out(q, e):
+    """The bytes of rows in 8 bits: data [r, 128 blocks] and scales [r, a multiple of 4]."""
+    r, blocks = e.shape
+    scales = torch.full((r, 4 * -(-blocks // 4)), 127, dtype=torch.uint8, device=e.device)
+    scales[:, :blocks] = (e + 127).to(torch.uint8)
+    return q.view(torch.uint8).reshape(r, -1), scales
+
+
+def _weights(w, taps):
+    """f32 weights [taps c, n] as the f32 values of their 8-bit form."""
+    c, n = w.shape[0] // taps, w.shape[1]
+    rows = w.reshape(taps, c, n).permute(0, 2, 1).reshape(taps * n, c)
+    return _values(*_quantize(rows), c).reshape(taps, n, c).permute(0, 2, 1).reshape(taps * c, n).contiguous()
+
+
+def _act(v, act):
+    if act == "silu":
+        return v * torch.sigmoid(v)
+    if act == "gelu":
+        return 0.5 * v * (1 + torch.erf(v * math.sqrt(0.5)))
+    return torch.relu(v) if act == "relu" else v
+
+
+def _norm(x, images, c, groups, gamma, beta, act):
+    """f32 [images, pixels, c] normalised over pixels and each group's channels."""
+    v = x.reshape(images, -1, groups, c // groups)
+    v = v - v.mean((1, 3), keepdim=True)
+    v = v * torch.rsqrt((v * v).mean((1, 3), keepdim=True) + EPS)
+    return _act(v.reshape(images, -1, c) * gamma + beta, act)
+
+
+def _patches(x, images, height, width, step):
+    """f32 pixels [images h w, c] as the rows [images oh ow, 9 c] of a zero-padded 3 x 3 convolution."""
+    c = x.shape[1]
+    x = x.reshape(images, height, width, c)
+    x = torch.cat([x.new_zeros(images, 1, width, c), x, x.new_zeros(images, 1, width, c)], 1)
+    x = torch.cat([x.new_zeros(images, height + 2, 1, c), x, x.new_zeros(images, height + 2, 1, c)], 2)
+    return torch.cat([x[:, dy:dy + height:step, dx:dx + width:step].reshape(-1, c)
+                      for dy in range(3) for dx in range(3)], 1)
+
+
+# ---- what a program holds --------------------------------------------------------
+
+
+@functools.lru_cache(maxsize=None)
+def _ien():
+    return importlib.import_module("image-engine-native_amd.ien")
+
+
+@functools.lru_cache(maxsize=None)
+def _context():
+    return _ien().Context(0)
+
+
+def _rows8(q, e, k):
+    """Quantised rows as the library holds them."""
+    data, scales = _laid_out(q, e)
+    return _ien().Rows8(data.shape[0], k, data=data, scales=scales)
+
+
+def _features(g, rows, c):
+    """What a map holds: channels of their own mean and spread, a few far values."""
+    x = torch.randn(rows, c, generator=g, device=DEVICE)
+    x += 0.02 * x * x * x
+    x *= 0.3 + 1.5 * torch.rand(c, generator=g, device=DEVICE)
+    return x.add_(torch.randn(c, generator=g, device=DEVICE))
+
+
+def _held(x, extra, dtype):
+    """Rows as `dtype` in a buffer with `extra` more columns, and the view of theirs."""
+    buffer = torch.zeros(x.shape[0], x.shape[1] + extra, dtype=dtype, device=DEVICE)
+    buffer[:, :x.shape[1]] = x
+    return buffer[:, :x.shape[1]]
+
+
+def _layer(g, taps, c, n):
+    """Weights, as the f32 that a file holds, and biases."""
+    w = torch.randn(taps * c, n, generator=g, device=DEVICE) / math.sqrt(taps * c)
+    b = 0.3 * torch.randn(n, generator=g, device=DEVICE)
+    if own:
+        return dict(matrix=_ien().Matrix8(_context(), w.cpu().numpy(), b.cpu().numpy(), taps=taps))
+    return dict(w=_weights(w, taps), b=b)
+
+
+def _gains(g, c):
+    return 1 + 0.2 * torch.randn(c, generator=g, device=DEVICE), 0.2 * torch.randn(c, generator=g, device=DEVICE)
+
+
+def prepare(case, seed):
+    if own:
+        _context()
+    g = torch.Generator(device=DEVICE)
+    g.manual_seed(seed)
+    kind, s = case["kind"], dict(case)
+    if kind in ("norm", "norm8"):
+        pixels = case["images"] * case["height"] * case["width"]
+        s["x"] = _held(_features(g, pixels, case["c"]), case["extra"], TYPES[case["into"]])
+        s["gamma"], s["beta"] = _gains(g, case["c"])
+        if own:
+            if kind == "norm8":
+                s["q"] = _ien().Rows8(pixels, case["c"])
+            s["y"] = torch.empty(pixels, case["c"], dtype=TYPES[case.get("outof", "f16")], device=DEVICE)
+    elif kind == "quant":
+        s["x"] = _held(_features(g, case["rows"], case["k"]), case["extra"], TYPES[case["into"]])
+        if own:
+            s["q"] = _ien().Rows8(case["rows"], case["k"])
+            s["y"] = torch.empty(case["rows"], case["k"], dtype=torch.float32, device=DEVICE)
+    elif kind in ("rows8", "conv8"):
+        if kind == "rows8":
+            taps, rows, k, n, outs = 1, case["rows"], case["k"], case["n"], case["rows"]
+        else:
+            taps, k, n, step = 9, case["cin"], case["cout"], case["step"]
+            rows = case["images"] * case["height"] * case["width"]
+            outs = case["images"] * -(-case["height"] // step) * -(-case["width"] // step)
+        q, e = _quantize(_act(_features(g, rows, k), "silu"))
+        s["layer"] = _layer(g, taps, k, n)
+        if case["add"]:
+            s["residual"] = _held(torch.randn(outs, n, generator=g, device=DEVICE), case["extra"], TYPES[case["outof"]])
+        if own:
+            s["q"] = _rows8(q, e, k)
+            s["y"] = _held(torch.zeros(outs, n, device=DEVICE), case["extra"], TYPES[case["outof"]])
+        else:
+            s["q"], s["e"] = q, e
+    else:
+        c, pixels = case["c"], case["images"] * case["height"] * case["width"]
+        s["x"] = _features(g, pixels, c).half()
+        s["norms"] = [_gains(g, c), _gains(g, c)]
+        s["layers"] = [_layer(g, 9, c, c), _layer(g, 9, c, c)]
+        if own:
+            s["q"] = _ien().Rows8(pixels, c)
+            s["h"], s["y"] = torch.empty_like(s["x"]), torch.empty_like(s["x"])
+    return s
+
+
+# ---- one pass --------------------------------------------------------------------
+
+
+def _act_of(s):
+    ien = _ien()
+    return {"none": ien.ACT_NONE, "relu": ien.ACT_RELU, "gelu": ien.ACT_GELU, "silu": ien.ACT_SILU}[s["act"]]
+
+
+def _run_own(s):
+    ien, ctx, kind = _ien(), _context(), s["kind"]
+    if kind == "norm":
+        ien.group_norm(ctx, s["x"], s["images"], s["groups"], s["gamma"], s["beta"], s["y"], eps=EPS, act=_act_of(s))
+    elif kind == "norm8":
+        ien.group_norm(ctx, s["x"], s["images"], s["groups"], s["gamma"], s["beta"], s["q"], eps=EPS, act=_act_of(s))
+        ien.dequantize8(ctx, s["q"], s["y"])
+    elif kind == "quant":
+        ien.quantize8(ctx, s["x"], s["q"])
+        ien.dequantize8(ctx, s["q"], s["y"])
+    elif kind == "rows8":
+        ien.multiply8(ctx, s["q"], s["layer"]["matrix"], s["y"], act=_act_of(s), add=s.get("residual"))
+    elif kind == "conv8":
+        ien.conv8(ctx, s["q"], s["images"], s["height"], s["width"], s["layer"]["matrix"], s["y"], step=s["step"],
+                  act=_act_of(s), add=s.get("residual"))
+    else:
+        (g1, b1), (g2, b2) = s["norms"]
+        first, second = s["layers"]
+        shape = s["images"], s["height"], s["width"]
+        ien.group_norm(ctx, s["x"], s["images"], s["groups"], g1, b1, s["q"], eps=EPS, act=ien.ACT_SILU)
+        ien.conv8(ctx, s["q"], *shape, first["matrix"], s["h"])
+        ien.group_norm(ctx, s["h"], s["images"], s["groups"], g2, b2, s["q"], eps=EPS, act=ien.ACT_SILU)
+        ien.conv8(ctx, s["q"], *shape, second["matrix"], s["y"], add=s["x"])
+    return s["y"]
+
+
+def _run_plain(s):
+    kind = s["kind"]
+    if kind in ("norm", "norm8"):
+        y = _norm(s["x"].float(), s["images"], s["c"], s["groups"], s["gamma"], s["beta"], s["act"]).reshape(-1, s["c"])
+        return y.to(TYPES[s["outof"]]) if kind == "norm" else _values(*_quantize(y), s["c"]).half()
+    if kind == "quant":
+        return _values(*_quantize(s["x"].float()), s["k"])
+    if kind in ("rows8", "conv8"):
+        x = _values(s["q"], s["e"], s["k"] if kind == "rows8" else s["cin"])
+        if kind == "conv8":
+            x = _patches(x, s["images"], s["height"], s["width"], s["step"])
+        y = x @ s["layer"]["w"] + s["layer"]["b"]
+        return _act(y + s["residual"].float() if s["add"] else y, s["act"]).to(TYPES[s["outof"]])
+    y = s["x"]
+    shape = s["images"], s["height"], s["width"]
+
+    def half(y, gains, layer):
+        v = _norm(y.float(), s["images"], s["c"], s["groups"], *gains, "silu").reshape(-1, s["c"])
+        return _patches(_values(*_quantize(v), s["c"]), *shape, 1) @ layer["w"] + layer["b"]
+
+    y = half(y, s["norms"][0], s["layers"][0]).half()
+    return (s["x"].float() + half(y, s["norms"][1], s["layers"][1])).half()
+
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+# ---- the work, and the results in 64 bits ----------------------------------------
+
+
+def work(case):
+    kind, size = case["kind"], {"f16": 2, "f32": 4}
+    row8 = lambda k: k + _blocks(k)  # noqa: E731
+    if kind in ("norm", "norm8"):
+        n = case["images"] * case["height"] * case["width"] * case["c"]
+        return dict(bytes=n * (size[case["into"]] + size[case.get("outof", "f16")]) + 8 * case["c"], flops=8.0 * n)
+    if kind == "quant":
+        n = case["rows"] * case["k"]
+        return dict(bytes=n * (size[case["into"]] + 4), flops=4.0 * n)
+    if kind == "block":
+        p, c = case["images"] * case["height"] * case["width"], case["c"]
+        return dict(bytes=p * c * 4 + 2 * 9 * row8(c) * c + 24 * c, flops=2 * 2.0 * p * 9 * c * c + 16.0 * p * c)
+    if kind == "rows8":
+        taps, rows, outs, k, n = 1, case["rows"], case["rows"], case["k"], case["n"]
+    else:
+        taps, rows, k, n, t = 9, case["images"] * case["height"] * case["width"], case["cin"], case["cout"], case["step"]
+        outs = case["images"] * -(-case["height"] // t) * -(-case["width"] // t)
+    written = outs * n * size[case["outof"]] * (2 if case["add"] else 1)
+    return dict(bytes=rows * row8(k) + taps * row8(k) * n + 4 * n + written, flops=2.0 * outs * taps * k * n)
+
+
+def _exact_quantized(x):
+    """f64 rows rounded to the 8-bit values, from the definition: the power of two of each block of 128 by
+    comparing, the rounding by hand (a normal value has 4 significant bits, the smallest step is 2^-9)."""
+    rows, k = x.shape
+    out = torch.zeros_like(x)
+    for begin in range(0, k, BLOCK):
+        part = x[:, begin:begin + BLOCK]
+        largest = part.abs().max(1).values
+        e = torch.ceil(torch.log2(torch.where(largest > 0, largest, 1.0) / 448.0))
+        e = torch.where(largest > 448.0 * torch.exp2(e), e + 1, e)
+        e = torch.where(largest <= 448.0 * torch.exp2(e - 1), e - 1, e)
+        unit = torch.exp2(torch.where(largest > 0, e, 0.0))[:, None]
+        v = part / unit
+        _, exponent = torch.frexp(v)
+        step = torch.exp2((exponent - 4).clamp(min=-9).double())
+        out[:, begin:begin + BLOCK] = torch.round(v / step) * step * unit
+    return out
+
+
+def _exact_norm(x, images, groups, gamma, beta, act):
+    rows, c = x.shape
+    y = torch.empty(rows, c, dtype=torch.float64, device=x.device)
+    pixels, per = rows // images, c // groups
+    for i in range(images):
+        for j in range(groups):
+            at = slice(i * pixels, (i + 1) * pixels), slice(j * per, (j + 1) * per)
+            var, mean = torch.var_mean(x[at].double(), unbiased=False)
+            y[at] = (x[at].double() - mean) / torch.sqrt(var + EPS)
+    y = y * gamma.double() + beta.double()
+    return _exact_act(y, act)
+
+
+def _exact_act(y, act):
+    if act == "silu":
+        return y / (1 + torch.exp(-y))
+    if act == "gelu":
+        return y * torch.special.ndtr(y)
+    return y.clamp(min=0) if act == "relu" else y
+
+
+def _exact_product(x, w, taps, images=1, height=1, width=1, step=1):
+    """f64: rows x (their 8-bit values) with weights [taps c, n], 3 x 3 taps on the pixels of a map."""
+    c = x.shape[1]
+    w = torch.cat([_exact_quantized(w[t * c:(t + 1) * c].double().t().contiguous()).t() for t in range(taps)])
+    if taps == 1:
+        return x @ w
+    oh, ow = -(-height // step), -(-width // step)
+    x, y = x.reshape(images, height, width, c), torch.zeros(images, oh, ow, w.shape[1], dtype=torch.float64, device=x.device)
+    for t in range(9):
+        dy, dx = t // 3 - 1, t % 3 - 1
+        oys = [oy for oy in range(oh) if 0 <= oy * step + dy < height]
+        oxs = [ox for ox in range(ow) if 0 <= ox * step + dx < width]
+        if not oys or not oxs:
+            continue
+        a = x[:, oys[0] * step + dy:oys[-1] * step + dy + 1:step, oxs[0] * step + dx:oxs[-1] * step + dx + 1:step]
+        y[:, oys[0]:oys[-1] + 1, oxs[0]:oxs[-1] + 1] += a @ w[t * c:(t + 1) * c].contiguous()
+    return y.reshape(images * oh * ow, -1)
+
+
+def exact(case, seed):
+    kind = case["kind"]
+    if kind == "norm8":
+        # A value that 32 bits put on the other side of a border between two 8-bit values is off by a sixteenth of
+        # itself, on either side and however good the statistics are; a map of millions holds a few.
+        return None
+    g = torch.Generator(device=DEVICE)
+    g.manual_seed(seed)
+    if kind == "norm":
+        x = _features(g, case["images"] * case["height"] * case["width"], case["c"]).to(TYPES[case["into"]])
+        return _exact_norm(x, case["images"], case["groups"], *_gains(g, case["c"]), case["act"])
+    if kind == "quant":
+        return _exact_quantized(_features(g, case["rows"], case["k"]).to(TYPES[case["into"]]).double())
+
+    def layer(taps, c, n):
+        w = torch.randn(taps * c, n, generator=g, device=DEVICE) / math.sqrt(taps * c)
+        return w, 0.3 * torch.randn(n, generator=g, device=DEVICE).double()
+
+    if kind in ("rows8", "conv8"):
+        if kind == "rows8":
+            taps, rows, k, n, shape = 1, case["rows"], case["k"], case["n"], ()
+        else:
+            taps, k, n = 9, case["cin"], case["cout"]
+            shape = case["images"], case["height"], case["width"], case["step"]
+            rows = shape[0] * shape[1] * shape[2]
+        # (The activation of the inputs in 32 bits: it makes them, and is no part of the operator.)
+        x = _exact_quantized(_act(_features(g, rows, k), "silu").double())
+        w, b = layer(taps, k, n)
+        y = _exact_product(x, w, taps, *shape) + b
+        if case["add"]:
+            y += torch.randn(y.shape[0], n, generator=g, device=DEVICE).to(TYPES[case["outof"]]).double()
+        return _exact_act(y, case["act"])
+    c, shape = case["c"], (case["images"], case["height"], case["width"])
+    x = _features(g, shape[0] * shape[1] * shape[2], c).half()
+    norms, layers = [_gains(g, c), _gains(g, c)], [layer(9, c, c), layer(9, c, c)]
+    y = x
+    for gains, (w, b) in zip(norms, layers):
+        v = _exact_quantized(_exact_norm(y, shape[0], case["groups"], *gains, "silu"))
+        y = _exact_product(v, w, 9, *shape) + b
+        if w is layers[0][0]:
+            y = y.half()  # the map between the two halves is kept in f16
+    return x.double() + y
