@@ -1474,6 +1474,7 @@ ien_status ien_multiply_ex(ien_ctx *ctx, const ien_input *input, size_t row0, si
                            const ien_matrix *w, const ien_output *out, ien_act act,
                            const float *d_slope, int accumulate) {
   IEN_CHECK(ctx && out && out->data, IEN_ERR_INPUT, "null argument");
+  IEN_CHECK(act != IEN_ACT_SILU, IEN_ERR_INPUT, "f16 products take no SiLU");
   if (rows == 0) return IEN_OK;
   ConvCall c;
   ien_status s = describe(input, row0, rows, w, &c);

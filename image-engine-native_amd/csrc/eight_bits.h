@@ -1,0 +1,148 @@
+// eight_bits.h -- rows in 8 bits (ien_rows8) and weights in 8 bits, shared by
+// quantize8.hip, multiply8.hip and group_norm.hip (internal).
+#pragma once
+
+#include "conv_common.h"
+#include "lanes.h"
+
+// Weights in 8 bits: panel t cb + b (tap t, block b of 128 channels) holds
+// npad rows of 128 e4m3 bytes, an output each (zeros past c and n), and npad
+// scale dwords (the byte in the low 8 bits); npad is n in whole 128s.  A
+// tile's share of a panel is one contiguous piece.
+struct ien_matrix8 {
+  ien_ctx *ctx = nullptr;
+  size_t taps = 0, c = 0, n = 0;
+  int cb = 0;
+  long npad = 0;
+  uint8_t *d_w = nullptr;
+  uint32_t *d_scales = nullptr;
+  float *d_bias = nullptr;  // npad floats, zero padded
+};
+
+namespace ien {
+
+constexpr int BLOCK8 = 128;  // values under one scale
+
+inline size_t blocks8(size_t k) { return (k + BLOCK8 - 1) / BLOCK8; }
+
+// Rows in 8 bits that an entry point was handed, or its refusal.
+ien_status check_rows8(const ien_rows8 *r, size_t k, const char *what);
+
+typedef int int2v __attribute__((ext_vector_type(2)));
+
+// The exponent of a block whose largest finite magnitude is `largest`: the
+// smallest e >= -127 with largest <= 448 2^e = 1.75 2^(e + 8), 0 for zero.
+__device__ __forceinline__ int exponent8(float largest) {
+  const uint32_t b = __float_as_uint(largest);
+  const int e = (int)(b >> 23) - 135 + ((b & 0x7fffff) > 0x600000 ? 1 : 0);
+  return b == 0 ? 0 : e < -127 ? -127 : e;
+}
+
+// 2^-e for the e that exponent8 gives (-127 .. 120): a normal f32.
+__device__ __forceinline__ float inverse_power(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }
+
+// 2^(scale - 127) for scales 0 .. 254.
+__device__ __forceinline__ float scale_power(int scale) {
+  return __uint_as_float(scale == 0 ? 0x00400000u : (uint32_t)scale << 23);
+}
+
+__device__ __forceinline__ bool finite8(float v) { return (__float_as_uint(v) & 0x7f800000) != 0x7f800000; }
+__device__ __forceinline__ float finite_magnitude(float v) { return finite8(v) ? fabsf(v) : 0.0f; }
+
+// Eight values times the power of two `inv` as e4m3 bytes, to nearest even
+// (finite ones are within 448 by the block's scale; others become NaN).
+__device__ __forceinline__ int2v pack8(const float *v, float inv) {
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) s[i] = finite8(v[i]) ? v[i] * inv : __uint_as_float(0x7fc00000);
+  int2v r;
+  r.x = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+  r.x = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], r.x, true);
+  r.y = __builtin_amdgcn_cvt_pk_fp8_f32(s[4], s[5], 0, false);
+  r.y = __builtin_amdgcn_cvt_pk_fp8_f32(s[6], s[7], r.y, true);
+  return r;
+}
+
+// The largest of v over each aligned group of 16 lanes, in all of them.
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp_from<0xB1>(v));
+  v = fmaxf(v, dpp_from<0x4E>(v));
+  v = fmaxf(v, dpp_from<0x141>(v));
+  return fmaxf(v, dpp_from<0x140>(v));
+}
+
+// Eight consecutive values from channel `at` of a row of c (T: f16 or f32),
+// zeros past c; VEC: the whole eight in 16-byte loads.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *row, long at, long c, float *v) {
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 2) {
+      const half8 h = *(const half8 *)(row + at);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = (float)h[i];
+    } else {
+      const float4v a = *(const float4v *)(row + at), b = *(const float4v *)(row + at + 4);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = at + i < c ? (float)row[at + i] : 0.0f;
+  }
+}
+
+// Their counterpart: f16 rounds to nearest even.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T *row, long at, long c, const float *v) {
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 2) {
+      half8 h;
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[i] = (_Float16)v[i];
+      *(half8 *)(row + at) = h;
+    } else {
+      *(float4v *)(row + at) = float4v{v[0], v[1], v[2], v[3]};
+      *(float4v *)(row + at + 4) = float4v{v[4], v[5], v[6], v[7]};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (at + i < c) row[at + i] = (T)v[i];
+  }
+}
+
+// Whether rows of `c` values of `bytes` each, `stride` apart, go in whole
+// eights through 16-byte accesses.
+inline bool whole_eights(const void *p, size_t c, size_t stride, size_t bytes) {
+  return c % 8 == 0 && stride * bytes % 16 == 0 && ((uintptr_t)p & 15) == 0;
+}
+
+inline bool act8_known(ien_act act) {
+  return act == IEN_ACT_NONE || act == IEN_ACT_RELU || act == IEN_ACT_GELU || act == IEN_ACT_SIGMOID ||
+         act == IEN_ACT_SILU;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act8(float v) {
+  if constexpr (ACT == IEN_ACT_SILU) return v * sigmoid_f(v);
+  else if constexpr (ACT == IEN_ACT_RELU) return v < 0.0f ? 0.0f : v;  // (a NaN stays one)
+  else return act_c<ACT>(v, 0.0f);
+}
+
+// f(Act<...>) with the activation as a compile-time choice.
+template <int A>
+struct Act {
+  static constexpr int value = A;
+};
+template <typename F>
+__device__ __forceinline__ void with_act8(int act, F f) {
+  switch (act) {
+    case IEN_ACT_RELU: f(Act<IEN_ACT_RELU>{}); break;
+    case IEN_ACT_GELU: f(Act<IEN_ACT_GELU>{}); break;
+    case IEN_ACT_SIGMOID: f(Act<IEN_ACT_SIGMOID>{}); break;
+    case IEN_ACT_SILU: f(Act<IEN_ACT_SILU>{}); break;
+    default: f(Act<IEN_ACT_NONE>{}); break;
+  }
+}
+
+}  // namespace ien

@@ -19,7 +19,7 @@ PAD_ZERO, PAD_REFLECT = 0, 1
 TAPS_CONV, TAPS_OFFSETS = 0, 1
 INPUT_ROWS, INPUT_IMAGE = 0, 1
 NHWC, NCHW = 0, 1
-ACT_NONE, ACT_RELU, ACT_GELU, ACT_PRELU, ACT_SIGMOID = range(5)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_PRELU, ACT_SIGMOID, ACT_SILU = range(6)
 OUT_F16, OUT_F32 = 0, 1
 MODEL_REALESRGAN, MODEL_SCUNET, MODEL_LAMA, MODEL_BIREFNET = 0, 1, 2, 3
 
@@ -42,6 +42,8 @@ EXPORTS = (
     "ien_fourier_new", "ien_fourier_free", "ien_fourier_half", "ien_fourier_forward",
     "ien_fourier_inverse", "ien_spectral_new", "ien_spectral_free", "ien_spectral_work",
     "ien_spectral_run",
+    "ien_rows8_stride", "ien_rows8_scale_stride", "ien_quantize8", "ien_dequantize8", "ien_matrix8_new",
+    "ien_matrix8_free", "ien_multiply8", "ien_group_norm", "ien_group_norm8",
 )
 
 
@@ -96,6 +98,18 @@ class Output(ctypes.Structure):
         ("layout", ctypes.c_int),
         ("type", ctypes.c_int),
     ]
+
+
+class Rows8Struct(ctypes.Structure):
+    """ien_rows8."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_size_t), ("scales", ctypes.c_void_p),
+                ("scale_stride", ctypes.c_size_t)]
+
+
+class Input8(ctypes.Structure):
+    """ien_input8."""
+    _fields_ = [("kind", ctypes.c_int), ("map", Rows8Struct), ("images", ctypes.c_size_t),
+                ("height", ctypes.c_size_t), ("width", ctypes.c_size_t), ("step", ctypes.c_size_t)]
 
 
 class Tensor(ctypes.Structure):
@@ -200,6 +214,19 @@ def load():
         L.ien_spectral_work.argtypes = [vp]
         L.ien_spectral_work.restype = sz
         L.ien_spectral_run.argtypes = [vp, vp, sz, vp, vp, vp, vp, vp, vp, sz]
+        rp, fl = ctypes.POINTER(Rows8Struct), ctypes.c_float
+        L.ien_rows8_stride.argtypes = [sz]
+        L.ien_rows8_stride.restype = sz
+        L.ien_rows8_scale_stride.argtypes = [sz]
+        L.ien_rows8_scale_stride.restype = sz
+        L.ien_quantize8.argtypes = [vp, vp, i, sz, sz, sz, rp]
+        L.ien_dequantize8.argtypes = [vp, rp, sz, sz, vp, i, sz]
+        L.ien_matrix8_new.argtypes = [vp, vp, i, sz, sz, sz, vp, ctypes.POINTER(vp)]
+        L.ien_matrix8_free.argtypes = [vp]
+        L.ien_matrix8_free.restype = None
+        L.ien_multiply8.argtypes = [vp, ctypes.POINTER(Input8), sz, sz, vp, ctypes.POINTER(Output), i, vp, sz]
+        L.ien_group_norm.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, vp, i, sz]
+        L.ien_group_norm8.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, rp]
         for name in EXPORTS:
             getattr(L, name)
         _lib = L
@@ -552,6 +579,142 @@ class Swin:
             self.free()
         except Exception:
             pass
+
+
+class Rows8:
+    """ien_rows8 over torch tensors: `rows` rows of k values in 8 bits (data:
+    uint8 [rows, stride], scales: uint8 [rows, scale_stride]), made here
+    unless given.  Row i of `row0 = i` views starts there."""
+
+    def __init__(self, rows, k, data=None, scales=None, device="cuda"):
+        import torch
+
+        L = load()
+        if data is None:
+            data = torch.empty(rows, L.ien_rows8_stride(k), dtype=torch.uint8, device=device)
+        if scales is None:
+            scales = torch.empty(rows, L.ien_rows8_scale_stride(k), dtype=torch.uint8, device=data.device)
+        for t in (data, scales):
+            if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise ValueError("rows in 8 bits are uint8 tensors of rows x bytes")
+        self.rows, self.k, self.data, self.scales = rows, k, data, scales
+
+    def struct(self):
+        s = Rows8Struct(self.data.data_ptr(), _row_stride(self.data), self.scales.data_ptr(), _row_stride(self.scales))
+        s._tensors = self.data, self.scales  # raw pointers: keep their storage alive
+        return s
+
+
+def _row_stride(t):
+    """Elements between the rows of a 2-D tensor with contiguous rows (one row: its length)."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("rows x channels with contiguous channels expected")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _out_type(t):
+    import torch
+
+    if t.dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"f16 or f32 expected, not {t.dtype}")
+    return OUT_F16 if t.dtype == torch.float16 else OUT_F32
+
+
+def quantize8(ctx, x, out):
+    """Rows x k (f16 or f32 tensor) into the Rows8 `out`."""
+    if tuple(x.shape) != (out.rows, out.k):
+        raise ValueError(f"{tuple(x.shape)} into {out.rows} rows of {out.k}")
+    check(load().ien_quantize8(ctx.h, _ptr(x), _out_type(x), out.rows, out.k, _row_stride(x),
+                               ctypes.byref(out.struct())))
+
+
+def dequantize8(ctx, x, y):
+    """The values of the Rows8 `x` into the rows x k tensor y (f16 or f32)."""
+    if tuple(y.shape) != (x.rows, x.k):
+        raise ValueError(f"{x.rows} rows of {x.k} into {tuple(y.shape)}")
+    check(load().ien_dequantize8(ctx.h, ctypes.byref(x.struct()), x.rows, x.k, _ptr(y), _out_type(y),
+                                 _row_stride(y)))
+
+
+class Matrix8:
+    """ien_matrix8: host weights (taps c) x n (numpy f32 or f16) + bias in 8 bits."""
+
+    def __init__(self, ctx, w, bias=None, taps=1):
+        import numpy as np
+
+        w = np.ascontiguousarray(w)
+        wtype = W_F16 if w.dtype == np.float16 else W_F32
+        if wtype == W_F32:
+            w = np.ascontiguousarray(w, dtype=np.float32)
+        k, n = w.shape
+        if k % taps:
+            raise ValueError(f"{k} rows of weights in {taps} taps")
+        b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+        if b is not None and b.shape != (n,):
+            raise ValueError(f"{b.shape} biases for {n} outputs")
+        h = ctypes.c_void_p()
+        check(load().ien_matrix8_new(ctx.h, _np_ptr(w), wtype, taps, k // taps, n, None if b is None else _np_ptr(b),
+                                     ctypes.byref(h)))
+        self.h, self.taps, self.c, self.n, self.ctx = h, taps, k // taps, n, ctx
+
+    def free(self):
+        if self.h:
+            load().ien_matrix8_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _multiply8(ctx, inp, row0, rows, c, matrix, out, act, add):
+    if c != matrix.c or tuple(out.shape) != (rows, matrix.n):
+        raise ValueError(f"rows of {c} by {matrix.c} x {matrix.n} into {tuple(out.shape)}")
+    if add is not None and (add.shape != out.shape or add.dtype != out.dtype):
+        raise ValueError("what is added has the output's shape and type")
+    o = Output(out.data_ptr(), _row_stride(out), NHWC, _out_type(out))
+    check(load().ien_multiply8(ctx.h, ctypes.byref(inp), row0, rows, matrix.h, ctypes.byref(o), act, _ptr(add),
+                               0 if add is None else _row_stride(add)))
+
+
+def multiply8(ctx, x, matrix, out, act=ACT_NONE, add=None, row0=0):
+    """out = act(x . w + bias + add): rows row0 .. of the Rows8 x, as many as
+    out (rows x n, f16 or f32) has; `add` like out, or out itself."""
+    if row0 + out.shape[0] > x.rows:
+        raise ValueError(f"rows {row0} .. {row0 + out.shape[0]} of {x.rows}")
+    _multiply8(ctx, Input8(INPUT_ROWS, x.struct(), 1, 1, x.rows, 1), row0, out.shape[0], x.k, matrix, out, act, add)
+
+
+def conv8(ctx, x, images, height, width, matrix, out, step=1, act=ACT_NONE, add=None, row0=0):
+    """The same for a 3 x 3 (9 taps) or 1 x 1 convolution of `images` maps of
+    height x width pixels in 8 bits, zero padding: output pixels row0 .., as
+    many as out has rows."""
+    if images * height * width != x.rows:
+        raise ValueError(f"{images} maps of {height} x {width} in {x.rows} rows")
+    _multiply8(ctx, Input8(INPUT_IMAGE, x.struct(), images, height, width, step), row0, out.shape[0], x.k, matrix, out,
+               act, add)
+
+
+def group_norm(ctx, x, images, groups, gamma, beta, y, eps=1e-5, act=ACT_NONE):
+    """act(group norm) of `images` maps of x.shape[0] / images pixels (x: rows x
+    channels, f16 or f32) into y: a tensor of x's shape (f16 or f32, x itself
+    too), or a Rows8.  gamma, beta: f32 tensors, or None for 1 and 0."""
+    rows, c = x.shape
+    if images < 1 or rows % images:
+        raise ValueError(f"{rows} pixels in {images} maps")
+    for t in (gamma, beta):
+        if t is not None and (tuple(t.shape) != (c,) or str(t.dtype) != "torch.float32" or t.stride(0) != 1 and c > 1):
+            raise ValueError(f"gamma and beta are {c} contiguous f32 values")
+    args = (ctx.h, _ptr(x), _out_type(x), images, rows // images, c, _row_stride(x), groups, _ptr(gamma), _ptr(beta),
+            eps, act)
+    if (y.rows, y.k) != (rows, c) if isinstance(y, Rows8) else tuple(y.shape) != (rows, c):
+        raise ValueError("the result has the input's rows and channels")
+    if isinstance(y, Rows8):
+        check(load().ien_group_norm8(*args, ctypes.byref(y.struct())))
+    else:
+        check(load().ien_group_norm(*args, _ptr(y), _out_type(y), _row_stride(y)))
 
 
 def bytes_to_floats(ctx, src, dst):

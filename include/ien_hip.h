@@ -100,7 +100,8 @@ typedef enum {
   IEN_ACT_RELU = 1,
   IEN_ACT_GELU = 2,
   IEN_ACT_PRELU = 3,
-  IEN_ACT_SIGMOID = 4
+  IEN_ACT_SIGMOID = 4,
+  IEN_ACT_SILU = 5 /* v sigmoid(v): ien_group_norm{,8} and ien_multiply8 only */
 } ien_act;
 
 /* The left operand of a product (gemm.rs:289-304).  `data` is device f16.
@@ -224,6 +225,90 @@ ien_status ien_normalize_bytes(ien_ctx *ctx, const uint8_t *d_rgb, size_t pixels
  * pixel). */
 ien_status ien_composite_bytes(ien_ctx *ctx, const uint8_t *d_rgb, const uint8_t *d_mask,
                                const float *d_pred, size_t pixels, uint8_t *d_out);
+
+/* ---- rows in 8 bits, their products, and group norm --------------------
+ * No counterpart in the reference: the steps of the residual blocks of image
+ * decoders and U-Nets, x + conv(act(norm(x))), with the convolution's
+ * operands in 8 bits (OCP e4m3) and a power-of-two scale for each block of
+ * 128 values, which the matrix instructions apply.  c, k and n are any sizes;
+ * multiples of 128 (c, k) and of 8 (n, strides) waste nothing. */
+
+/* Rows of k values in 8 bits, device memory.  Row r is ceil(k / 128) blocks
+ * of 128 bytes from data + r * stride, zeros past k, and a scale byte a block
+ * from scales + r * scale_stride: block b stands for e4m3 x 2^(scale - 127),
+ * scales 0 .. 254.  data is 16-byte aligned, scales 4-byte, stride a multiple
+ * of 16, scale_stride of 4; ien_rows8_stride and ien_rows8_scale_stride give
+ * the smallest for k. */
+typedef struct {
+  uint8_t *data;
+  size_t stride;
+  uint8_t *scales;
+  size_t scale_stride;
+} ien_rows8;
+size_t ien_rows8_stride(size_t k);       /* 128 ceil(k / 128) */
+size_t ien_rows8_scale_stride(size_t k); /* 4 ceil(k / 512) */
+
+/* Rows of k values (f16 or f32 by `type`, `stride` elements apart) in 8 bits:
+ * a block's scale is the smallest 2^e (e >= -127) that keeps its largest
+ * finite magnitude at most 448 2^e, 1 for a block of zeros; values are
+ * rounded to nearest even.  Infinities and NaN become NaN and do not count
+ * into the scale. */
+ien_status ien_quantize8(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t rows, size_t k,
+                         size_t stride, const ien_rows8 *out);
+/* The values that rows in 8 bits stand for, as f16 or f32 rows `stride`
+ * elements apart (f32 holds each exactly; f16 rounds to nearest even, past
+ * 65504 to infinity). */
+ien_status ien_dequantize8(ien_ctx *ctx, const ien_rows8 *x, size_t rows, size_t k, void *d_y,
+                           ien_out_type type, size_t stride);
+
+/* Weights in 8 bits: row-major (taps c) x n host weights (f32, or f16 bits),
+ * taps 1 or 9 (3 x 3, row-major), channels c fastest, plus an optional
+ * length-n host bias (kept in f32).  Quantised once, on the device, with a
+ * scale for each 128 channels of a tap and output, as ien_quantize8 does. */
+typedef struct ien_matrix8 ien_matrix8;
+ien_status ien_matrix8_new(ien_ctx *ctx, const void *w, ien_wtype wtype, size_t taps, size_t c,
+                           size_t n, const float *bias, ien_matrix8 **out);
+void ien_matrix8_free(ien_matrix8 *m);
+
+/* The left operand of ien_multiply8: rows of c values in 8 bits.
+ * ROWS: the rows themselves (height, width, images and step unused; taps 1).
+ * IMAGE: `images` maps of height x width pixels, one row a pixel, one map
+ * after the other; output pixel (y, x) is centred on input pixel
+ * (step y, step x), step 1 or 2, zeros past the edge; 1 or 9 taps. */
+typedef struct {
+  ien_input_kind kind;
+  ien_rows8 map;
+  size_t images, height, width, step;
+} ien_input8;
+
+/* out[r] = act(input[r] . w + bias + add[r]) for rows row0 .. row0 + rows of
+ * the input (IMAGE: of its output pixels, images x ceil(height / step) x
+ * ceil(width / step)), into f16 or f32 NHWC rows `out->stride` elements apart
+ * (row row0 at out->data; add's rows likewise).  Sums are f32, rounded once.
+ * d_add (or NULL): rows of out's type, add_stride elements apart; it may be
+ * out->data itself, with its stride, which accumulates.  act: NONE, RELU,
+ * GELU, SIGMOID or SILU.  out overlaps neither the input nor, otherwise, add. */
+ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *input, size_t row0, size_t rows,
+                         const ien_matrix8 *w, const ien_output *out, ien_act act,
+                         const void *d_add, size_t add_stride);
+
+/* Group norm with an activation, channels last: `images` maps of `pixels`
+ * rows of c values (f16 or f32 by `type`, `stride` elements apart, c at most
+ * 8192), each normalised over all its pixels and a group's c / groups
+ * consecutive channels (f32 statistics of the deviations from the mean, the
+ * variance over n), y = act((x - mean) / sqrt(variance + eps) gamma[c] +
+ * beta[c]) with gamma and beta device f32 (NULL: 1 and 0).  y: f16 or f32
+ * rows, y_stride elements apart; it may be d_x itself with its type and
+ * stride.  act: NONE, RELU, GELU, SIGMOID or SILU. */
+ien_status ien_group_norm(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t images,
+                          size_t pixels, size_t c, size_t stride, size_t groups,
+                          const float *d_gamma, const float *d_beta, float eps, ien_act act,
+                          void *d_y, ien_out_type y_type, size_t y_stride);
+/* The same into rows in 8 bits, as ien_quantize8 of the f32 results. */
+ien_status ien_group_norm8(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t images,
+                           size_t pixels, size_t c, size_t stride, size_t groups,
+                           const float *d_gamma, const float *d_beta, float eps, ien_act act,
+                           const ien_rows8 *out);
 
 /* ---- resampling and padding ------------------------------------------- */
 
