@@ -14,6 +14,16 @@
 // output's own rounding, and as much as f32 outputs would be off in all.
 // Those take their operands as bf16, which holds e4m3 values under any of the
 // scales exactly, and the bf16 instructions (6e-9), at half the rate.
+//
+// A workgroup of four waves computes a tile of rows x outputs, a block of 128
+// deep at a time through a ring of stages in LDS that buffer loads fill without
+// registers; the 3 x 3 taps are the blocks' order, each lane's row at the tap's
+// pixel or, off the map, past the buffer's end.  What bounds it is the way into
+// LDS: some 65 KB a us and CU whatever the tile, so the largest tile (256 x
+// 256, 66 KB a block for 1.45 us of matrix time) is the fastest, and smaller
+// ones are for what would leave CUs idle.  8192 x 8192 -> 8192: 411 us, 2.67
+// PFLOP/s, 16384 rows 2048 -> 8192 262 us (of it 60 the writing of the result,
+// in step on all CUs); a wave a 32 x 32 tile straight from memory took 2040.
 
 #include "eight_bits.h"
 
@@ -39,6 +49,10 @@ struct Args8 {
   int f32, act;
   const void *add;
   long as;
+  int image, vec;  // a map's pixels; whole eights of the output (and of add)
+  int tiles_m, tiles_n, ksplit, kchunks;
+  float *part;
+  int *tile_count;
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -53,62 +67,407 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A wave 32 rows x 32 outputs.  The weights are the A operand: a lane gets
-// one row's results, four consecutive outputs at a time.
-__global__ __launch_bounds__(256) void k_multiply8(Args8 a) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
-  const long n0 = ((long)blockIdx.x * 4 + threadIdx.x / 64) * 32;
-  if (n0 >= a.npad) return;
-  const long r = (long)blockIdx.y * 32 + l32;
-  const bool live = r < a.rows;
-  const long p = a.row0 + (live ? r : 0), image = p / (a.OH * a.OW), q = p - image * a.OH * a.OW;
-  const long oy = q / a.OW, ox = q - oy * a.OW;
-  floatx16 acc = {};
-  for (int t = 0; t < a.taps; t++) {
-    const long iy = oy * a.step + (a.taps == 9 ? t / 3 - 1 : 0), ix = ox * a.step + (a.taps == 9 ? t % 3 - 1 : 0);
-    const bool in = live && iy >= 0 && iy < a.H && ix >= 0 && ix < a.W;
-    const long pixel = in ? (image * a.H + iy) * a.W + ix : 0;
-    const uint8_t *x = a.x + pixel * a.xs;
-    for (int b = 0; b < a.cb; b++) {
-      const long panel = ((long)t * a.cb + b) * a.npad + n0 + l32;
-      const int sx = in ? a.scales[pixel * a.ss + b] : 127, sw = (int)a.ws[panel];
+// A tile of a launch: FM x FN blocks of 32 rows x 32 outputs a wave, WM x WN
+// waves, a ring of S stages in LDS, each a block of 128 deep of the tile's
+// rows and weights and their scales.
+template <int FM_, int FN_, int WM_, int WN_, int S_>
+struct Tile8 {
+  static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, S = S_;
+  static constexpr int TM = 32 * FM * WM, TN = 32 * FN * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int B0 = TM * BLOCK8, SX0 = B0 + TN * BLOCK8, SW0 = SX0 + TM * 4;
+  static constexpr int A_LOADS = TM / 8 / WAVES, B_LOADS = TN / 8 / WAVES;  // a wave and stage, 1 KiB each
+  static constexpr int S_PIECES = (TM + TN) / 64, S_LOADS = (S_PIECES + WAVES - 1) / WAVES;  // 256 bytes each
+  static constexpr int STAGE = SX0 + WAVES * S_LOADS * 256;
+  static constexpr int LOADS = A_LOADS + B_LOADS + S_LOADS;
+  static constexpr int PITCH = 32 * FN + 4;  // floats between the epilogue's rows
+  static constexpr int STAGING = WM * WN * 32 * PITCH * 4;
+  static constexpr int BIAS0 = S * STAGE > STAGING ? S * STAGE : STAGING;
+  static constexpr int LDS = BIAS0 + TN * 4;
+  static_assert(A_LOADS * 8 * WAVES == TM && B_LOADS * 8 * WAVES == TN, "loads a wave");
+};
+
+constexpr int NOWHERE = 0x7ffffff0;  // past every buffer: reads zeros
+
+// dma_lds and dma_lds4 with the LDS place as a wave's base and a constant,
+// and a uniform offset `soff` beside the lane's (which alone is checked
+// against the buffer's end).
+template <int CONST>
+__device__ __forceinline__ void dma16_at(int4v rsrc, unsigned wave_base, int off) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+               :: "s"(wave_base), "n"(CONST), "v"(off), "s"(rsrc) : "memory", "m0", "scc");
+}
+template <int CONST>
+__device__ __forceinline__ void dma4_at(int4v rsrc, unsigned wave_base, int off, int soff) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds"
+               :: "s"(wave_base), "n"(CONST), "v"(off), "s"(rsrc), "s"(soff) : "memory", "m0", "scc");
+}
+
+// How many of n things are done before step k of `steps`.
+constexpr int share8(int k, int n, int steps) { return k >= steps ? n : k * n / steps; }
+
+// f(Const<0>) .. f(Const<N - 1>).
+template <int V>
+struct Const {
+  static constexpr int value = V;
+  constexpr operator int() const { return V; }
+};
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (I < N) {
+    f(Const<I>{});
+    each<N, I + 1>(f);
+  }
+}
+
+template <typename T, bool F32>
+__global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8(Args8 a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % T::WM, wn = wave / T::WM;
+
+  // Each XCD a band of the tiles, in groups of 8 row tiles: neighbours share rows and weights.
+  const int tiles = gridDim.x, xcd = blockIdx.x & 7, full = tiles >> 3, rest = tiles & 7;
+  const int at = xcd * full + min(xcd, rest) + (blockIdx.x >> 3);
+  const int group = at / (8 * a.tiles_n), gm = min(8, a.tiles_m - 8 * group), in_group = at - group * 8 * a.tiles_n;
+  const long m0 = (long)(8 * group + in_group % gm) * T::TM;
+  const long n0 = (long)(in_group / gm) * T::TN;
+
+  // Where the tile's first row lies, and the others relative to it.
+  long oy0 = 0, ox0 = a.row0 + m0, first = ox0;
+  if (a.image) {
+    const long p = a.row0 + m0, im = p / (a.OH * a.OW), q = p - im * a.OH * a.OW;
+    oy0 = q / a.OW;
+    ox0 = q - oy0 * a.OW;
+    first = (im * a.H + oy0 * a.step) * a.W + ox0 * a.step;
+  }
+  // Row r of the tile: its pixel after the first one's, and a bit for each
+  // tap that falls on the map.
+  auto place = [&](int r, int *pixel) {
+    *pixel = r;
+    if (m0 + r >= a.rows) return 0;
+    if (!a.image) return 1;
+    const unsigned x = (unsigned)ox0 + r, down = x / (unsigned)a.OW, ox = x - down * (unsigned)a.OW;
+    const unsigned y = (unsigned)oy0 + down, maps = y / (unsigned)a.OH, oy = y - maps * (unsigned)a.OH;
+    *pixel = ((int)(maps * (unsigned)a.H) + ((int)oy - (int)oy0) * a.step) * (int)a.W + ((int)ox - (int)ox0) * a.step;
+    if (a.taps == 1) return 1;
+    const int iy = oy * a.step, ix = ox * a.step;
+    const int across = (ix > 0 ? 1 : 0) | 2 | (ix + 1 < a.W ? 4 : 0);
+    return (iy > 0 ? across : 0) | across << 3 | (iy + 1 < a.H ? across << 6 : 0);
+  };
+  int off[T::A_LOADS], mask[T::A_LOADS];
 #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        const int8v wv = *(const int8v *)(a.w + panel * 128 + s * 64 + hi * 32);
-        int8v xv = {};
-        if (in) {  // rows are 16-byte aligned only
-          u32x4 lo = *(const u32x4 *)(x + b * 128 + s * 64 + hi * 32), up = *(const u32x4 *)(x + b * 128 + s * 64 + hi * 32 + 16);
-          __builtin_memcpy(&xv, &lo, 16);
-          __builtin_memcpy((char *)&xv + 16, &up, 16);
-        }
-        if (!a.f32) {
-          acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, xv, acc, 0, 0, 0, sw, 0, sx);
-        } else {
-          const float fw = scale_power(sw), fx = scale_power(sx);
+  for (int i = 0; i < T::A_LOADS; i++) {
+    const int row = (wave + T::WAVES * i) * 8 + (lane >> 3);
+    mask[i] = place(row, &off[i]);
+    off[i] = off[i] * (int)a.xs + 16 * ((lane & 7) ^ (row & 7));
+  }
+  int soff[T::S_LOADS], smask[T::S_LOADS];
 #pragma unroll
-          for (int i = 0; i < 8; i += 2)
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen8(wv[i], wv[i + 1], fw), widen8(xv[i], xv[i + 1], fx),
-                                                          acc, 0, 0, 0);
-        }
+  for (int i = 0; i < T::S_LOADS; i++) {
+    const int piece = wave + T::WAVES * i;  // (past the scales: into the stage's spare lines)
+    smask[i] = piece < T::TM / 64 ? place(piece * 64 + lane, &soff[i]) : 0;
+    soff[i] = piece < T::TM / 64 ? soff[i] * (int)a.ss : (piece * 64 + lane - T::TM) * 4;
+  }
+
+  // The stream of blocks to load: addresses of the next one's rows and scales
+  // (of the tile's first row under the block's tap) and of its weights.
+  const int chunks = min(a.taps * a.cb - (int)blockIdx.y * a.kchunks, a.kchunks), c_begin = blockIdx.y * a.kchunks;
+  int tap = c_begin / a.cb, ib = c_begin - tap * a.cb, left = chunks;
+  int kx = a.taps == 9 ? tap % 3 : 0;
+  const long shift = a.taps == 9 ? (long)(tap / 3 - 1) * a.W + kx - 1 : 0;
+  long xat = (long)a.x + (first + shift) * a.xs + ib * BLOCK8, sat = (long)a.scales + (first + shift) * a.ss;
+  long wat = (long)a.w + ((long)c_begin * a.npad + n0) * BLOCK8, vat = (long)a.ws + ((long)c_begin * a.npad + n0) * 4;
+  const long across = a.xs - a.cb * BLOCK8, down = (a.W - 2) * a.xs - a.cb * BLOCK8, sdown = (a.W - 2) * a.ss;
+  const unsigned wave_lds = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
+  const unsigned wave_lds4 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 256);
+  int woff[T::B_LOADS];
+#pragma unroll
+  for (int i = 0; i < T::B_LOADS; i++) {
+    const int row = (wave + T::WAVES * i) * 8 + (lane >> 3);
+    woff[i] = row * BLOCK8 + 16 * ((lane & 7) ^ (row & 7));
+  }
+  // Load I of the block into stage STAGE, by this wave: first its rows, then
+  // its weights, then its scales.
+  auto load = [&](auto stage, auto I) {
+    constexpr int BASE = decltype(stage)::value * T::STAGE, i = decltype(I)::value;
+    const int all = left > 0 ? 0x7fffff00 : 0;  // (past the last block: zeros)
+    if constexpr (i < T::A_LOADS) {
+      // Off the map: past the end.
+      const int o = off[i] | (__builtin_amdgcn_sbfe(~mask[i], tap, 1) & 0x7fffff00);
+      dma16_at<BASE + T::WAVES * i * 1024>(uniform_rsrc((const void *)xat, all), wave_lds, o);
+    } else if constexpr (i < T::A_LOADS + T::B_LOADS) {
+      constexpr int k = i - T::A_LOADS;
+      dma16_at<BASE + T::B0 + T::WAVES * k * 1024>(uniform_rsrc((const void *)wat, all), wave_lds, woff[k]);
+    } else {
+      constexpr int k = i - T::A_LOADS - T::B_LOADS;
+      const int piece = wave + T::WAVES * k;
+      const bool rows = piece < T::TM / 64;
+      const int o = rows ? soff[k] | (__builtin_amdgcn_sbfe(~smask[k], tap, 1) & 0x7fffff00) : soff[k];
+      dma4_at<BASE + T::SX0 + T::WAVES * k * 256>(uniform_rsrc((const void *)(rows ? sat : vat), all), wave_lds4, o,
+                                                  rows ? ib & ~3 : 0);
+    }
+  };
+  auto advance = [&] {
+    left--;
+    xat += BLOCK8;
+    wat += a.npad * BLOCK8;
+    vat += a.npad * 4;
+    // (Without branches, which the products would be moved across.)
+    const int over = -(int)(++ib == a.cb), wrap = -(int)(kx == 2) & over;
+    ib &= ~over;
+    tap -= over;
+    kx = (kx - over) & ~wrap;
+    xat += (long)over & (wrap ? down : across);
+    sat += (long)over & (wrap ? sdown : a.ss);
+  };
+
+  // Half s of a block: 16-byte slots 4 s + 2 hi, + 1 of each row, at those
+  // places xor row % 8 (no two of eight neighbouring rows on one bank).
+  struct Half {
+    int8v x[T::FM], w[T::FN];
+  };
+  int place16[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) place16[k] = l32 * BLOCK8 + 16 * ((4 * (k >> 1) + 2 * hi + (k & 1)) ^ (l32 & 7));
+  const unsigned char *xp = lds + wm * T::FM * 32 * BLOCK8, *wp = lds + T::B0 + wn * T::FN * 32 * BLOCK8;
+  const unsigned char *sp = lds + T::SX0 + (wm * T::FM * 32 + l32) * 4, *vp = lds + T::SW0 + (wn * T::FN * 32 + l32) * 4;
+  // Fragment I of half s: the rows' first, then the weights'.
+  auto read = [&](Half &h, auto stage, auto s, auto I) {
+    constexpr int BASE = decltype(stage)::value * T::STAGE, i = decltype(I)::value, S = decltype(s)::value;
+    const unsigned char *p = i < T::FM ? xp + BASE + i * 32 * BLOCK8 : wp + BASE + (i - T::FM) * 32 * BLOCK8;
+    const int4v lo = *(const int4v *)(p + place16[2 * S]), up = *(const int4v *)(p + place16[2 * S + 1]);
+    const int8v v = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+    if constexpr (i < T::FM)
+      h.x[i] = v;
+    else
+      h.w[i - T::FM] = v;
+  };
+  struct Scales {
+    int x[T::FM], w[T::FN];
+  };
+  auto read_scales = [&](Scales &v, auto stage) {
+    constexpr int BASE = decltype(stage)::value * T::STAGE;
+#pragma unroll
+    for (int i = 0; i < T::FM; i++) v.x[i] = *(const int *)(sp + BASE + i * 128);
+#pragma unroll
+    for (int j = 0; j < T::FN; j++) v.w[j] = *(const int *)(vp + BASE + j * 128);
+  };
+  floatx16 acc[T::FM][T::FN] = {};
+  constexpr int PRODUCTS = T::FM * T::FN;
+  // The products of half a block, beside(k) between them.
+  auto multiply = [&](const Half &h, const Scales &v, auto beside) {
+    if constexpr (!F32) {
+      each<PRODUCTS>([&](auto k) {
+        constexpr int i = decltype(k)::value / T::FN, j = decltype(k)::value % T::FN;
+        beside(k);
+        __builtin_amdgcn_sched_barrier(0);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(h.w[j], h.x[i], acc[i][j], 0, 0, 0, v.w[j], 0, v.x[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    } else {
+      each<PRODUCTS>(beside);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        bf16x8 x[T::FM], w[T::FN];
+#pragma unroll
+        for (int i = 0; i < T::FM; i++) x[i] = widen8(h.x[i][e], h.x[i][e + 1], scale_power(v.x[i] & 255));
+#pragma unroll
+        for (int j = 0; j < T::FN; j++) w[j] = widen8(h.w[j][e], h.w[j][e + 1], scale_power(v.w[j]));
+#pragma unroll
+        for (int i = 0; i < T::FM; i++)
+#pragma unroll
+          for (int j = 0; j < T::FN; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[i][j], 0, 0, 0);
       }
     }
+  };
+
+  // Block c's second half is read while its first is multiplied.  Then every
+  // wave has read all of it, the next block has landed, and under the second
+  // half's products the next one's first half is read and the block S further
+  // loaded into this one's place.  (Blocks past the last are zeros.)
+  if (wave < T::TN / 64)  // the epilogue's biases
+    dma4_at<T::BIAS0>(uniform_rsrc((const void *)(a.bias + n0), (a.npad - n0) * 4), wave_lds4, (wave * 64 + lane) * 4, 0);
+  each<T::S>([&](auto stage) {
+    each<T::LOADS>([&](auto i) { load(stage, i); });
+    advance();
+  });
+  wait_vm<(T::S - 1) * T::LOADS>();
+  lds_barrier();
+  constexpr int FRAGS = T::FM + T::FN, EARLY = (PRODUCTS + 1) / 2;  // products among which the fragments are read
+  Half h0, h1;
+  Scales v[T::S];
+  int b = c_begin % a.cb;
+  each<FRAGS>([&](auto i) { read(h0, Const<0>{}, Const<0>{}, i); });
+  read_scales(v[0], Const<0>{});
+  auto align = [&](Scales &v) {
+#pragma unroll
+    for (int i = 0; i < T::FM; i++) v.x[i] >>= 8 * (b & 3);
+    b = b + 1 == a.cb ? 0 : b + 1;
+  };
+  // The products of `now` while half s of stage NEXT is read into `then`, and where `loads`, stage STAGE's next block loaded.
+  auto work = [&](const Half &now, const Scales &v, Half &then, auto next, auto s, auto stage, auto loads) {
+    multiply(now, v, [&](auto k) {
+      constexpr int K = decltype(k)::value, from = share8(K, FRAGS, EARLY), to = share8(K + 1, FRAGS, EARLY);
+      each<to - from>([&](auto i) { read(then, next, s, Const<from + decltype(i)::value>{}); });
+      if constexpr (decltype(loads)::value) {
+        constexpr int first = K * T::LOADS / PRODUCTS, last = (K + 1) * T::LOADS / PRODUCTS;
+        each<last - first>([&](auto i) { load(stage, Const<first + decltype(i)::value>{}); });
+      }
+    });
+  };
+  auto step = [&](auto stage) {
+    constexpr int s = decltype(stage)::value;
+    const Const<(s + 1) % T::S> next;
+    align(v[s]);
+    work(h0, v[s], h1, stage, Const<1>{}, stage, Const<0>{});
+    wait_vm<(T::S - 2) * T::LOADS>();
+    lds_barrier();
+    read_scales(v[next], next);
+    work(h1, v[s], h0, next, Const<0>{}, stage, Const<1>{});
+    advance();
+  };
+  int c = 0;
+  for (; c + T::S <= chunks; c += T::S) each<T::S>(step);
+  each<T::S - 1>([&](auto stage) {
+    if (c + decltype(stage)::value < chunks) step(stage);
+  });
+  wait_vm<0>();
+  __syncthreads();  // no load is on its way into LDS, every wave is done with the stages
+
+  if (a.ksplit > 1) {
+    ConvArgs split{};
+    split.part = a.part;
+    split.tile_count = a.tile_count;
+    split.ksplit = a.ksplit;
+    if (!count_in<T::FM, T::FN, T::THREADS>(split, acc, (int *)lds, tid)) return;
+    __syncthreads();
   }
-  if (!live) return;
+
+  // Each wave 32 of its rows at a time through LDS of its own, for whole lines
+  // out: eights of a row's outputs, always the same ones for a lane.
+  float *st = (float *)lds + wave * 32 * T::PITCH;
+  constexpr int COLS = 32 * T::FN, EIGHTS = COLS / 8, ITEMS = 32 * EIGHTS / 64;
+  const long nw = n0 + wn * COLS;
+  using Y = std::conditional_t<F32, float, _Float16>;
+  const int row = lane / EIGHTS, col = lane % EIGHTS * 8;
+  float bias[8];
+  load8<float, true>((const float *)(lds + T::BIAS0) + wn * COLS, col, 0, bias);
+  auto stage_rows = [&](const floatx16 (&v)[T::FN]) {
+#pragma unroll
+    for (int j = 0; j < T::FN; j++)
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        *(float4v *)(st + l32 * T::PITCH + 32 * j + 8 * q + 4 * hi) =
+            float4v{v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
+  };
   with_act8(a.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const long n = n0 + 8 * (i / 4) + 4 * hi + i % 4;
-      if (n >= a.n) continue;
-      float v = acc[i] + a.bias[n];
-      if (a.f32) {
-        if (a.add) v += ((const float *)a.add)[r * a.as + n];
-        ((float *)a.y)[r * a.ys + n] = act8<decltype(act)::value>(v);
+    for (int i = 0; i < T::FM; i++) {
+      const long r0 = m0 + (wm * T::FM + i) * 32;
+      if (a.vec) {
+        const bool in = nw + col < a.n;
+        Y *y = (Y *)a.y + (r0 + row) * a.ys + nw + col;
+        float old[ITEMS][8];
+        if (a.add) {
+          const Y *add = (const Y *)a.add + (r0 + row) * a.as + nw + col;
+#pragma unroll
+          for (int e = 0; e < ITEMS; e++)
+            if (in && r0 + row + e * (64 / EIGHTS) < a.rows) load8<Y, true>(add + e * (64 / EIGHTS) * a.as, 0, 0, old[e]);
+        }
+        stage_rows(acc[i]);
+#pragma unroll
+        for (int e = 0; e < ITEMS; e++) {
+          if (!in || r0 + row + e * (64 / EIGHTS) >= a.rows) continue;
+          float v[8];
+          load8<float, true>(st, (row + e * (64 / EIGHTS)) * T::PITCH + col, 0, v);
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[k] += bias[k];
+          if (a.add) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] += old[e][k];
+          }
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[k] = act8<decltype(act)::value>(v[k]);
+          store8<Y, true>(y + e * (64 / EIGHTS) * a.ys, 0, 0, v);
+        }
       } else {
-        if (a.add) v += (float)((const _Float16 *)a.add)[r * a.as + n];
-        ((_Float16 *)a.y)[r * a.ys + n] = (_Float16)act8<decltype(act)::value>(v);
+        stage_rows(acc[i]);
+        for (int e = lane; e < 32 * COLS; e += 64) {
+          const int r = e / COLS, c = e % COLS;
+          const long n = nw + c;
+          if (r0 + r >= a.rows || n >= a.n) continue;
+          float v = st[r * T::PITCH + c] + ((const float *)(lds + T::BIAS0))[wn * COLS + c];
+          if (a.add) v += (float)((const Y *)a.add)[(r0 + r) * a.as + n];
+          ((Y *)a.y)[(r0 + r) * a.ys + n] = (Y)act8<decltype(act)::value>(v);
+        }
       }
+      __builtin_amdgcn_wave_barrier();
     }
   });
+}
+
+struct Plan8 {
+  int tile, ksplit;
+  double us;
+};
+
+// The tiles a launch chooses among, largest first, and what they were measured
+// at: us a block of depth of one tile on a CU alone and among its neighbours,
+// and us a round of tiles for their outputs.
+struct Choice8 {
+  int tm, tn;
+  double alone, among, out;
+};
+constexpr Choice8 CHOICES8[] = {{256, 256, 1.45, 1.45, 8.0}, {128, 128, 0.58, 0.50, 3.0}, {64, 128, 0.42, 0.34, 1.7},
+                                {64, 64, 0.38, 0.22, 1.2}};
+
+template <typename T, bool F32>
+void launch(ien_ctx *ctx, Args8 &a) {
+  hipLaunchKernelGGL((k_tile8<T, F32>), dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)a.ksplit), dim3(T::THREADS), 0,
+                     ctx->stream, a);
+}
+
+// The tile, and in how many splits of the depth: by the estimated time.  Few
+// tiles leave CUs idle, which splits fill for a pass through device memory and
+// about 5 us; f32 outputs take twice the matrix time and no 256 x 256 tiles (their
+// operands as bf16 do not fit in registers beside the sums).
+Plan8 plan8(int cus, long workspace, long rows, long n, int chunks, bool f32, bool add) {
+  Plan8 best = {-1, 1, 1e30};
+  for (int t = f32 ? 1 : 0; t < 4; t++) {
+    const Choice8 &c = CHOICES8[t];
+    const long tiles = ((rows + c.tm - 1) / c.tm) * ((n + c.tn - 1) / c.tn);
+    for (int ks = 1; ks <= 16 && ks <= chunks; ks++) {
+      if (ks > 1 && (tiles * ks > 2 * cus || tiles > ien_ctx::SPLITK_TILES || tiles * ks * c.tm * c.tn > workspace)) break;
+      const int deep = (chunks + ks - 1) / ks;
+      if ((chunks + deep - 1) / deep != ks) continue;
+      const long rounds = (tiles * ks + cus - 1) / cus;
+      double us = (rounds == 1 ? c.alone : rounds * c.among) * deep * (f32 ? 1.5 : 1.0) + rounds * c.out * (add ? 2 : 1);
+      if (ks > 1) us += 5.0 + 1e-6 * (double)(tiles * ks) * c.tm * c.tn * 3;
+      if (us < best.us) best = {t, ks, us};
+    }
+  }
+  return best;
+}
+
+void run_tiles(ien_ctx *ctx, Args8 &a) {
+  const int chunks = a.taps * a.cb;
+  const Plan8 p = plan8(ctx->cus, (long)ctx->splitk_floats, a.rows, a.n, chunks, a.f32, a.add);
+  const Choice8 &c = CHOICES8[p.tile];
+  a.tiles_m = (int)((a.rows + c.tm - 1) / c.tm);
+  a.tiles_n = (int)((a.n + c.tn - 1) / c.tn);
+  a.ksplit = p.ksplit;
+  a.kchunks = (chunks + p.ksplit - 1) / p.ksplit;
+  a.part = ctx->splitk;
+  a.tile_count = (int *)(ctx->splitk + ctx->splitk_floats);
+  switch (p.tile) {
+    case 0: launch<Tile8<4, 4, 2, 2, 2>, false>(ctx, a); break;
+    case 1: a.f32 ? launch<Tile8<2, 2, 2, 2, 2>, true>(ctx, a) : launch<Tile8<2, 2, 2, 2, 2>, false>(ctx, a); break;
+    case 2: a.f32 ? launch<Tile8<1, 2, 2, 2, 3>, true>(ctx, a) : launch<Tile8<1, 2, 2, 2, 3>, false>(ctx, a); break;
+    default: a.f32 ? launch<Tile8<1, 1, 2, 2, 4>, true>(ctx, a) : launch<Tile8<1, 1, 2, 2, 4>, false>(ctx, a); break;
+  }
 }
 
 }  // namespace
@@ -170,9 +529,15 @@ ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *in, size_t row0, size_t
   a.act = act;
   a.add = d_add;
   a.as = (long)add_stride;
-  IEN_CHECK((rows + 31) / 32 < 65536, IEN_ERR_INPUT, "%zu rows", rows);
-  hipLaunchKernelGGL(k_multiply8, dim3((unsigned)(w->npad / 128), (unsigned)((rows + 31) / 32)), dim3(256), 0,
-                     ctx->stream, a);
+  a.image = in->kind == IEN_INPUT_IMAGE;
+  const size_t size = a.f32 ? 4 : 2;
+  a.vec = whole_eights(a.y, w->n, out->stride, size) && (!d_add || whole_eights(d_add, w->n, add_stride, size));
+  // A tile addresses its rows' values by 31-bit offsets from its first one's.
+  IEN_CHECK(in->map.stride < (1u << 20) && in->map.scale_stride < (1u << 20) &&
+                (!a.image || (in->width + 256) * std::max(in->map.stride, in->map.scale_stride) < (1u << 29)),
+            IEN_ERR_INPUT, "rows in 8 bits %zu and %zu bytes apart, %ld to a line of a map", in->map.stride,
+            in->map.scale_stride, a.W);
+  run_tiles(ctx, a);
   IEN_HIP(hipGetLastError());
   return IEN_OK;
 }
