@@ -74,17 +74,20 @@ __device__ __forceinline__ float max16(float v) {
   return fmaxf(v, dpp_from<0x140>(v));
 }
 
+typedef half8 half8_any __attribute__((aligned(2)));
+typedef float4v float4_any __attribute__((aligned(4)));
+
 // Eight consecutive values from channel `at` of a row of c (T: f16 or f32),
-// zeros past c; VEC: the whole eight in 16-byte loads.
+// zeros past c; VEC: the whole eight in 16-byte loads, at any element.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T *row, long at, long c, float *v) {
   if constexpr (VEC) {
     if constexpr (sizeof(T) == 2) {
-      const half8 h = *(const half8 *)(row + at);
+      const half8 h = *(const half8_any *)(row + at);
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = (float)h[i];
     } else {
-      const float4v a = *(const float4v *)(row + at), b = *(const float4v *)(row + at + 4);
+      const float4v a = *(const float4_any *)(row + at), b = *(const float4_any *)(row + at + 4);
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
     }
@@ -102,22 +105,16 @@ __device__ __forceinline__ void store8(T *row, long at, long c, const float *v) 
       half8 h;
 #pragma unroll
       for (int i = 0; i < 8; i++) h[i] = (_Float16)v[i];
-      *(half8 *)(row + at) = h;
+      *(half8_any *)(row + at) = h;
     } else {
-      *(float4v *)(row + at) = float4v{v[0], v[1], v[2], v[3]};
-      *(float4v *)(row + at + 4) = float4v{v[4], v[5], v[6], v[7]};
+      *(float4_any *)(row + at) = float4v{v[0], v[1], v[2], v[3]};
+      *(float4_any *)(row + at + 4) = float4v{v[4], v[5], v[6], v[7]};
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
       if (at + i < c) row[at + i] = (T)v[i];
   }
-}
-
-// Whether rows of `c` values of `bytes` each, `stride` apart, go in whole
-// eights through 16-byte accesses.
-inline bool whole_eights(const void *p, size_t c, size_t stride, size_t bytes) {
-  return c % 8 == 0 && stride * bytes % 16 == 0 && ((uintptr_t)p & 15) == 0;
 }
 
 inline bool act8_known(ien_act act) {
@@ -127,7 +124,8 @@ inline bool act8_known(ien_act act) {
 
 template <int ACT>
 __device__ __forceinline__ float act8(float v) {
-  if constexpr (ACT == IEN_ACT_SILU) return v * sigmoid_f(v);
+  if constexpr (ACT == IEN_ACT_SILU)
+    return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));  // (1 ulp; past e^88 the result is -0)
   else if constexpr (ACT == IEN_ACT_RELU) return v < 0.0f ? 0.0f : v;  // (a NaN stays one)
   else return act_c<ACT>(v, 0.0f);
 }

@@ -1,6 +1,22 @@
 // group_norm.hip -- group norm with an activation over channels-last maps
 // (ien_group_norm, ien_group_norm8): y = act((x - m) / sqrt(v + eps) gamma +
 // beta) with m and v over a map's pixels and a group's channels.
+//
+// A lane keeps eight consecutive channels of every px-th pixel, so a pixel is
+// read in 16-byte pieces whatever the groups, and holds a mean and the squares
+// of the deviations from it for each of its channels.  A batch of pixels in
+// registers gives both exactly as defined (first the mean, then the squares);
+// batches, lanes and workgroups join by
+//   m = m1 + d n2 / n,  q = q1 + q2 + d^2 n1 n2 / n,  d = m2 - m1, n = n1 + n2
+// (Chan, Golub and LeVeque), which cancels nothing, wherever the mean lies, and
+// channels of a group by the same with equal counts.  The order is fixed by the
+// sizes alone.
+//
+// Memory bounds it: x is read for the statistics, read again and y written.  The
+// two passes share a split of the pixels, and the second takes each part from
+// its end, so that some of it is still in the L2 of its XCD; the rest comes from
+// the memory-side cache where x fits that.  Maps whose blocks of channels fit in a
+// workgroup's registers take one launch and are read once.
 
 #include "eight_bits.h"
 
@@ -9,7 +25,7 @@ namespace {
 
 struct NormArgs {
   const void *x;
-  long images, pixels, stride;
+  long pixels, stride;
   int c, groups, act;
   const float *gamma, *beta;
   float eps;
@@ -17,97 +33,353 @@ struct NormArgs {
   long ystride;
   uint8_t *scales;
   long scale_stride;
+  int span;     // channels a workgroup handles (c, or a part in one launch)
+  int chunks;   // parts of an image's pixels
+  long chunk;   // pixels of a part
+  float2 *part;  // [image][chunk][group]: mean and squares
 };
 
-template <int N>
-__device__ float block_sum(float v, float *lds) {
-  v = group_sum<64>(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N / 64; i++) s += lds[i];
-  return s;
-}
+constexpr int LANES = 1024;  // of a workgroup
 
-// A workgroup an image and group: the mean, then the squares of the
-// deviations from it.
+struct Shared {
+  float m[8 * LANES], q[8 * LANES], n[LANES];  // [channel of the eight][lane]
+};
+
+// (m1, q1) of n1 joined with (m2, q2): w = n2 / (n1 + n2), nw = n1 w.
+__device__ __forceinline__ void join(float &m1, float &q1, float m2, float q2, float w, float nw) {
+  const float d = m2 - m1;
+  m1 += d * w;
+  q1 += q2 + d * d * nw;
+}
+// n2 / n (1 ulp: where both means agree it does not matter).
+__device__ __forceinline__ float share(float n2, float n) { return n > 0.0f ? n2 * __builtin_amdgcn_rcpf(n) : 0.0f; }
+
+// `eights` lanes a pixel, px pixels side by side.
+struct Place {
+  int eights, px, slot, eight;
+  __device__ Place(int span, int round) {
+    eights = (span / 8 + (span % 8 != 0) + round - 1) / round * round;
+    px = LANES / eights;
+    slot = threadIdx.x / eights;
+    eight = threadIdx.x - slot * eights;
+    if (slot >= px) eight = eights;  // (idle)
+  }
+};
+
+// Eight channels of a pixel; past the end zeros.
 template <typename T>
-__global__ __launch_bounds__(256) void k_norm_stats(NormArgs a, float *__restrict__ stats) {
-  __shared__ float lds[4];
-  const int per = a.c / a.groups;
-  const long image = blockIdx.x / a.groups, g = blockIdx.x % a.groups, n = a.pixels * per;
-  const T *x = (const T *)a.x + image * a.pixels * a.stride + g * per;
-  float s = 0.0f;
-  for (long i = threadIdx.x; i < n; i += 256) s += (float)x[i / per * a.stride + i % per];
-  const float mean = block_sum<256>(s, lds) / (float)n;
-  s = 0.0f;
-  for (long i = threadIdx.x; i < n; i += 256) {
-    const float d = (float)x[i / per * a.stride + i % per] - mean;
-    s += d * d;
-  }
-  const float var = block_sum<256>(s, lds) / (float)n;
-  if (threadIdx.x == 0) {
-    stats[2 * blockIdx.x] = mean;
-    stats[2 * blockIdx.x + 1] = 1.0f / sqrtf(var + a.eps);
-  }
+__device__ __forceinline__ void load_eight(const T *row, int at, int c, float *v) {
+  if (at + 8 <= c)
+    load8<T, true>(row, at, c, v);
+  else
+    load8<T, false>(row, at, c, v);
 }
 
-// 16 lanes a block of 128 channels of a pixel.
-template <typename T, typename Y>
-__global__ __launch_bounds__(256) void k_norm_apply(NormArgs a, const float *__restrict__ stats) {
-  const int blocks = (a.c + 127) / 128, per = a.c / a.groups;
-  const long total = a.images * a.pixels * blocks;
-  const int lane8 = (threadIdx.x & 15) * 8;
-  for (long item = (long)blockIdx.x * 16 + threadIdx.x / 16; item < total; item += (long)gridDim.x * 16) {
-    const long r = item / blocks, image = r / a.pixels;
-    const int b = (int)(item - r * blocks), at = b * 128 + lane8;
-    float v[8];
-    load8<T, false>((const T *)a.x + r * a.stride, at, a.c, v);
+// U pixels' values, `many` of them counted, into a lane's statistics.
+template <int U>
+__device__ __forceinline__ void take(const float (&v)[U][8], int many, float &n, float *m, float *q) {
+  const float k = (float)many, w = share(k, n + k), nw = n * w;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int ch = at + i;
-      if (ch < a.c) {
-        const float *st = stats + 2 * (image * a.groups + ch / per);
-        v[i] = (v[i] - st[0]) * st[1] * (a.gamma ? a.gamma[ch] : 1.0f) + (a.beta ? a.beta[ch] : 0.0f);
-      }
+  for (int i = 0; i < 8; i++) {
+    float s = 0.0f, e = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; u++) s += u < many ? v[u][i] : 0.0f;
+    const float mean = many == U ? s * (1.0f / U) : s / k;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const float d = v[u][i] - mean;
+      e += u < many ? d * d : 0.0f;
     }
-    with_act8(a.act, [&](auto act) {
+    const float d = mean - m[i];
+    m[i] += d * w;
+    q[i] += e + d * d * nw;
+  }
+  n += k;
+}
+
+// The lanes' statistics of the workgroup's channels, joined by group: f(group
+// of the span, mean, squares), one lane a group.  Channels first, where a lane's
+// eight have a group in common: runs of W = gcd(per, 8) channels.
+template <typename F>
+__device__ __forceinline__ void by_group(Shared &s, const Place &p, float n, float (&m)[8], float (&q)[8], int span,
+                                         int per, F f) {
+  const int t = threadIdx.x, W = per & 7 ? per & -per : 8, runs = 8 / W;
+  auto pairs = [&](auto width) {  // runs of `width` to runs of twice as many
+    constexpr int V = decltype(width)::value;
+#pragma unroll
+    for (int i = 0; i < 4 / V; i++) {
+      const float a = m[2 * i], b = m[2 * i + 1], d = b - a;
+      m[i] = a + 0.5f * d;
+      q[i] = q[2 * i] + q[2 * i + 1] + d * d * (0.5f * V * n);
+    }
+  };
+  if (W >= 2) pairs(Act<1>{});
+  if (W >= 4) pairs(Act<2>{});
+  if (W >= 8) pairs(Act<4>{});
+  s.n[t] = n;
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < runs) s.m[i * LANES + t] = m[i], s.q[i * LANES + t] = q[i];
+  int width = 1;
+  while (width < p.px) width *= 2;
+  for (int w = width / 2; w >= 1; w /= 2) {
+    __syncthreads();
+    if (p.slot < w && p.slot + w < p.px) {
+      const int o = t + w * p.eights;
+      const float n2 = s.n[o], k = share(n2, n + n2), nk = W * n * k;
+      n += n2;
+      s.n[t] = n;
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        if (at + i < a.c) v[i] = act8<decltype(act)::value>(v[i]);
-    });
-    if constexpr (sizeof(Y) == 1) {
-      float m = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) m = fmaxf(m, finite_magnitude(v[i]));
-      const int e = exponent8(max16(m));
-      *(int2v *)((uint8_t *)a.y + r * a.ystride + at) = pack8(v, inverse_power(e));
-      if (lane8 == 0) a.scales[r * a.scale_stride + b] = (uint8_t)(e + 127);
-    } else {
-      store8<Y, false>((Y *)a.y + r * a.ystride, at, a.c, v);
+        if (i < runs) {
+          join(m[i], q[i], s.m[i * LANES + o], s.q[i * LANES + o], k, nk);
+          s.m[i * LANES + t] = m[i], s.q[i * LANES + t] = q[i];
+        }
+    }
+  }
+  __syncthreads();
+  const float each = s.n[0] * W;  // values of a run
+  const int many = per / W;       // runs of a group
+  auto at = [&](int r) { return (r & (runs - 1)) * LANES + r / runs; };
+  if (many <= 8) {
+    for (int g = t; g < span / per; g += LANES) {
+      float mean = 0.0f, squares = 0.0f;
+      for (int r = 0; r < many; r++) mean += s.m[at(g * many + r)];
+      mean /= (float)many;
+      for (int r = 0; r < many; r++) {
+        const float d = s.m[at(g * many + r)] - mean;
+        squares += s.q[at(g * many + r)] + each * d * d;
+      }
+      f(g, mean, squares);
+    }
+  } else {
+    for (int g = t >> 6; g < span / per; g += LANES / 64) {
+      float mean = 0.0f, squares = 0.0f;
+      for (int r = t & 63; r < many; r += 64) mean += s.m[at(g * many + r)];
+      mean = group_sum<64>(mean) / (float)many;
+      for (int r = t & 63; r < many; r += 64) {
+        const float d = s.m[at(g * many + r)] - mean;
+        squares += s.q[at(g * many + r)] + each * d * d;
+      }
+      squares = group_sum<64>(squares);
+      if ((t & 63) == 0) f(g, mean, squares);
     }
   }
 }
 
-ien_status run(ien_ctx *ctx, const NormArgs &a, ien_out_type type, int y_bytes) {
-  IEN_CHECK(a.images * a.groups * 2 <= (long)ctx->splitk_floats, IEN_ERR_INPUT, "%ld maps of %d groups past the workspace",
-            a.images, a.groups);
-  const unsigned stat = (unsigned)(a.images * a.groups);
-  const long items = a.images * a.pixels * ((a.c + 127) / 128);
-  const unsigned grid = (unsigned)std::min((items + 15) / 16, 1L << 24);
-  auto go = [&](auto tag) {
-    using T = decltype(tag);
-    hipLaunchKernelGGL(k_norm_stats<T>, dim3(stat), dim3(256), 0, ctx->stream, a, ctx->splitk);
-    if (y_bytes == 1)
-      hipLaunchKernelGGL((k_norm_apply<T, uint8_t>), dim3(grid), dim3(256), 0, ctx->stream, a, ctx->splitk);
-    else if (y_bytes == 2)
-      hipLaunchKernelGGL((k_norm_apply<T, _Float16>), dim3(grid), dim3(256), 0, ctx->stream, a, ctx->splitk);
+// A part of an image's pixels: its groups' means and squares.
+template <typename T>
+__global__ __launch_bounds__(LANES) void k_norm_stats(NormArgs a) {
+  __shared__ Shared s;
+  constexpr int U = sizeof(T) == 2 ? 8 : 4;
+  const Place p(a.c, 1);
+  const int image = blockIdx.x / a.chunks, part = blockIdx.x % a.chunks, at = p.eight * 8;
+  const long begin = part * a.chunk;
+  const int many = (int)min(a.chunk, a.pixels - begin);
+  const T *x = (const T *)a.x + (image * a.pixels + begin + p.slot) * a.stride;
+  float n = 0.0f, m[8] = {}, q[8] = {};
+  if (p.eight < p.eights) {
+    int left = (unsigned)(many - p.slot + p.px - 1) / (unsigned)p.px;  // this lane's pixels
+    const long step = p.px * a.stride;
+    float v[U][8];
+    for (; left >= U; left -= U, x += U * step) {
+#pragma unroll
+      for (int u = 0; u < U; u++) load_eight(x + u * step, at, a.c, v[u]);
+      take<U>(v, U, n, m, q);
+    }
+    if (left > 0) {
+#pragma unroll
+      for (int u = 0; u < U; u++) load_eight(x + (u < left ? u : 0) * step, at, a.c, v[u]);
+      take<U>(v, left, n, m, q);
+    }
+  }
+  float2 *out = a.part + (long)blockIdx.x * a.groups;
+  by_group(s, p, n, m, q, a.c, a.c / a.groups, [&](int g, float mean, float squares) { out[g] = {mean, squares}; });
+}
+
+// A lane's eight channels' way from x to y.
+struct Line {
+  float mean[8], gain[8], bias[8];
+  __device__ void set(const NormArgs &a, int c0, int at, const float2 *stats) {
+    const int per = a.c / a.groups;
+#pragma unroll
+    for (int i = 0; i < 8; i++) gain[i] = 1.0f, bias[i] = 0.0f;
+    if (a.gamma) load_eight(a.gamma + c0, at, a.span, gain);
+    if (a.beta) load_eight(a.beta + c0, at, a.span, bias);
+    int g = at / per, in = at - g * per;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float2 st = stats[min(g, a.span / per - 1)];
+      mean[i] = st.x;
+      gain[i] *= st.y;
+      if (++in == per) in = 0, g++;
+    }
+  }
+};
+
+// Eight results of pixel r from channel c0 + at on (`at` within the span).
+template <typename Y, int ACT>
+__device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, int c0, int at, float *v) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = act8<ACT>((v[i] - l.mean[i]) * l.gain[i] + l.bias[i]);
+  if constexpr (sizeof(Y) == 1) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (at + i >= a.span) v[i] = 0.0f;
+      top = fmaxf(top, finite_magnitude(v[i]));
+    }
+    const int e = exponent8(max16(top));
+    *(int2v *)((uint8_t *)a.y + r * a.ystride + c0 + at) = pack8(v, inverse_power(e));
+    if ((at & 127) == 0) a.scales[r * a.scale_stride + (c0 + at) / 128] = (uint8_t)(e + 127);
+  } else {
+    Y *y = (Y *)a.y + r * a.ystride + c0;
+    if (at + 8 <= a.span)
+      store8<Y, true>(y, at, a.span, v);
     else
-      hipLaunchKernelGGL((k_norm_apply<T, float>), dim3(grid), dim3(256), 0, ctx->stream, a, ctx->splitk);
+      store8<Y, false>(y, at, a.span, v);
+  }
+}
+
+// The parts' statistics joined, and the same part of the pixels again, from its end.
+template <typename T, typename Y>
+__global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
+  constexpr int U = sizeof(T) == 2 ? 4 : 2;
+  __shared__ float sm[LANES], sq[LANES], sn[LANES];
+  extern __shared__ float2 stats[];  // [group]: mean, 1 / deviation
+  const int t = threadIdx.x, per = a.c / a.groups, image = blockIdx.x / a.chunks, mine = blockIdx.x % a.chunks;
+  const float2 *part = a.part + (long)image * a.chunks * a.groups;
+  for (int g0 = 0; g0 < a.groups; g0 += LANES) {
+    const int many = min(a.groups - g0, LANES), rows = LANES / many, row = t / many, g = t - row * many;
+    float n = 0.0f, m = 0.0f, q = 0.0f;
+    constexpr int AHEAD = 8;
+    if (row < rows)
+      for (int k0 = row; k0 < a.chunks; k0 += AHEAD * rows) {
+        float2 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) v[i] = part[(long)min(k0 + i * rows, a.chunks - 1) * a.groups + g0 + g];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+          const int k = k0 + i * rows;
+          const float n2 = k < a.chunks ? (float)min(a.chunk, a.pixels - k * a.chunk) * per : 0.0f, w = share(n2, n + n2);
+          if (k < a.chunks) join(m, q, v[i].x, v[i].y, w, n * w);
+          n += n2;
+        }
+      }
+    sn[t] = n, sm[t] = m, sq[t] = q;
+    int width = 1;
+    while (width < min(rows, a.chunks)) width *= 2;
+    for (int w = width / 2; w >= 1; w /= 2) {
+      __syncthreads();
+      if (row < w && row + w < rows) {
+        const int o = t + w * many;
+        const float n2 = sn[o], k = share(n2, n + n2);
+        join(m, q, sm[o], sq[o], k, n * k);
+        n += n2;
+        sn[t] = n, sm[t] = m, sq[t] = q;
+      }
+    }
+    if (row == 0) stats[g0 + g] = {m, 1.0f / sqrtf(q / n + a.eps)};
+    __syncthreads();
+  }
+
+  const Place p(a.c, sizeof(Y) == 1 ? 16 : 1);
+  const int at = p.eight * 8;
+  if (p.eight >= p.eights) return;
+  Line l;
+  l.set(a, 0, at, stats);
+  const long begin = mine * a.chunk, r0 = image * a.pixels + begin + p.slot;
+  const int count = (unsigned)((int)min(a.chunk, a.pixels - begin) - p.slot + p.px - 1) / (unsigned)p.px;
+  const long step = p.px * a.stride;
+  const T *x = (const T *)a.x + r0 * a.stride;
+  with_act8(a.act, [&](auto act) {
+    for (int k = (count - 1) / U * U; k >= 0; k -= U) {
+      float v[U][8];
+#pragma unroll
+      for (int u = 0; u < U; u++) load_eight(x + min(k + u, count - 1) * step, at, a.c, v[u]);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (k + u < count) put<Y, decltype(act)::value>(a, l, r0 + (long)(k + u) * p.px, 0, at, v[u]);
+    }
+  });
+}
+
+// One launch: a workgroup a span of whole groups (and blocks of 128 channels)
+// of an image, its values kept in registers, up to R pixels a lane.
+constexpr int HELD = 8;
+template <typename T, typename Y>
+__global__ __launch_bounds__(LANES) void k_norm_held(NormArgs a) {
+  __shared__ Shared s;
+  extern __shared__ float2 stats[];
+  const Place p(a.span, 16);
+  const int spans = a.c / a.span, image = blockIdx.x / spans, c0 = blockIdx.x % spans * a.span, at = p.eight * 8;
+  const int per = a.c / a.groups;
+  const long r0 = image * a.pixels + p.slot;
+  const T *x = (const T *)a.x + r0 * a.stride + c0;
+  const int count = p.eight < p.eights ? (int)(unsigned)((int)a.pixels - p.slot + p.px - 1) / (unsigned)p.px : 0;
+  float v[HELD][8] = {}, n = 0.0f, m[8] = {}, q[8] = {};
+#pragma unroll
+  for (int u = 0; u < HELD; u++)
+    if (u < count) load_eight(x + (long)u * p.px * a.stride, at, a.span, v[u]);
+  if (count > 0) take<HELD>(v, count, n, m, q);
+  by_group(s, p, n, m, q, a.span, per, [&](int g, float mean, float squares) {
+    stats[g] = {mean, 1.0f / sqrtf(squares / ((float)a.pixels * per) + a.eps)};
+  });
+  __syncthreads();
+  if (count == 0) return;
+  Line l;
+  l.set(a, c0, at, stats);
+  with_act8(a.act, [&](auto act) {
+#pragma unroll
+    for (int u = 0; u < HELD; u++)
+      if (u < count) put<Y, decltype(act)::value>(a, l, r0 + (long)u * p.px, c0, at, v[u]);
+  });
+}
+
+ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_bytes) {
+  const int per = a.c / a.groups;
+  // One launch where a lane's share is at most HELD pixels of it: the smallest
+  // span of whole groups and blocks of 128 channels.
+  int span = per;
+  while (span % 128 != 0 && span < a.c) span += per;
+  if (span % 128 != 0 || a.c % span != 0) span = a.c;
+  const int lanes = (span + 127) / 128 * 16;
+  const bool held = a.pixels <= (long)HELD * (LANES / lanes);
+  a.span = held ? span : a.c;
+  // Otherwise a workgroup a part of at least four rounds of pixels, one for each CU.
+  const int px = LANES / ((a.c + 7) / 8);
+  const long rounds = (a.pixels + px - 1) / px;
+  long parts = std::max(1L, std::min((rounds + 3) / 4, ctx->cus / images));
+  a.chunk = std::min((rounds + parts - 1) / parts, (1L << 30) / px) * px;  // (counted in 32 bits)
+  a.chunks = (int)((a.pixels + a.chunk - 1) / a.chunk);
+  a.part = (float2 *)ctx->splitk;
+  const long most = held ? 1L << 16 : std::max(1L, (long)(ctx->splitk_floats / 2) / ((long)a.chunks * a.groups));
+  const void *x = a.x;
+  uint8_t *y = (uint8_t *)a.y, *scales = a.scales;
+  auto go = [&](auto t, auto u, long many) {
+    using T = decltype(t);
+    using Y = decltype(u);
+    const size_t shared = (size_t)(held ? a.span / per : a.groups) * sizeof(float2);
+    if (held) {
+      hipLaunchKernelGGL((k_norm_held<T, Y>), dim3((unsigned)(many * (a.c / a.span))), dim3(LANES), shared, ctx->stream, a);
+    } else {
+      const dim3 grid((unsigned)(many * a.chunks));
+      hipLaunchKernelGGL(k_norm_stats<T>, grid, dim3(LANES), 0, ctx->stream, a);
+      hipLaunchKernelGGL((k_norm_apply<T, Y>), grid, dim3(LANES), shared, ctx->stream, a);
+    }
   };
-  type == IEN_OUT_F16 ? go((_Float16)0) : go(0.0f);
+  const int x_bytes = type == IEN_OUT_F16 ? 2 : 4;
+  for (long i = 0; i < images; i += most) {  // (one turn but for a great many images)
+    const long many = std::min(most, images - i), r = i * a.pixels;
+    a.x = (const uint8_t *)x + r * a.stride * x_bytes;
+    a.y = y + r * a.ystride * y_bytes;
+    a.scales = scales + r * a.scale_stride;
+    if (x_bytes == 2)
+      y_bytes == 1 ? go((_Float16)0, (uint8_t)0, many)
+                   : y_bytes == 2 ? go((_Float16)0, (_Float16)0, many) : go((_Float16)0, 0.0f, many);
+    else
+      y_bytes == 1 ? go(0.0f, (uint8_t)0, many) : y_bytes == 2 ? go(0.0f, (_Float16)0, many) : go(0.0f, 0.0f, many);
+  }
   IEN_HIP(hipGetLastError());
   return IEN_OK;
 }
@@ -126,7 +398,6 @@ ien_status describe(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t ima
             "%zu maps of %zu pixels, %zu apart", images, pixels, stride);
   *a = NormArgs{};
   a->x = d_x;
-  a->images = (long)images;
   a->pixels = (long)pixels;
   a->stride = (long)stride;
   a->c = (int)c;
@@ -159,7 +430,7 @@ ien_status ien_group_norm(ien_ctx *ctx, const void *d_x, ien_out_type type, size
             "in place with another type or stride");
   a.y = d_y;
   a.ystride = (long)y_stride;
-  return run(ctx, a, type, y_type == IEN_OUT_F16 ? 2 : 4);
+  return run(ctx, a, (long)images, type, y_type == IEN_OUT_F16 ? 2 : 4);
 }
 
 ien_status ien_group_norm8(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t images, size_t pixels, size_t c,
@@ -176,7 +447,7 @@ ien_status ien_group_norm8(ien_ctx *ctx, const void *d_x, ien_out_type type, siz
   a.ystride = (long)out->stride;
   a.scales = out->scales;
   a.scale_stride = (long)out->scale_stride;
-  return run(ctx, a, type, 1);
+  return run(ctx, a, (long)images, type, 1);
 }
 
 }  // extern "C"

@@ -49,7 +49,7 @@ struct Args8 {
   int f32, act;
   const void *add;
   long as;
-  int image, vec;  // a map's pixels; whole eights of the output (and of add)
+  int image, vec;  // a map's pixels; whole eights of outputs
   int tiles_m, tiles_n, ksplit, kchunks;
   float *part;
   int *tile_count;
@@ -353,7 +353,13 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   using Y = std::conditional_t<F32, float, _Float16>;
   const int row = lane / EIGHTS, col = lane % EIGHTS * 8;
   float bias[8];
-  load8<float, true>((const float *)(lds + T::BIAS0) + wn * COLS, col, 0, bias);
+  // Eight floats of LDS, 16-byte aligned.
+  auto take = [](const float *p, float *v) {
+    const float4v a = *(const float4v *)p, b = *(const float4v *)(p + 4);
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = a[k], v[4 + k] = b[k];
+  };
+  take((const float *)(lds + T::BIAS0) + wn * COLS + col, bias);
   auto stage_rows = [&](const floatx16 (&v)[T::FN]) {
 #pragma unroll
     for (int j = 0; j < T::FN; j++)
@@ -382,7 +388,7 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
         for (int e = 0; e < ITEMS; e++) {
           if (!in || r0 + row + e * (64 / EIGHTS) >= a.rows) continue;
           float v[8];
-          load8<float, true>(st, (row + e * (64 / EIGHTS)) * T::PITCH + col, 0, v);
+          take(st + (row + e * (64 / EIGHTS)) * T::PITCH + col, v);
 #pragma unroll
           for (int k = 0; k < 8; k++) v[k] += bias[k];
           if (a.add) {
@@ -530,8 +536,7 @@ ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *in, size_t row0, size_t
   a.add = d_add;
   a.as = (long)add_stride;
   a.image = in->kind == IEN_INPUT_IMAGE;
-  const size_t size = a.f32 ? 4 : 2;
-  a.vec = whole_eights(a.y, w->n, out->stride, size) && (!d_add || whole_eights(d_add, w->n, add_stride, size));
+  a.vec = w->n % 8 == 0;
   // A tile addresses its rows' values by 31-bit offsets from its first one's.
   IEN_CHECK(in->map.stride < (1u << 20) && in->map.scale_stride < (1u << 20) &&
                 (!a.image || (in->width + 256) * std::max(in->map.stride, in->map.scale_stride) < (1u << 29)),

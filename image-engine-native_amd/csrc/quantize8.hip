@@ -123,7 +123,7 @@ ien_status ien_quantize8(ien_ctx *ctx, const void *d_x, ien_out_type type, size_
   if (s != IEN_OK) return s;
   const int blocks = (int)blocks8(k);
   const dim3 grid(grid_of((long)rows * blocks));
-  const bool vec = whole_eights(d_x, k, stride, type == IEN_OUT_F16 ? 2 : 4);
+  const bool vec = k % 8 == 0;
   auto launch = [&](auto kernel, auto *x) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, x, (long)stride, (long)rows, (long)k, blocks,
                        args_of(*out));
@@ -148,7 +148,7 @@ ien_status ien_dequantize8(ien_ctx *ctx, const ien_rows8 *x, size_t rows, size_t
   if (s != IEN_OK) return s;
   const int blocks = (int)blocks8(k);
   const dim3 grid(grid_of((long)rows * blocks));
-  const bool vec = whole_eights(d_y, k, stride, type == IEN_OUT_F16 ? 2 : 4);
+  const bool vec = k % 8 == 0;
   auto launch = [&](auto kernel, auto *y) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, args_of(*x), (long)rows, (long)k, blocks, y,
                        (long)stride);
