@@ -39,8 +39,8 @@ struct NormArgs {
   float2 *part;  // [image][chunk][group]: mean and squares
 };
 
-constexpr int LANES = 1024;  // of a workgroup
-
+// LANES: of a workgroup.
+template <int LANES>
 struct Shared {
   float m[8 * LANES], q[8 * LANES], n[LANES];  // [channel of the eight][lane]
 };
@@ -55,9 +55,10 @@ __device__ __forceinline__ void join(float &m1, float &q1, float m2, float q2, f
 __device__ __forceinline__ float share(float n2, float n) { return n > 0.0f ? n2 * __builtin_amdgcn_rcpf(n) : 0.0f; }
 
 // `eights` lanes a pixel, px pixels side by side.
+template <int LANES>
 struct Place {
   int eights, px, slot, eight;
-  __device__ Place(int span, int round) {
+  __device__ __forceinline__ Place(int span, int round) {
     eights = (span / 8 + (span % 8 != 0) + round - 1) / round * round;
     px = LANES / eights;
     slot = threadIdx.x / eights;
@@ -75,24 +76,27 @@ __device__ __forceinline__ void load_eight(const T *row, int at, int c, float *v
     load8<T, false>(row, at, c, v);
 }
 
-// U pixels' values, `many` of them counted, into a lane's statistics.
-template <int U>
-__device__ __forceinline__ void take(const float (&v)[U][8], int many, float &n, float *m, float *q) {
-  const float k = (float)many, w = share(k, n + k), nw = n * w;
+// U pixels' values, the first `many` of them counted (ALL: all), into a lane's
+// statistics.
+template <bool ALL, int U>
+__device__ __forceinline__ void take(const float (&v)[U][8], int many, float &n, float (&m)[8], float (&q)[8]) {
+  const float k = ALL ? (float)U : (float)many, w = share(k, n + k), nw = n * w;
+  float counts[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) counts[u] = u < many ? 1.0f : 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
+    // (Sums from the first value on: of equal ones exact.)
     float s = 0.0f, e = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; u++) s += u < many ? v[u][i] : 0.0f;
-    const float mean = many == U ? s * (1.0f / U) : s / k;
+    for (int u = 1; u < U; u++) s += ALL ? v[u][i] - v[0][i] : (v[u][i] - v[0][i]) * counts[u];
+    const float mean = v[0][i] + (ALL ? s * (1.0f / U) : s * __builtin_amdgcn_rcpf(k));
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const float d = v[u][i] - mean;
-      e += u < many ? d * d : 0.0f;
+      e += ALL ? d * d : d * d * counts[u];
     }
-    const float d = mean - m[i];
-    m[i] += d * w;
-    q[i] += e + d * d * nw;
+    join(m[i], q[i], mean, e, w, nw);
   }
   n += k;
 }
@@ -100,8 +104,8 @@ __device__ __forceinline__ void take(const float (&v)[U][8], int many, float &n,
 // The lanes' statistics of the workgroup's channels, joined by group: f(group
 // of the span, mean, squares), one lane a group.  Channels first, where a lane's
 // eight have a group in common: runs of W = gcd(per, 8) channels.
-template <typename F>
-__device__ __forceinline__ void by_group(Shared &s, const Place &p, float n, float (&m)[8], float (&q)[8], int span,
+template <int LANES, typename F>
+__device__ __forceinline__ void by_group(Shared<LANES> &s, const Place<LANES> &p, float n, float (&m)[8], float (&q)[8], int span,
                                          int per, F f) {
   const int t = threadIdx.x, W = per & 7 ? per & -per : 8, runs = 8 / W;
   auto pairs = [&](auto width) {  // runs of `width` to runs of twice as many
@@ -167,32 +171,36 @@ __device__ __forceinline__ void by_group(Shared &s, const Place &p, float n, flo
   }
 }
 
-// A part of an image's pixels: its groups' means and squares.
+// A lane's statistics of its `left` pixels from x on, `step` apart.
 template <typename T>
-__global__ __launch_bounds__(LANES) void k_norm_stats(NormArgs a) {
-  __shared__ Shared s;
+__device__ __forceinline__ void gather(const T *x, long step, int left, int at, int c, float &n, float (&m)[8],
+                                       float (&q)[8]) {
   constexpr int U = sizeof(T) == 2 ? 8 : 4;
-  const Place p(a.c, 1);
+  float v[U][8];
+  for (; left >= U; left -= U, x += U * step) {
+#pragma unroll
+    for (int u = 0; u < U; u++) load_eight(x + u * step, at, c, v[u]);
+    take<true>(v, U, n, m, q);
+  }
+  if (left > 0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) load_eight(x + (u < left ? u : 0) * step, at, c, v[u]);
+    take<false>(v, left, n, m, q);
+  }
+}
+
+// A part of an image's pixels: its groups' means and squares.
+template <typename T, int LANES>
+__global__ __launch_bounds__(LANES) void k_norm_stats(NormArgs a) {
+  __shared__ Shared<LANES> s;
+  const Place<LANES> p(a.c, 1);
   const int image = blockIdx.x / a.chunks, part = blockIdx.x % a.chunks, at = p.eight * 8;
   const long begin = part * a.chunk;
   const int many = (int)min(a.chunk, a.pixels - begin);
   const T *x = (const T *)a.x + (image * a.pixels + begin + p.slot) * a.stride;
   float n = 0.0f, m[8] = {}, q[8] = {};
-  if (p.eight < p.eights) {
-    int left = (unsigned)(many - p.slot + p.px - 1) / (unsigned)p.px;  // this lane's pixels
-    const long step = p.px * a.stride;
-    float v[U][8];
-    for (; left >= U; left -= U, x += U * step) {
-#pragma unroll
-      for (int u = 0; u < U; u++) load_eight(x + u * step, at, a.c, v[u]);
-      take<U>(v, U, n, m, q);
-    }
-    if (left > 0) {
-#pragma unroll
-      for (int u = 0; u < U; u++) load_eight(x + (u < left ? u : 0) * step, at, a.c, v[u]);
-      take<U>(v, left, n, m, q);
-    }
-  }
+  if (p.eight < p.eights)
+    gather(x, p.px * a.stride, (unsigned)(many - p.slot + p.px - 1) / (unsigned)p.px, at, a.c, n, m, q);
   float2 *out = a.part + (long)blockIdx.x * a.groups;
   by_group(s, p, n, m, q, a.c, a.c / a.groups, [&](int g, float mean, float squares) { out[g] = {mean, squares}; });
 }
@@ -241,87 +249,99 @@ __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, in
   }
 }
 
-// The parts' statistics joined, and the same part of the pixels again, from its end.
+// A lane's `count` pixels r, r + px, ... from x on, `step` apart, from the last.
 template <typename T, typename Y>
-__global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
+__device__ __forceinline__ void apply(const NormArgs &a, const Line &l, const T *x, long step, int count, long r, int px,
+                                      int c0, int at) {
   constexpr int U = sizeof(T) == 2 ? 4 : 2;
-  __shared__ float sm[LANES], sq[LANES], sn[LANES];
+  with_act8(a.act, [&](auto act) {
+    for (int k = (count - 1) / U * U; k >= 0; k -= U) {
+      float v[U][8];
+#pragma unroll
+      for (int u = 0; u < U; u++) load_eight(x + min(k + u, count - 1) * step, at, a.span, v[u]);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (k + u < count) put<Y, decltype(act)::value>(a, l, r + (long)(k + u) * px, c0, at, v[u]);
+    }
+  });
+}
+
+// The parts' statistics joined, and the same part of the pixels again, from its
+// end.  The parts' means are summed from the first one's on, then the squares
+// about their mean; all but the last part hold a.chunk pixels.
+template <typename T, typename Y, int LANES>
+__global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
+  constexpr int HERE = 8192 / LANES;  // parts a lane keeps for the second sum
+  __shared__ float sums[LANES], means[LANES];
   extern __shared__ float2 stats[];  // [group]: mean, 1 / deviation
   const int t = threadIdx.x, per = a.c / a.groups, image = blockIdx.x / a.chunks, mine = blockIdx.x % a.chunks;
-  const float2 *part = a.part + (long)image * a.chunks * a.groups;
+  const float whole = (float)a.chunk, last = (float)(a.pixels - (a.chunks - 1) * a.chunk);
   for (int g0 = 0; g0 < a.groups; g0 += LANES) {
     const int many = min(a.groups - g0, LANES), rows = LANES / many, row = t / many, g = t - row * many;
-    float n = 0.0f, m = 0.0f, q = 0.0f;
-    constexpr int AHEAD = 8;
-    if (row < rows)
-      for (int k0 = row; k0 < a.chunks; k0 += AHEAD * rows) {
-        float2 v[AHEAD];
+    const float2 *part = a.part + (long)image * a.chunks * a.groups + g0 + g;
+    const float base = part[0].x;
+    // A lane's parts row, row + rows, ...: f(its mean and squares, its pixels).
+    float2 v[HERE];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) v[i] = part[(long)min(k0 + i * rows, a.chunks - 1) * a.groups + g0 + g];
+    for (int i = 0; i < HERE; i++) v[i] = part[(long)min(row + i * rows, a.chunks - 1) * a.groups];
+    auto each = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-          const int k = k0 + i * rows;
-          const float n2 = k < a.chunks ? (float)min(a.chunk, a.pixels - k * a.chunk) * per : 0.0f, w = share(n2, n + n2);
-          if (k < a.chunks) join(m, q, v[i].x, v[i].y, w, n * w);
-          n += n2;
-        }
+      for (int i = 0; i < HERE; i++) {
+        const int k = row + i * rows;
+        f(v[i], k >= a.chunks ? 0.0f : k == a.chunks - 1 ? last : whole);
       }
-    sn[t] = n, sm[t] = m, sq[t] = q;
-    int width = 1;
-    while (width < min(rows, a.chunks)) width *= 2;
-    for (int w = width / 2; w >= 1; w /= 2) {
+      for (int k = row + HERE * rows; k < a.chunks; k += rows) f(part[(long)k * a.groups], k == a.chunks - 1 ? last : whole);
+    };
+    auto sum = [&](float s) {  // over a group's lanes, in the first one
       __syncthreads();
-      if (row < w && row + w < rows) {
-        const int o = t + w * many;
-        const float n2 = sn[o], k = share(n2, n + n2);
-        join(m, q, sm[o], sq[o], k, n * k);
-        n += n2;
-        sn[t] = n, sm[t] = m, sq[t] = q;
-      }
-    }
-    if (row == 0) stats[g0 + g] = {m, 1.0f / sqrtf(q / n + a.eps)};
+      sums[t] = s;
+      __syncthreads();
+      s = 0.0f;
+      if (row == 0)
+        for (int k = 0; k < rows; k++) s += sums[k * many + t];
+      return s;
+    };
+    float s = 0.0f;
+    if (row < rows) each([&](float2 x, float n) { s += n * (x.x - base); });
+    s = sum(s);
+    if (row == 0) means[t] = base + s / (float)a.pixels;
+    __syncthreads();
+    const float mean = means[g];
+    s = 0.0f;
+    if (row < rows)
+      each([&](float2 x, float n) {
+        const float d = x.x - mean;
+        s += n > 0.0f ? x.y + (n * per) * d * d : 0.0f;
+      });
+    s = sum(s);
+    if (row == 0) stats[g0 + t] = {mean, 1.0f / sqrtf(s / ((float)a.pixels * per) + a.eps)};
     __syncthreads();
   }
 
-  const Place p(a.c, sizeof(Y) == 1 ? 16 : 1);
+  const Place<LANES> p(a.c, sizeof(Y) == 1 ? 16 : 1);
   const int at = p.eight * 8;
   if (p.eight >= p.eights) return;
   Line l;
   l.set(a, 0, at, stats);
   const long begin = mine * a.chunk, r0 = image * a.pixels + begin + p.slot;
   const int count = (unsigned)((int)min(a.chunk, a.pixels - begin) - p.slot + p.px - 1) / (unsigned)p.px;
-  const long step = p.px * a.stride;
-  const T *x = (const T *)a.x + r0 * a.stride;
-  with_act8(a.act, [&](auto act) {
-    for (int k = (count - 1) / U * U; k >= 0; k -= U) {
-      float v[U][8];
-#pragma unroll
-      for (int u = 0; u < U; u++) load_eight(x + min(k + u, count - 1) * step, at, a.c, v[u]);
-#pragma unroll
-      for (int u = 0; u < U; u++)
-        if (k + u < count) put<Y, decltype(act)::value>(a, l, r0 + (long)(k + u) * p.px, 0, at, v[u]);
-    }
-  });
+  if (count > 0) apply<T, Y>(a, l, (const T *)a.x + r0 * a.stride, p.px * a.stride, count, r0, p.px, 0, at);
 }
 
 // One launch: a workgroup a span of whole groups (and blocks of 128 channels)
-// of an image, its values kept in registers, up to R pixels a lane.
-constexpr int HELD = 8;
-template <typename T, typename Y>
-__global__ __launch_bounds__(LANES) void k_norm_held(NormArgs a) {
-  __shared__ Shared s;
+// of an image.
+template <typename T, typename Y, int LANES>
+__global__ __launch_bounds__(LANES) void k_norm_one(NormArgs a) {
+  __shared__ Shared<LANES> s;
   extern __shared__ float2 stats[];
-  const Place p(a.span, 16);
+  const Place<LANES> p(a.span, 16);
   const int spans = a.c / a.span, image = blockIdx.x / spans, c0 = blockIdx.x % spans * a.span, at = p.eight * 8;
   const int per = a.c / a.groups;
   const long r0 = image * a.pixels + p.slot;
   const T *x = (const T *)a.x + r0 * a.stride + c0;
-  const int count = p.eight < p.eights ? (int)(unsigned)((int)a.pixels - p.slot + p.px - 1) / (unsigned)p.px : 0;
-  float v[HELD][8] = {}, n = 0.0f, m[8] = {}, q[8] = {};
-#pragma unroll
-  for (int u = 0; u < HELD; u++)
-    if (u < count) load_eight(x + (long)u * p.px * a.stride, at, a.span, v[u]);
-  if (count > 0) take<HELD>(v, count, n, m, q);
+  const int count = p.eight < p.eights ? (unsigned)((int)a.pixels - p.slot + p.px - 1) / (unsigned)p.px : 0;
+  float n = 0.0f, m[8] = {}, q[8] = {};
+  gather(x, p.px * a.stride, count, at, a.span, n, m, q);
   by_group(s, p, n, m, q, a.span, per, [&](int g, float mean, float squares) {
     stats[g] = {mean, 1.0f / sqrtf(squares / ((float)a.pixels * per) + a.eps)};
   });
@@ -329,25 +349,23 @@ __global__ __launch_bounds__(LANES) void k_norm_held(NormArgs a) {
   if (count == 0) return;
   Line l;
   l.set(a, c0, at, stats);
-  with_act8(a.act, [&](auto act) {
-#pragma unroll
-    for (int u = 0; u < HELD; u++)
-      if (u < count) put<Y, decltype(act)::value>(a, l, r0 + (long)u * p.px, c0, at, v[u]);
-  });
+  apply<T, Y>(a, l, x, p.px * a.stride, count, r0, p.px, c0, at);
 }
+
+constexpr int ONE = 512;  // lanes of one launch's workgroups
 
 ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_bytes) {
   const int per = a.c / a.groups;
-  // One launch where a lane's share is at most HELD pixels of it: the smallest
-  // span of whole groups and blocks of 128 channels.
+  // One launch where a lane's share is a few pixels of the smallest span of
+  // whole groups and blocks of 128 channels.
   int span = per;
   while (span % 128 != 0 && span < a.c) span += per;
   if (span % 128 != 0 || a.c % span != 0) span = a.c;
-  const int lanes = (span + 127) / 128 * 16;
-  const bool held = a.pixels <= (long)HELD * (LANES / lanes);
+  const int lanes = (span + 127) / 128 * 16, held = a.pixels <= 8 * (ONE / lanes) ? ONE : a.pixels <= 8 * (1024 / lanes) ? 1024 : 0;
   a.span = held ? span : a.c;
   // Otherwise a workgroup a part of at least four rounds of pixels, one for each CU.
-  const int px = LANES / ((a.c + 7) / 8);
+  const int wide = (a.c + 7) / 8, of = wide <= 256 && images * a.pixels * wide <= 2048L * ctx->cus ? 256 : 1024;
+  const int px = of / wide;
   const long rounds = (a.pixels + px - 1) / px;
   long parts = std::max(1L, std::min((rounds + 3) / 4, ctx->cus / images));
   a.chunk = std::min((rounds + parts - 1) / parts, (1L << 30) / px) * px;  // (counted in 32 bits)
@@ -359,13 +377,18 @@ ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_b
   auto go = [&](auto t, auto u, long many) {
     using T = decltype(t);
     using Y = decltype(u);
-    const size_t shared = (size_t)(held ? a.span / per : a.groups) * sizeof(float2);
-    if (held) {
-      hipLaunchKernelGGL((k_norm_held<T, Y>), dim3((unsigned)(many * (a.c / a.span))), dim3(LANES), shared, ctx->stream, a);
+    const unsigned shared = (unsigned)((held ? a.span / per : a.groups) * sizeof(float2));
+    const dim3 spans((unsigned)(many * (a.c / a.span))), grid((unsigned)(many * a.chunks));
+    if (held == ONE) {
+      hipLaunchKernelGGL((k_norm_one<T, Y, ONE>), spans, dim3(ONE), shared, ctx->stream, a);
+    } else if (held) {
+      hipLaunchKernelGGL((k_norm_one<T, Y, 1024>), spans, dim3(1024), shared, ctx->stream, a);
+    } else if (of == 256) {
+      hipLaunchKernelGGL((k_norm_stats<T, 256>), grid, dim3(256), 0, ctx->stream, a);
+      hipLaunchKernelGGL((k_norm_apply<T, Y, 256>), grid, dim3(256), shared, ctx->stream, a);
     } else {
-      const dim3 grid((unsigned)(many * a.chunks));
-      hipLaunchKernelGGL(k_norm_stats<T>, grid, dim3(LANES), 0, ctx->stream, a);
-      hipLaunchKernelGGL((k_norm_apply<T, Y>), grid, dim3(LANES), shared, ctx->stream, a);
+      hipLaunchKernelGGL((k_norm_stats<T, 1024>), grid, dim3(1024), 0, ctx->stream, a);
+      hipLaunchKernelGGL((k_norm_apply<T, Y, 1024>), grid, dim3(1024), shared, ctx->stream, a);
     }
   };
   const int x_bytes = type == IEN_OUT_F16 ? 2 : 4;

@@ -450,7 +450,7 @@ Plan8 plan8(int cus, long workspace, long rows, long n, int chunks, bool f32, bo
       const int deep = (chunks + ks - 1) / ks;
       if ((chunks + deep - 1) / deep != ks) continue;
       const long rounds = (tiles * ks + cus - 1) / cus;
-      double us = (rounds == 1 ? c.alone : rounds * c.among) * deep * (f32 ? 1.5 : 1.0) + rounds * c.out * (add ? 2 : 1);
+      double us = (rounds == 1 ? c.alone : rounds * c.among) * deep * (f32 ? 1.5 : 1.0) + rounds * (c.out + (t == 0 && add ? 8.0 : 0.0));
       if (ks > 1) us += 5.0 + 1e-6 * (double)(tiles * ks) * c.tm * c.tn * 3;
       if (us < best.us) best = {t, ks, us};
     }
