@@ -34,16 +34,22 @@ struct NormArgs {
   uint8_t *scales;
   long scale_stride;
   int span;     // channels a workgroup handles (c, or a part in one launch)
+  int px;       // pixels side by side in one launch
   int chunks;   // parts of an image's pixels
   long chunk;   // pixels of a part
   float2 *part;  // [image][chunk][group]: mean and squares
 };
 
-// LANES: of a workgroup.
-template <int LANES>
+constexpr int LANES = 1024;  // of a workgroup, at most
+
+// LDS of a workgroup's lanes while they join: a count, and the means and
+// squares of up to eight runs of channels, [run][lane].
 struct Shared {
-  float m[8 * LANES], q[8 * LANES], n[LANES];  // [channel of the eight][lane]
+  float *n, *m, *q;
+  int lanes;
+  __device__ __forceinline__ Shared(float *p) : n(p), m(p + blockDim.x), q(m + 8 * blockDim.x), lanes(blockDim.x) {}
 };
+inline size_t shared_floats(int lanes) { return (size_t)17 * lanes; }
 
 // (m1, q1) of n1 joined with (m2, q2): w = n2 / (n1 + n2), nw = n1 w.
 __device__ __forceinline__ void join(float &m1, float &q1, float m2, float q2, float w, float nw) {
@@ -55,25 +61,30 @@ __device__ __forceinline__ void join(float &m1, float &q1, float m2, float q2, f
 __device__ __forceinline__ float share(float n2, float n) { return n > 0.0f ? n2 * __builtin_amdgcn_rcpf(n) : 0.0f; }
 
 // `eights` lanes a pixel, px pixels side by side.
-template <int LANES>
 struct Place {
   int eights, px, slot, eight;
-  __device__ __forceinline__ Place(int span, int round) {
+  __device__ __forceinline__ Place(int span, int round, int pixels) {
     eights = (span / 8 + (span % 8 != 0) + round - 1) / round * round;
-    px = LANES / eights;
+    px = pixels ? pixels : (int)blockDim.x / eights;
     slot = threadIdx.x / eights;
     eight = threadIdx.x - slot * eights;
     if (slot >= px) eight = eights;  // (idle)
   }
 };
 
-// Eight channels of a pixel; past the end zeros.
+// Eight channels of a pixel as they are; past the end zeros.  EIGHTS: c is in
+// eights, and no branch stands between the loads of a batch.
 template <typename T>
-__device__ __forceinline__ void load_eight(const T *row, int at, int c, float *v) {
-  if (at + 8 <= c)
-    load8<T, true>(row, at, c, v);
-  else
-    load8<T, false>(row, at, c, v);
+using Eight = T __attribute__((ext_vector_type(8)));
+template <bool EIGHTS, typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T *row, int at, int c) {
+  typedef Eight<T> Any __attribute__((aligned(sizeof(T))));
+  if (EIGHTS || at + 8 <= c) return *(const Any *)(row + at);
+  Eight<T> v = {};
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (at + i < c) v[i] = row[at + i];
+  return v;
 }
 
 // U pixels' values, the first `many` of them counted (ALL: all), into a lane's
@@ -104,8 +115,8 @@ __device__ __forceinline__ void take(const float (&v)[U][8], int many, float &n,
 // The lanes' statistics of the workgroup's channels, joined by group: f(group
 // of the span, mean, squares), one lane a group.  Channels first, where a lane's
 // eight have a group in common: runs of W = gcd(per, 8) channels.
-template <int LANES, typename F>
-__device__ __forceinline__ void by_group(Shared<LANES> &s, const Place<LANES> &p, float n, float (&m)[8], float (&q)[8], int span,
+template <typename F>
+__device__ __forceinline__ void by_group(const Shared &s, const Place &p, float n, float (&m)[8], float (&q)[8], int span,
                                          int per, F f) {
   const int t = threadIdx.x, W = per & 7 ? per & -per : 8, runs = 8 / W;
   auto pairs = [&](auto width) {  // runs of `width` to runs of twice as many
@@ -123,7 +134,7 @@ __device__ __forceinline__ void by_group(Shared<LANES> &s, const Place<LANES> &p
   s.n[t] = n;
 #pragma unroll
   for (int i = 0; i < 8; i++)
-    if (i < runs) s.m[i * LANES + t] = m[i], s.q[i * LANES + t] = q[i];
+    if (i < runs) s.m[i * s.lanes + t] = m[i], s.q[i * s.lanes + t] = q[i];
   int width = 1;
   while (width < p.px) width *= 2;
   for (int w = width / 2; w >= 1; w /= 2) {
@@ -136,17 +147,17 @@ __device__ __forceinline__ void by_group(Shared<LANES> &s, const Place<LANES> &p
 #pragma unroll
       for (int i = 0; i < 8; i++)
         if (i < runs) {
-          join(m[i], q[i], s.m[i * LANES + o], s.q[i * LANES + o], k, nk);
-          s.m[i * LANES + t] = m[i], s.q[i * LANES + t] = q[i];
+          join(m[i], q[i], s.m[i * s.lanes + o], s.q[i * s.lanes + o], k, nk);
+          s.m[i * s.lanes + t] = m[i], s.q[i * s.lanes + t] = q[i];
         }
     }
   }
   __syncthreads();
   const float each = s.n[0] * W;  // values of a run
   const int many = per / W;       // runs of a group
-  auto at = [&](int r) { return (r & (runs - 1)) * LANES + r / runs; };
+  auto at = [&](int r) { return (r & (runs - 1)) * s.lanes + r / runs; };
   if (many <= 8) {
-    for (int g = t; g < span / per; g += LANES) {
+    for (int g = t; g < span / per; g += s.lanes) {
       float mean = 0.0f, squares = 0.0f;
       for (int r = 0; r < many; r++) mean += s.m[at(g * many + r)];
       mean /= (float)many;
@@ -157,7 +168,7 @@ __device__ __forceinline__ void by_group(Shared<LANES> &s, const Place<LANES> &p
       f(g, mean, squares);
     }
   } else {
-    for (int g = t >> 6; g < span / per; g += LANES / 64) {
+    for (int g = t >> 6; g < span / per; g += s.lanes >> 6) {
       float mean = 0.0f, squares = 0.0f;
       for (int r = t & 63; r < many; r += 64) mean += s.m[at(g * many + r)];
       mean = group_sum<64>(mean) / (float)many;
@@ -172,35 +183,39 @@ __device__ __forceinline__ void by_group(Shared<LANES> &s, const Place<LANES> &p
 }
 
 // A lane's statistics of its `left` pixels from x on, `step` apart.
-template <typename T>
+template <bool EIGHTS, typename T>
 __device__ __forceinline__ void gather(const T *x, long step, int left, int at, int c, float &n, float (&m)[8],
                                        float (&q)[8]) {
   constexpr int U = sizeof(T) == 2 ? 8 : 4;
-  float v[U][8];
-  for (; left >= U; left -= U, x += U * step) {
+  auto batch = [&](auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    Eight<T> x8[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) load_eight(x + u * step, at, c, v[u]);
-    take<true>(v, U, n, m, q);
-  }
-  if (left > 0) {
+    for (int u = 0; u < U; u++) x8[u] = load_eight<EIGHTS>(x + (ALL || u < left ? u : 0) * step, at, c);
+    float v[U][8];
 #pragma unroll
-    for (int u = 0; u < U; u++) load_eight(x + (u < left ? u : 0) * step, at, c, v[u]);
-    take<false>(v, left, n, m, q);
-  }
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[u][i] = (float)x8[u][i];
+    take<ALL>(v, left, n, m, q);
+  };
+  for (; left >= U; left -= U, x += U * step) batch(Act<1>{});
+  if (left > 0) batch(Act<0>{});
 }
 
 // A part of an image's pixels: its groups' means and squares.
-template <typename T, int LANES>
+template <typename T, bool EIGHTS>
 __global__ __launch_bounds__(LANES) void k_norm_stats(NormArgs a) {
-  __shared__ Shared<LANES> s;
-  const Place<LANES> p(a.c, 1);
+  extern __shared__ float lds[];
+  const Shared s(lds);
+  const Place p(a.c, 1, 0);
   const int image = blockIdx.x / a.chunks, part = blockIdx.x % a.chunks, at = p.eight * 8;
   const long begin = part * a.chunk;
   const int many = (int)min(a.chunk, a.pixels - begin);
   const T *x = (const T *)a.x + (image * a.pixels + begin + p.slot) * a.stride;
   float n = 0.0f, m[8] = {}, q[8] = {};
   if (p.eight < p.eights)
-    gather(x, p.px * a.stride, (unsigned)(many - p.slot + p.px - 1) / (unsigned)p.px, at, a.c, n, m, q);
+    gather<EIGHTS>(x, p.px * a.stride, (unsigned)(many - p.slot + p.px - 1) / (unsigned)p.px, at, a.c, n, m, q);
   float2 *out = a.part + (long)blockIdx.x * a.groups;
   by_group(s, p, n, m, q, a.c, a.c / a.groups, [&](int g, float mean, float squares) { out[g] = {mean, squares}; });
 }
@@ -212,8 +227,13 @@ struct Line {
     const int per = a.c / a.groups;
 #pragma unroll
     for (int i = 0; i < 8; i++) gain[i] = 1.0f, bias[i] = 0.0f;
-    if (a.gamma) load_eight(a.gamma + c0, at, a.span, gain);
-    if (a.beta) load_eight(a.beta + c0, at, a.span, bias);
+    auto get = [&](const float *from, float *to) {
+      const Eight<float> v = load_eight<false>(from + c0, at, a.span);
+#pragma unroll
+      for (int i = 0; i < 8; i++) to[i] = v[i];
+    };
+    if (a.gamma) get(a.gamma, gain);
+    if (a.beta) get(a.beta, bias);
     int g = at / per, in = at - g * per;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -226,7 +246,7 @@ struct Line {
 };
 
 // Eight results of pixel r from channel c0 + at on (`at` within the span).
-template <typename Y, int ACT>
+template <typename Y, bool EIGHTS, int ACT>
 __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, int c0, int at, float *v) {
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = act8<ACT>((v[i] - l.mean[i]) * l.gain[i] + l.bias[i]);
@@ -234,7 +254,7 @@ __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, in
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      if (at + i >= a.span) v[i] = 0.0f;
+      if (!EIGHTS && at + i >= a.span) v[i] = 0.0f;
       top = fmaxf(top, finite_magnitude(v[i]));
     }
     const int e = exponent8(max16(top));
@@ -242,26 +262,43 @@ __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, in
     if ((at & 127) == 0) a.scales[r * a.scale_stride + (c0 + at) / 128] = (uint8_t)(e + 127);
   } else {
     Y *y = (Y *)a.y + r * a.ystride + c0;
-    if (at + 8 <= a.span)
+    if (EIGHTS || at + 8 <= a.span)
       store8<Y, true>(y, at, a.span, v);
     else
       store8<Y, false>(y, at, a.span, v);
   }
 }
 
-// A lane's `count` pixels r, r + px, ... from x on, `step` apart, from the last.
-template <typename T, typename Y>
-__device__ __forceinline__ void apply(const NormArgs &a, const Line &l, const T *x, long step, int count, long r, int px,
-                                      int c0, int at) {
-  constexpr int U = sizeof(T) == 2 ? 4 : 2;
+// A lane's `count` pixels r, r + px, ... from x on, `step` apart, from the last:
+// a batch is loaded while the one after it (the first one by the caller) is written.
+template <typename T>
+constexpr int BATCH = sizeof(T) == 2 ? 4 : 2;
+template <bool EIGHTS, typename T>
+__device__ __forceinline__ void load_batch(Eight<T> (&to)[BATCH<T>], const T *x, long step, int k, int count, int at, int c) {
+#pragma unroll
+  for (int u = 0; u < BATCH<T>; u++) to[u] = load_eight<EIGHTS>(x + max(min(k + u, count - 1), 0) * step, at, c);
+}
+template <typename T>
+__device__ __forceinline__ int last_batch(int count) {
+  return (count - 1) / BATCH<T> * BATCH<T>;
+}
+template <bool EIGHTS, typename T, typename Y>
+__device__ __forceinline__ void apply(const NormArgs &a, const Line &l, Eight<T> (&now)[BATCH<T>], const T *x, long step,
+                                      int count, long r, int px, int c0, int at) {
+  constexpr int U = BATCH<T>;
   with_act8(a.act, [&](auto act) {
-    for (int k = (count - 1) / U * U; k >= 0; k -= U) {
-      float v[U][8];
+    for (int k = last_batch<T>(count); k >= 0; k -= U) {
+      Eight<T> next[U];
+      load_batch<EIGHTS>(next, x, step, k - U, count, at, a.span);
 #pragma unroll
-      for (int u = 0; u < U; u++) load_eight(x + min(k + u, count - 1) * step, at, a.span, v[u]);
+      for (int u = 0; u < U; u++) {
+        float v[8];
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (k + u < count) put<Y, decltype(act)::value>(a, l, r + (long)(k + u) * px, c0, at, v[u]);
+        for (int i = 0; i < 8; i++) v[i] = (float)now[u][i];
+        if (k + u < count) put<Y, EIGHTS, decltype(act)::value>(a, l, r + (long)(k + u) * px, c0, at, v);
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) now[u] = next[u];
     }
   });
 }
@@ -269,26 +306,38 @@ __device__ __forceinline__ void apply(const NormArgs &a, const Line &l, const T 
 // The parts' statistics joined, and the same part of the pixels again, from its
 // end.  The parts' means are summed from the first one's on, then the squares
 // about their mean; all but the last part hold a.chunk pixels.
-template <typename T, typename Y, int LANES>
+template <typename T, typename Y, bool EIGHTS>
 __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
-  constexpr int HERE = 8192 / LANES;  // parts a lane keeps for the second sum
-  __shared__ float sums[LANES], means[LANES];
-  extern __shared__ float2 stats[];  // [group]: mean, 1 / deviation
+  constexpr int HERE = 16;  // parts a lane keeps for the second sum
+  extern __shared__ float lds[];
+  const int lanes = blockDim.x;
+  float *sums = lds, *means = lds + lanes;
+  float2 *stats = (float2 *)(means + lanes);  // [group]: mean, 1 / deviation
   const int t = threadIdx.x, per = a.c / a.groups, image = blockIdx.x / a.chunks, mine = blockIdx.x % a.chunks;
+  const Place p(a.c, sizeof(Y) == 1 ? 16 : 1, 0);
+  const int at = p.eight * 8;
+  const long begin = mine * a.chunk, r0 = image * a.pixels + begin + p.slot, step = p.px * a.stride;
+  const T *x = (const T *)a.x + r0 * a.stride;
+  const int count =
+      p.eight < p.eights ? (unsigned)((int)min(a.chunk, a.pixels - begin) - p.slot + p.px - 1) / (unsigned)p.px : 0;
+  Eight<T> now[BATCH<T>];
+  if (count > 0) load_batch<EIGHTS>(now, x, step, last_batch<T>(count), count, at, a.c);
+
   const float whole = (float)a.chunk, last = (float)(a.pixels - (a.chunks - 1) * a.chunk);
-  for (int g0 = 0; g0 < a.groups; g0 += LANES) {
-    const int many = min(a.groups - g0, LANES), rows = LANES / many, row = t / many, g = t - row * many;
+  for (int g0 = 0; g0 < a.groups; g0 += lanes) {
+    const int many = min(a.groups - g0, lanes), rows = lanes / many, row = t / many, g = t - row * many;
     const float2 *part = a.part + (long)image * a.chunks * a.groups + g0 + g;
     const float base = part[0].x;
     // A lane's parts row, row + rows, ...: f(its mean and squares, its pixels).
     float2 v[HERE];
 #pragma unroll
-    for (int i = 0; i < HERE; i++) v[i] = part[(long)min(row + i * rows, a.chunks - 1) * a.groups];
+    for (int i = 0; i < HERE; i++)
+      if (i * rows < a.chunks) v[i] = part[(long)min(row + i * rows, a.chunks - 1) * a.groups];
     auto each = [&](auto f) {
 #pragma unroll
       for (int i = 0; i < HERE; i++) {
         const int k = row + i * rows;
-        f(v[i], k >= a.chunks ? 0.0f : k == a.chunks - 1 ? last : whole);
+        if (i * rows < a.chunks) f(v[i], k >= a.chunks ? 0.0f : k == a.chunks - 1 ? last : whole);
       }
       for (int k = row + HERE * rows; k < a.chunks; k += rows) f(part[(long)k * a.groups], k == a.chunks - 1 ? last : whole);
     };
@@ -318,30 +367,32 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
     __syncthreads();
   }
 
-  const Place<LANES> p(a.c, sizeof(Y) == 1 ? 16 : 1);
-  const int at = p.eight * 8;
-  if (p.eight >= p.eights) return;
+  if (count <= 0) return;
   Line l;
   l.set(a, 0, at, stats);
-  const long begin = mine * a.chunk, r0 = image * a.pixels + begin + p.slot;
-  const int count = (unsigned)((int)min(a.chunk, a.pixels - begin) - p.slot + p.px - 1) / (unsigned)p.px;
-  if (count > 0) apply<T, Y>(a, l, (const T *)a.x + r0 * a.stride, p.px * a.stride, count, r0, p.px, 0, at);
+  apply<EIGHTS, T, Y>(a, l, now, x, step, count, r0, p.px, 0, at);
 }
 
 // One launch: a workgroup a span of whole groups (and blocks of 128 channels)
-// of an image.
-template <typename T, typename Y, int LANES>
+// of an image, a.px lanes an eight whatever the span (so that the statistics do
+// not depend on it).
+template <typename T, typename Y, bool EIGHTS>
 __global__ __launch_bounds__(LANES) void k_norm_one(NormArgs a) {
-  __shared__ Shared<LANES> s;
-  extern __shared__ float2 stats[];
-  const Place<LANES> p(a.span, 16);
+  extern __shared__ float lds[];
+  const Shared s(lds);
+  float2 *stats = (float2 *)(lds + 17 * blockDim.x);
+  const Place p(a.span, sizeof(Y) == 1 ? 16 : 1, a.px);
   const int spans = a.c / a.span, image = blockIdx.x / spans, c0 = blockIdx.x % spans * a.span, at = p.eight * 8;
   const int per = a.c / a.groups;
   const long r0 = image * a.pixels + p.slot;
   const T *x = (const T *)a.x + r0 * a.stride + c0;
   const int count = p.eight < p.eights ? (unsigned)((int)a.pixels - p.slot + p.px - 1) / (unsigned)p.px : 0;
   float n = 0.0f, m[8] = {}, q[8] = {};
-  gather(x, p.px * a.stride, count, at, a.span, n, m, q);
+  Eight<T> now[BATCH<T>];
+  if (count > 0) {
+    gather<EIGHTS>(x, p.px * a.stride, count, at, a.span, n, m, q);
+    load_batch<EIGHTS>(now, x, p.px * a.stride, last_batch<T>(count), count, at, a.span);
+  }
   by_group(s, p, n, m, q, a.span, per, [&](int g, float mean, float squares) {
     stats[g] = {mean, 1.0f / sqrtf(squares / ((float)a.pixels * per) + a.eps)};
   });
@@ -349,47 +400,53 @@ __global__ __launch_bounds__(LANES) void k_norm_one(NormArgs a) {
   if (count == 0) return;
   Line l;
   l.set(a, c0, at, stats);
-  apply<T, Y>(a, l, x, p.px * a.stride, count, r0, p.px, c0, at);
+  apply<EIGHTS, T, Y>(a, l, now, x, p.px * a.stride, count, r0, p.px, c0, at);
 }
 
-constexpr int ONE = 512;  // lanes of one launch's workgroups
+// The smallest run of whole groups and multiples of `unit` channels that c is made of.
+int smallest_span(int c, int per, int unit) {
+  int span = per;
+  while (span % unit != 0 && span < c) span += per;
+  return span % unit == 0 && c % span == 0 ? span : c;
+}
 
 ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_bytes) {
   const int per = a.c / a.groups;
-  // One launch where a lane's share is a few pixels of the smallest span of
-  // whole groups and blocks of 128 channels.
-  int span = per;
-  while (span % 128 != 0 && span < a.c) span += per;
-  if (span % 128 != 0 || a.c % span != 0) span = a.c;
-  const int lanes = (span + 127) / 128 * 16, held = a.pixels <= 8 * (ONE / lanes) ? ONE : a.pixels <= 8 * (1024 / lanes) ? 1024 : 0;
-  a.span = held ? span : a.c;
-  // Otherwise a workgroup a part of at least four rounds of pixels, one for each CU.
-  const int wide = (a.c + 7) / 8, of = wide <= 256 && images * a.pixels * wide <= 2048L * ctx->cus ? 256 : 1024;
-  const int px = of / wide;
-  const long rounds = (a.pixels + px - 1) / px;
-  long parts = std::max(1L, std::min((rounds + 3) / 4, ctx->cus / images));
+  // One launch where a lane's share is a few pixels.
+  const int wide = smallest_span(a.c, per, 128);
+  a.px = std::min(64, LANES / ((wide + 127) / 128 * 16));
+  const bool one = a.pixels <= 8 * a.px;
+  a.span = !one ? a.c : y_bytes == 1 ? wide : smallest_span(a.c, per, 8);
+  const int eights = (a.span + 7) / 8, one_lanes = ((y_bytes == 1 ? (eights + 15) / 16 * 16 : eights) * a.px + 63) / 64 * 64;
+  // Otherwise a workgroup a part of at least four rounds of pixels: one for each
+  // CU of a long map; of a shorter one, whose second pass spends most of its time on
+  // joining the parts, one for every other CU.
+  const int lanes = eights <= 512 ? 512 : LANES, px = lanes / eights;
+  const long rounds = (a.pixels + px - 1) / px, most_parts = images * a.pixels * eights > 2048L * ctx->cus ? ctx->cus : ctx->cus / 2;
+  const long parts = std::max(1L, std::min((rounds + 3) / 4, most_parts / images));
   a.chunk = std::min((rounds + parts - 1) / parts, (1L << 30) / px) * px;  // (counted in 32 bits)
   a.chunks = (int)((a.pixels + a.chunk - 1) / a.chunk);
   a.part = (float2 *)ctx->splitk;
-  const long most = held ? 1L << 16 : std::max(1L, (long)(ctx->splitk_floats / 2) / ((long)a.chunks * a.groups));
+  const long most = one ? 1L << 16 : std::max(1L, (long)(ctx->splitk_floats / 2) / ((long)a.chunks * a.groups));
   const void *x = a.x;
   uint8_t *y = (uint8_t *)a.y, *scales = a.scales;
-  auto go = [&](auto t, auto u, long many) {
+  auto go_eights = [&](auto t, auto u, auto e, long many) {
     using T = decltype(t);
     using Y = decltype(u);
-    const unsigned shared = (unsigned)((held ? a.span / per : a.groups) * sizeof(float2));
-    const dim3 spans((unsigned)(many * (a.c / a.span))), grid((unsigned)(many * a.chunks));
-    if (held == ONE) {
-      hipLaunchKernelGGL((k_norm_one<T, Y, ONE>), spans, dim3(ONE), shared, ctx->stream, a);
-    } else if (held) {
-      hipLaunchKernelGGL((k_norm_one<T, Y, 1024>), spans, dim3(1024), shared, ctx->stream, a);
-    } else if (of == 256) {
-      hipLaunchKernelGGL((k_norm_stats<T, 256>), grid, dim3(256), 0, ctx->stream, a);
-      hipLaunchKernelGGL((k_norm_apply<T, Y, 256>), grid, dim3(256), shared, ctx->stream, a);
+    constexpr bool E = decltype(e)::value;
+    if (one) {
+      const size_t shared = shared_floats(one_lanes) * 4 + a.span / per * sizeof(float2);
+      hipLaunchKernelGGL((k_norm_one<T, Y, E>), dim3((unsigned)(many * (a.c / a.span))), dim3(one_lanes), shared, ctx->stream, a);
     } else {
-      hipLaunchKernelGGL((k_norm_stats<T, 1024>), grid, dim3(1024), 0, ctx->stream, a);
-      hipLaunchKernelGGL((k_norm_apply<T, Y, 1024>), grid, dim3(1024), shared, ctx->stream, a);
+      const dim3 grid((unsigned)(many * a.chunks));
+      hipLaunchKernelGGL((k_norm_stats<T, E>), grid, dim3(lanes), shared_floats(lanes) * 4, ctx->stream, a);
+      hipLaunchKernelGGL((k_norm_apply<T, Y, E>), grid, dim3(lanes), 2 * lanes * 4 + a.groups * sizeof(float2), ctx->stream, a);
     }
+  };
+  // (Lanes past a row in 8 bits write zeros: they are no whole eights.)
+  const bool in_eights = a.c % (y_bytes == 1 ? 128 : 8) == 0;
+  auto go = [&](auto t, auto u, long many) {
+    in_eights ? go_eights(t, u, Act<1>{}, many) : go_eights(t, u, Act<0>{}, many);
   };
   const int x_bytes = type == IEN_OUT_F16 ? 2 : 4;
   for (long i = 0; i < images; i += most) {  // (one turn but for a great many images)
