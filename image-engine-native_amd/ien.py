@@ -9,6 +9,7 @@ missing or unloadable library raises.
 
 import ctypes
 import pathlib
+import struct
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libien_hip.so"
@@ -214,19 +215,19 @@ def load():
         L.ien_spectral_work.argtypes = [vp]
         L.ien_spectral_work.restype = sz
         L.ien_spectral_run.argtypes = [vp, vp, sz, vp, vp, vp, vp, vp, vp, sz]
-        rp, fl = ctypes.POINTER(Rows8Struct), ctypes.c_float
+        fl = ctypes.c_float
         L.ien_rows8_stride.argtypes = [sz]
         L.ien_rows8_stride.restype = sz
         L.ien_rows8_scale_stride.argtypes = [sz]
         L.ien_rows8_scale_stride.restype = sz
-        L.ien_quantize8.argtypes = [vp, vp, i, sz, sz, sz, rp]
-        L.ien_dequantize8.argtypes = [vp, rp, sz, sz, vp, i, sz]
+        L.ien_quantize8.argtypes = [vp, vp, i, sz, sz, sz, vp]
+        L.ien_dequantize8.argtypes = [vp, vp, sz, sz, vp, i, sz]
         L.ien_matrix8_new.argtypes = [vp, vp, i, sz, sz, sz, vp, ctypes.POINTER(vp)]
         L.ien_matrix8_free.argtypes = [vp]
         L.ien_matrix8_free.restype = None
-        L.ien_multiply8.argtypes = [vp, ctypes.POINTER(Input8), sz, sz, vp, ctypes.POINTER(Output), i, vp, sz]
+        L.ien_multiply8.argtypes = [vp, vp, sz, sz, vp, vp, i, vp, sz]
         L.ien_group_norm.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, vp, i, sz]
-        L.ien_group_norm8.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, rp]
+        L.ien_group_norm8.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, vp]
         for name in EXPORTS:
             getattr(L, name)
         _lib = L
@@ -584,7 +585,8 @@ class Swin:
 class Rows8:
     """ien_rows8 over torch tensors: `rows` rows of k values in 8 bits (data:
     uint8 [rows, stride], scales: uint8 [rows, scale_stride]), made here
-    unless given.  Row i of `row0 = i` views starts there."""
+    unless given.  The tensors stay this object's (their addresses are read
+    once, here); another Rows8 takes other ones, views of these among them."""
 
     def __init__(self, rows, k, data=None, scales=None, device="cuda"):
         import torch
@@ -597,12 +599,18 @@ class Rows8:
         for t in (data, scales):
             if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
                 raise ValueError("rows in 8 bits are uint8 tensors of rows x bytes")
-        self.rows, self.k, self.data, self.scales = rows, k, data, scales
+        if data.device != scales.device:
+            raise ValueError(f"rows in 8 bits on {data.device} and {scales.device}")
+        self.rows, self.k, self._data, self._scales = rows, k, data, scales
+        self._fields = data.data_ptr(), _row_stride(data), scales.data_ptr(), _row_stride(scales)
+        self._struct = Rows8Struct(*self._fields)
+        self._at = ctypes.addressof(self._struct)
+
+    data = property(lambda self: self._data)
+    scales = property(lambda self: self._scales)
 
     def struct(self):
-        s = Rows8Struct(self.data.data_ptr(), _row_stride(self.data), self.scales.data_ptr(), _row_stride(self.scales))
-        s._tensors = self.data, self.scales  # raw pointers: keep their storage alive
-        return s
+        return self._struct
 
 
 def _row_stride(t):
@@ -612,28 +620,52 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-def _out_type(t):
+# The entry points below are called for steps of a few microseconds: what they
+# check costs as little as it can.  OUT_F16 and OUT_F32 by torch's types.
+_OUT_TYPES = {}
+
+
+def _out_type(dtype):
+    if dtype in _OUT_TYPES:
+        return _OUT_TYPES[dtype]
     import torch
 
-    if t.dtype not in (torch.float16, torch.float32):
-        raise ValueError(f"f16 or f32 expected, not {t.dtype}")
-    return OUT_F16 if t.dtype == torch.float16 else OUT_F32
+    _OUT_TYPES.update({torch.float16: OUT_F16, torch.float32: OUT_F32})
+    if dtype not in _OUT_TYPES:
+        raise ValueError(f"f16 or f32 expected, not {dtype}")
+    return _OUT_TYPES[dtype]
+
+
+def _rows_of(t):
+    """(rows, columns, address, type, stride) of a tensor of rows on the GPU."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError("rows x channels with contiguous channels expected")
+    rows, c = shape
+    stride = strides[0]
+    if not t.is_cuda:
+        raise ValueError(f"a tensor on the GPU expected, not on {t.device}")
+    return rows, c, t.data_ptr(), _out_type(t.dtype), stride if rows > 1 or stride > c else c
 
 
 def quantize8(ctx, x, out):
     """Rows x k (f16 or f32 tensor) into the Rows8 `out`."""
-    if tuple(x.shape) != (out.rows, out.k):
+    rows, k, at, kind, stride = _rows_of(x)
+    if rows != out.rows or k != out.k:
         raise ValueError(f"{tuple(x.shape)} into {out.rows} rows of {out.k}")
-    check(load().ien_quantize8(ctx.h, _ptr(x), _out_type(x), out.rows, out.k, _row_stride(x),
-                               ctypes.byref(out.struct())))
+    status = (_lib or load()).ien_quantize8(ctx.h, at, kind, rows, k, stride, out._at)
+    if status:
+        check(status)
 
 
 def dequantize8(ctx, x, y):
     """The values of the Rows8 `x` into the rows x k tensor y (f16 or f32)."""
-    if tuple(y.shape) != (x.rows, x.k):
+    rows, k, at, kind, stride = _rows_of(y)
+    if rows != x.rows or k != x.k:
         raise ValueError(f"{x.rows} rows of {x.k} into {tuple(y.shape)}")
-    check(load().ien_dequantize8(ctx.h, ctypes.byref(x.struct()), x.rows, x.k, _ptr(y), _out_type(y),
-                                 _row_stride(y)))
+    status = (_lib or load()).ien_dequantize8(ctx.h, x._at, rows, k, at, kind, stride)
+    if status:
+        check(status)
 
 
 class Matrix8:
@@ -669,52 +701,74 @@ class Matrix8:
             pass
 
 
-def _multiply8(ctx, inp, row0, rows, c, matrix, out, act, add):
-    if c != matrix.c or tuple(out.shape) != (rows, matrix.n):
-        raise ValueError(f"rows of {c} by {matrix.c} x {matrix.n} into {tuple(out.shape)}")
-    if add is not None and (add.shape != out.shape or add.dtype != out.dtype):
-        raise ValueError("what is added has the output's shape and type")
-    o = Output(out.data_ptr(), _row_stride(out), NHWC, _out_type(out))
-    check(load().ien_multiply8(ctx.h, ctypes.byref(inp), row0, rows, matrix.h, ctypes.byref(o), act, _ptr(add),
-                               0 if add is None else _row_stride(add)))
+# ien_input8 and ien_output as bytes.
+_INPUT8, _OUTPUT = struct.Struct("@iPNPNNNNN").pack, struct.Struct("@PNii").pack
+
+
+def _multiply8(ctx, x, shape, row0, matrix, out, act, add):
+    rows, n, at, kind, stride = _rows_of(out)
+    if x.k != matrix.c or n != matrix.n:
+        raise ValueError(f"rows of {x.k} by {matrix.c} x {matrix.n} into {tuple(out.shape)}")
+    add_at = None
+    add_stride = 0
+    if add is not None:
+        add_rows, add_n, add_at, add_kind, add_stride = _rows_of(add)
+        if add_rows != rows or add_n != n or add_kind != kind:
+            raise ValueError("what is added has the output's shape and type")
+    status = (_lib or load()).ien_multiply8(ctx.h, _INPUT8(shape[0], *x._fields, *shape[1:]), row0, rows, matrix.h,
+                                            _OUTPUT(at, stride, NHWC, kind), act, add_at, add_stride)
+    if status:
+        check(status)
 
 
 def multiply8(ctx, x, matrix, out, act=ACT_NONE, add=None, row0=0):
     """out = act(x . w + bias + add): rows row0 .. of the Rows8 x, as many as
     out (rows x n, f16 or f32) has; `add` like out, or out itself."""
-    if row0 + out.shape[0] > x.rows:
+    if row0 < 0 or row0 + out.shape[0] > x.rows:
         raise ValueError(f"rows {row0} .. {row0 + out.shape[0]} of {x.rows}")
-    _multiply8(ctx, Input8(INPUT_ROWS, x.struct(), 1, 1, x.rows, 1), row0, out.shape[0], x.k, matrix, out, act, add)
+    _multiply8(ctx, x, (INPUT_ROWS, 1, 1, x.rows, 1), row0, matrix, out, act, add)
 
 
 def conv8(ctx, x, images, height, width, matrix, out, step=1, act=ACT_NONE, add=None, row0=0):
     """The same for a 3 x 3 (9 taps) or 1 x 1 convolution of `images` maps of
     height x width pixels in 8 bits, zero padding: output pixels row0 .., as
     many as out has rows."""
-    if images * height * width != x.rows:
-        raise ValueError(f"{images} maps of {height} x {width} in {x.rows} rows")
-    _multiply8(ctx, Input8(INPUT_IMAGE, x.struct(), images, height, width, step), row0, out.shape[0], x.k, matrix, out,
-               act, add)
+    if images * height * width != x.rows or images < 0 or height < 0 or width < 0 or row0 < 0 or step not in (1, 2):
+        raise ValueError(f"{images} maps of {height} x {width} in {x.rows} rows, step {step}, from row {row0}")
+    _multiply8(ctx, x, (INPUT_IMAGE, images, height, width, step), row0, matrix, out, act, add)
+
+
+def _channels_of(t, c):
+    """The address of c f32 values on the GPU, or None."""
+    if t is None:
+        return None
+    if t.shape != (c,) or not t.is_cuda or not t.is_contiguous() or _out_type(t.dtype) != OUT_F32:
+        raise ValueError(f"gamma and beta are {c} contiguous f32 values on the GPU")
+    return t.data_ptr()
 
 
 def group_norm(ctx, x, images, groups, gamma, beta, y, eps=1e-5, act=ACT_NONE):
     """act(group norm) of `images` maps of x.shape[0] / images pixels (x: rows x
     channels, f16 or f32) into y: a tensor of x's shape (f16 or f32, x itself
     too), or a Rows8.  gamma, beta: f32 tensors, or None for 1 and 0."""
-    rows, c = x.shape
+    rows, c, at, kind, stride = _rows_of(x)
     if images < 1 or rows % images:
         raise ValueError(f"{rows} pixels in {images} maps")
-    for t in (gamma, beta):
-        if t is not None and (tuple(t.shape) != (c,) or str(t.dtype) != "torch.float32" or t.stride(0) != 1 and c > 1):
-            raise ValueError(f"gamma and beta are {c} contiguous f32 values")
-    args = (ctx.h, _ptr(x), _out_type(x), images, rows // images, c, _row_stride(x), groups, _ptr(gamma), _ptr(beta),
-            eps, act)
-    if (y.rows, y.k) != (rows, c) if isinstance(y, Rows8) else tuple(y.shape) != (rows, c):
-        raise ValueError("the result has the input's rows and channels")
     if isinstance(y, Rows8):
-        check(load().ien_group_norm8(*args, ctypes.byref(y.struct())))
+        if y.rows != rows or y.k != c:
+            raise ValueError("the result has the input's rows and channels")
+        status = (_lib or load()).ien_group_norm8(
+            ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(gamma, c), _channels_of(beta, c),
+            eps, act, y._at)
     else:
-        check(load().ien_group_norm(*args, _ptr(y), _out_type(y), _row_stride(y)))
+        y_rows, y_c, y_at, y_kind, y_stride = _rows_of(y)
+        if y_rows != rows or y_c != c:
+            raise ValueError("the result has the input's rows and channels")
+        status = (_lib or load()).ien_group_norm(
+            ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(gamma, c), _channels_of(beta, c),
+            eps, act, y_at, y_kind, y_stride)
+    if status:
+        check(status)
 
 
 def bytes_to_floats(ctx, src, dst):
