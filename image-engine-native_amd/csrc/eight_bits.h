@@ -31,6 +31,10 @@ inline size_t blocks8(size_t k) { return (k + BLOCK8 - 1) / BLOCK8; }
 // Rows in 8 bits that an entry point was handed, or its refusal.
 ien_status check_rows8(const ien_rows8 *r, size_t k, const char *what);
 
+// multiply8.hip: 64 x the tile + the splits of the depth of a product of `rows`
+// rows, `chunks` blocks deep, n outputs.
+int multiply8_choice(int cus, long workspace, long rows, long n, int chunks, bool exact, bool add);
+
 typedef int int2v __attribute__((ext_vector_type(2)));
 
 // The exponent of a block whose largest finite magnitude is `largest`: the

@@ -12,8 +12,11 @@
 // values loses the 1; sums of 64 random products are off by 1.4e-5 of
 // themselves, whatever their accumulator holds).  That is a fortieth of an f16
 // output's own rounding, and as much as f32 outputs would be off in all.
-// Those take their operands as bf16, which holds e4m3 values under any of the
-// scales exactly, and the bf16 instructions (6e-9), at half the rate.
+// Those, and f16 outputs on request, take their operands as bf16, which holds
+// e4m3 values under any of the scales exactly, and the bf16 instructions
+// (6e-9), at half the rate.  (Rounded to 8 bits again after a norm, f16 results
+// off by 1.4e-5 gave a residual block of 64 x 64 x 512 an error of 4.6e-4 in
+// place of 2.2e-4.)
 //
 // A workgroup of four waves computes a tile of rows x outputs, a block of 128
 // deep at a time through a ring of stages in LDS that buffer loads fill without
@@ -46,7 +49,7 @@ struct Args8 {
   long n, npad;
   void *y;
   long ys;
-  int f32, act;
+  int f32, exact, act;  // f32 outputs are exact
   const void *add;
   long as;
   int image, vec;  // a map's pixels; whole eights of outputs
@@ -119,7 +122,7 @@ __device__ __forceinline__ void each(F f) {
   }
 }
 
-template <typename T, bool F32>
+template <typename T, bool EXACT, typename Y>
 __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8(Args8 a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
@@ -257,7 +260,7 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   constexpr int PRODUCTS = T::FM * T::FN;
   // The products of half a block, beside(k) between them.
   auto multiply = [&](const Half &h, const Scales &v, auto beside) {
-    if constexpr (!F32) {
+    if constexpr (!EXACT) {
       each<PRODUCTS>([&](auto k) {
         constexpr int i = decltype(k)::value / T::FN, j = decltype(k)::value % T::FN;
         beside(k);
@@ -266,20 +269,19 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
         __builtin_amdgcn_sched_barrier(0);
       });
     } else {
-      each<PRODUCTS>(beside);
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
+      each<4>([&](auto e) {
+        constexpr int E = 2 * decltype(e)::value;
         bf16x8 x[T::FM], w[T::FN];
 #pragma unroll
-        for (int i = 0; i < T::FM; i++) x[i] = widen8(h.x[i][e], h.x[i][e + 1], scale_power(v.x[i] & 255));
+        for (int i = 0; i < T::FM; i++) x[i] = widen8(h.x[i][E], h.x[i][E + 1], scale_power(v.x[i] & 255));
 #pragma unroll
-        for (int j = 0; j < T::FN; j++) w[j] = widen8(h.w[j][e], h.w[j][e + 1], scale_power(v.w[j]));
-#pragma unroll
-        for (int i = 0; i < T::FM; i++)
-#pragma unroll
-          for (int j = 0; j < T::FN; j++)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[i][j], 0, 0, 0);
-      }
+        for (int j = 0; j < T::FN; j++) w[j] = widen8(h.w[j][E], h.w[j][E + 1], scale_power(v.w[j]));
+        each<PRODUCTS>([&](auto k) {
+          constexpr int i = decltype(k)::value / T::FN, j = decltype(k)::value % T::FN;
+          if constexpr (E == 0) beside(k);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[i][j], 0, 0, 0);
+        });
+      });
     }
   };
 
@@ -350,7 +352,6 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   float *st = (float *)lds + wave * 32 * T::PITCH;
   constexpr int COLS = 32 * T::FN, EIGHTS = COLS / 8, ITEMS = 32 * EIGHTS / 64;
   const long nw = n0 + wn * COLS;
-  using Y = std::conditional_t<F32, float, _Float16>;
   const int row = lane / EIGHTS, col = lane % EIGHTS * 8;
   float bias[8];
   // Eight floats of LDS, 16-byte aligned.
@@ -415,34 +416,58 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   });
 }
 
-struct Plan8 {
-  int tile, ksplit;
-  double us;
-};
-
 // The tiles a launch chooses among, largest first, and what they were measured
 // at: us a block of depth of one tile on a CU alone and among its neighbours,
-// and us a round of tiles for their outputs.
+// with 8-bit and with bf16 instructions, and us a round of tiles for their
+// outputs (with a residual to add, where no second workgroup of the CU hides it).
 struct Choice8 {
   int tm, tn;
-  double alone, among, out;
+  double alone[2], among[2], out, out_add;
 };
-constexpr Choice8 CHOICES8[] = {{256, 256, 1.45, 1.45, 8.0}, {128, 128, 0.58, 0.50, 3.0}, {64, 128, 0.42, 0.34, 1.7},
-                                {64, 64, 0.38, 0.22, 1.2}};
+constexpr Choice8 CHOICES8[] = {{256, 256, {1.45, 2.9}, {1.45, 2.9}, 8.0, 16.0},
+                                {128, 128, {0.58, 0.90}, {0.50, 0.72}, 3.0, 3.0},
+                                {64, 128, {0.42, 0.68}, {0.34, 0.46}, 1.7, 1.7},
+                                {64, 64, {0.38, 0.60}, {0.22, 0.28}, 1.2, 1.2}};
 
-template <typename T, bool F32>
+template <typename T>
 void launch(ien_ctx *ctx, Args8 &a) {
-  hipLaunchKernelGGL((k_tile8<T, F32>), dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)a.ksplit), dim3(T::THREADS), 0,
-                     ctx->stream, a);
+  const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)a.ksplit);
+  if (a.f32)
+    hipLaunchKernelGGL((k_tile8<T, true, float>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  else if (a.exact)
+    hipLaunchKernelGGL((k_tile8<T, true, _Float16>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL((k_tile8<T, false, _Float16>), grid, dim3(T::THREADS), 0, ctx->stream, a);
 }
 
-// The tile, and in how many splits of the depth: by the estimated time.  Few
-// tiles leave CUs idle, which splits fill for a pass through device memory and
-// about 5 us; f32 outputs take twice the matrix time and no 256 x 256 tiles (their
-// operands as bf16 do not fit in registers beside the sums).
-Plan8 plan8(int cus, long workspace, long rows, long n, int chunks, bool f32, bool add) {
-  Plan8 best = {-1, 1, 1e30};
-  for (int t = f32 ? 1 : 0; t < 4; t++) {
+void run_tiles(ien_ctx *ctx, Args8 &a) {
+  const int chunks = a.taps * a.cb;
+  const int plan = multiply8_choice(ctx->cus, (long)ctx->splitk_floats, a.rows, a.n, chunks, a.exact, a.add);
+  const int tile = plan / 64, ksplit = plan % 64;
+  const Choice8 &c = CHOICES8[tile];
+  a.tiles_m = (int)((a.rows + c.tm - 1) / c.tm);
+  a.tiles_n = (int)((a.n + c.tn - 1) / c.tn);
+  a.ksplit = ksplit;
+  a.kchunks = (chunks + ksplit - 1) / ksplit;
+  a.part = ctx->splitk;
+  a.tile_count = (int *)(ctx->splitk + ctx->splitk_floats);
+  switch (tile) {
+    case 0: launch<Tile8<4, 4, 2, 2, 2>>(ctx, a); break;
+    case 1: launch<Tile8<2, 2, 2, 2, 2>>(ctx, a); break;
+    case 2: launch<Tile8<1, 2, 2, 2, 3>>(ctx, a); break;
+    default: launch<Tile8<1, 1, 2, 2, 4>>(ctx, a); break;
+  }
+}
+
+}  // namespace
+
+// The tile (times 64) and in how many splits of the depth: by the estimated
+// time.  Few tiles leave CUs idle, which splits fill for a pass through device
+// memory and about 5 us.
+int multiply8_choice(int cus, long workspace, long rows, long n, int chunks, bool exact, bool add) {
+  int best = -1;
+  double best_us = 1e30;
+  for (int t = 0; t < 4; t++) {
     const Choice8 &c = CHOICES8[t];
     const long tiles = ((rows + c.tm - 1) / c.tm) * ((n + c.tn - 1) / c.tn);
     for (int ks = 1; ks <= 16 && ks <= chunks; ks++) {
@@ -450,33 +475,14 @@ Plan8 plan8(int cus, long workspace, long rows, long n, int chunks, bool f32, bo
       const int deep = (chunks + ks - 1) / ks;
       if ((chunks + deep - 1) / deep != ks) continue;
       const long rounds = (tiles * ks + cus - 1) / cus;
-      double us = (rounds == 1 ? c.alone : rounds * c.among) * deep * (f32 ? 1.5 : 1.0) + rounds * (c.out + (t == 0 && add ? 8.0 : 0.0));
-      if (ks > 1) us += 5.0 + 1e-6 * (double)(tiles * ks) * c.tm * c.tn * 3;
-      if (us < best.us) best = {t, ks, us};
+      double us = (rounds == 1 ? c.alone[exact] : rounds * c.among[exact]) * deep + rounds * (add ? c.out_add : c.out);
+      if (ks > 1) us += 5.0 + 3e-6 * (double)(tiles * ks) * c.tm * c.tn;
+      if (us < best_us) best_us = us, best = 64 * t + ks;
     }
   }
   return best;
 }
 
-void run_tiles(ien_ctx *ctx, Args8 &a) {
-  const int chunks = a.taps * a.cb;
-  const Plan8 p = plan8(ctx->cus, (long)ctx->splitk_floats, a.rows, a.n, chunks, a.f32, a.add);
-  const Choice8 &c = CHOICES8[p.tile];
-  a.tiles_m = (int)((a.rows + c.tm - 1) / c.tm);
-  a.tiles_n = (int)((a.n + c.tn - 1) / c.tn);
-  a.ksplit = p.ksplit;
-  a.kchunks = (chunks + p.ksplit - 1) / p.ksplit;
-  a.part = ctx->splitk;
-  a.tile_count = (int *)(ctx->splitk + ctx->splitk_floats);
-  switch (p.tile) {
-    case 0: launch<Tile8<4, 4, 2, 2, 2>, false>(ctx, a); break;
-    case 1: a.f32 ? launch<Tile8<2, 2, 2, 2, 2>, true>(ctx, a) : launch<Tile8<2, 2, 2, 2, 2>, false>(ctx, a); break;
-    case 2: a.f32 ? launch<Tile8<1, 2, 2, 2, 3>, true>(ctx, a) : launch<Tile8<1, 2, 2, 2, 3>, false>(ctx, a); break;
-    default: a.f32 ? launch<Tile8<1, 1, 2, 2, 4>, true>(ctx, a) : launch<Tile8<1, 1, 2, 2, 4>, false>(ctx, a); break;
-  }
-}
-
-}  // namespace
 }  // namespace ien
 
 using namespace ien;
@@ -532,6 +538,7 @@ ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *in, size_t row0, size_t
   a.y = out->data;
   a.ys = (long)out->stride;
   a.f32 = out->type == IEN_OUT_F32;
+  a.exact = a.f32 || in->exact;
   a.act = act;
   a.add = d_add;
   a.as = (long)add_stride;

@@ -279,12 +279,21 @@ typedef struct {
   ien_input_kind kind;
   ien_rows8 map;
   size_t images, height, width, step;
+  int exact; /* f16 outputs: exact sums of products too, see ien_multiply8 */
 } ien_input8;
 
 /* out[r] = act(input[r] . w + bias + add[r]) for rows row0 .. row0 + rows of
  * the input (IMAGE: of its output pixels, images x ceil(height / step) x
  * ceil(width / step)), into f16 or f32 NHWC rows `out->stride` elements apart
  * (row row0 at out->data; add's rows likewise).  Sums are f32, rounded once.
+ * The 8-bit matrix instructions that f16 outputs take line neighbouring
+ * products up on some 16 bits before they are added, which puts a sum 1.5e-5
+ * of itself off: less than the f16 rounding after it, unless a later step
+ * rounds to 8 bits again, where a tie that falls the other way counts.  With
+ * input->exact, and for f32 outputs always, the products are added in f32, at
+ * half the rate.
+ * A map's pixels are less than 1 MiB each in bytes, and a line of them (and
+ * 256 more) less than 512 MiB.
  * d_add (or NULL): rows of out's type, add_stride elements apart; it may be
  * out->data itself, with its stride, which accumulates.  act: NONE, RELU,
  * GELU, SIGMOID or SILU.  out overlaps neither the input nor, otherwise, add. */
