@@ -316,7 +316,8 @@ def _run_own(s):
         first, second = s["layers"]
         shape = s["images"], s["height"], s["width"]
         ien.group_norm(ctx, s["x"], s["images"], s["groups"], g1, b1, s["q"], eps=EPS, act=ien.ACT_SILU)
-        ien.conv8(ctx, s["q"], *shape, first["matrix"], s["h"])
+        # (Rounded to 8 bits again after the norm: its sums are exact.)
+        ien.conv8(ctx, s["q"], *shape, first["matrix"], s["h"], exact=True)
         ien.group_norm(ctx, s["h"], s["images"], s["groups"], g2, b2, s["q"], eps=EPS, act=ien.ACT_SILU)
         ien.conv8(ctx, s["q"], *shape, second["matrix"], s["y"], add=s["x"])
     return s["y"]
