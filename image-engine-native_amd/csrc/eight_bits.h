@@ -8,9 +8,9 @@
 // Weights in 8 bits: panel t cb + b (tap t, block b of 128 channels) holds
 // npad rows of 128 e4m3 bytes, an output each (zeros past c and n), and npad
 // scale dwords (the byte in the low 8 bits); npad is n in whole 128s.  A
-// tile's share of a panel is one contiguous piece.  SLACK8 rows and scales
-// follow the last panel (not set: no stored output comes from them): tiles of
-// 256 outputs read that far.
+// tile's share of a panel is one contiguous piece.  SLACK8 more panels and 128
+// rows and scales follow (not set: no stored output comes from them): tiles of
+// 256 outputs and the loads ahead of the last block read that far.
 struct ien_matrix8 {
   ien_ctx *ctx = nullptr;
   size_t taps = 0, c = 0, n = 0;
@@ -24,7 +24,7 @@ struct ien_matrix8 {
 namespace ien {
 
 constexpr int BLOCK8 = 128;  // values under one scale
-constexpr int SLACK8 = 128;  // rows past the last panel of weights
+constexpr int SLACK8 = 4;    // panels of weights past the last one
 
 inline size_t blocks8(size_t k) { return (k + BLOCK8 - 1) / BLOCK8; }
 

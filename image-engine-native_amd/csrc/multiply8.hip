@@ -21,12 +21,13 @@
 // A workgroup of four waves computes a tile of rows x outputs, a block of 128
 // deep at a time through a ring of stages in LDS that buffer loads fill without
 // registers; the 3 x 3 taps are the blocks' order, each lane's row at the tap's
-// pixel or, off the map, past the buffer's end.  What bounds it is the way into
-// LDS: some 65 KB a us and CU whatever the tile, so the largest tile (256 x
-// 256, 66 KB a block for 1.45 us of matrix time) is the fastest, and smaller
-// ones are for what would leave CUs idle.  8192 x 8192 -> 8192: 411 us, 2.67
-// PFLOP/s, 16384 rows 2048 -> 8192 262 us (of it 60 the writing of the result,
-// in step on all CUs); a wave a 32 x 32 tile straight from memory took 2040.
+// pixel or, off the map, past the buffer's end.  The 256 x 256 tile is bound by
+// the matrix instructions (1.45 us a block, 2.9 PFLOP/s over all CUs), smaller
+// ones by their way into and out of LDS and, a workgroup a CU, by the time a
+// block takes from one barrier to the next; they are for what would leave CUs
+// idle.  8192 x 8192 -> 8192: 411 us, 2.67 PFLOP/s; 16384 rows 2048 -> 8192 262
+// us with its inputs in the memory-side cache, 280 without (of it 60 the writing
+// of the result, in step on all CUs).
 
 #include "eight_bits.h"
 
@@ -91,17 +92,17 @@ struct Tile8 {
 
 constexpr int NOWHERE = 0x7ffffff0;  // past every buffer: reads zeros
 
-// dma_lds and dma_lds4 with the LDS place as a wave's base and a constant,
-// and a uniform offset `soff` beside the lane's (which alone is checked
-// against the buffer's end).
+// Buffer loads into LDS (dma_lds) with the place as a wave's base and a
+// constant, and a uniform offset beside the lane's: 16 bytes a lane, or a byte
+// a lane, each in a dword of LDS.
 template <int CONST>
-__device__ __forceinline__ void dma16_at(int4v rsrc, unsigned wave_base, int off) {
-  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
-               :: "s"(wave_base), "n"(CONST), "v"(off), "s"(rsrc) : "memory", "m0", "scc");
+__device__ __forceinline__ void dma16_at(int4v rsrc, unsigned wave_base, int off, int soff) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
+               :: "s"(wave_base), "n"(CONST), "v"(off), "s"(rsrc), "s"(soff) : "memory", "m0", "scc");
 }
 template <int CONST>
-__device__ __forceinline__ void dma4_at(int4v rsrc, unsigned wave_base, int off, int soff) {
-  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds"
+__device__ __forceinline__ void dma1_at(int4v rsrc, unsigned wave_base, int off, int soff) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_ubyte %2, %3, %4 offen lds"
                :: "s"(wave_base), "n"(CONST), "v"(off), "s"(rsrc), "s"(soff) : "memory", "m0", "scc");
 }
 
@@ -163,66 +164,73 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   for (int i = 0; i < T::A_LOADS; i++) {
     const int row = (wave + T::WAVES * i) * 8 + (lane >> 3);
     mask[i] = place(row, &off[i]);
-    off[i] = off[i] * (int)a.xs + 16 * ((lane & 7) ^ (row & 7));
+    off[i] = off[i] * (int)a.xs + 16 * ((lane & 7) ^ (row >> 1 & 7));
   }
   int soff[T::S_LOADS], smask[T::S_LOADS];
 #pragma unroll
   for (int i = 0; i < T::S_LOADS; i++) {
     const int piece = wave + T::WAVES * i;  // (past the scales: into the stage's spare lines)
-    smask[i] = piece < T::TM / 64 ? place(piece * 64 + lane, &soff[i]) : 0;
+    smask[i] = piece < T::TM / 64 ? place(piece * 64 + lane, &soff[i]) : -1;
     soff[i] = piece < T::TM / 64 ? soff[i] * (int)a.ss : (piece * 64 + lane - T::TM) * 4;
   }
 
-  // The stream of blocks to load: addresses of the next one's rows and scales
-  // (of the tile's first row under the block's tap) and of its weights.
+  // The stream of blocks to load, from this split's first: a tap and a block of
+  // its channels, as a uniform offset from where the tile's first row has its
+  // first tap.  (One step costs a wave that is alone on its SIMD some 4 cycles an
+  // instruction, so a step has few: the taps' offsets are lanes of a register,
+  // and nothing asks whether a block is past the last one.  Those are read,
+  // SLACK8 panels further on at most, and not multiplied.)
   const int chunks = min(a.taps * a.cb - (int)blockIdx.y * a.kchunks, a.kchunks), c_begin = blockIdx.y * a.kchunks;
-  int tap = c_begin / a.cb, ib = c_begin - tap * a.cb, left = chunks;
-  int kx = a.taps == 9 ? tap % 3 : 0;
-  const long shift = a.taps == 9 ? (long)(tap / 3 - 1) * a.W + kx - 1 : 0;
-  long xat = (long)a.x + (first + shift) * a.xs + ib * BLOCK8, sat = (long)a.scales + (first + shift) * a.ss;
-  long wat = (long)a.w + ((long)c_begin * a.npad + n0) * BLOCK8, vat = (long)a.ws + ((long)c_begin * a.npad + n0) * 4;
-  const long across = a.xs - a.cb * BLOCK8, down = (a.W - 2) * a.xs - a.cb * BLOCK8, sdown = (a.W - 2) * a.ss;
+  int tap = c_begin / a.cb, ib = c_begin - tap * a.cb;
+  const long corner = first - (a.taps == 9 ? a.W + 1 : 0);
+  const int t9 = a.taps == 9 ? min(lane, 8) : 0;
+  const int tap_pixels = t9 / 3 * (int)a.W + t9 % 3;
+  const int tap_bytes = tap_pixels * (int)a.xs, tap_scales = tap_pixels * (int)a.ss;
+  int xo, so, vo = 0;
+  auto at_tap = [&] {
+    xo = __builtin_amdgcn_readlane(tap_bytes, tap) + ib * BLOCK8;
+    so = __builtin_amdgcn_readlane(tap_scales, tap) + ib;
+  };
+  at_tap();
+  const int4v xr = uniform_rsrc(a.x + corner * a.xs, 0x7fffff00), sr = uniform_rsrc(a.scales + corner * a.ss, 0x7fffff00);
+  const int4v vr = uniform_rsrc(a.ws + (long)c_begin * a.npad + n0, 0x7fffff00);
+  const uint8_t *w = a.w + ((long)c_begin * a.npad + n0) * BLOCK8;
   const unsigned wave_lds = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
   const unsigned wave_lds4 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 256);
   int woff[T::B_LOADS];
 #pragma unroll
   for (int i = 0; i < T::B_LOADS; i++) {
     const int row = (wave + T::WAVES * i) * 8 + (lane >> 3);
-    woff[i] = row * BLOCK8 + 16 * ((lane & 7) ^ (row & 7));
+    woff[i] = row * BLOCK8 + 16 * ((lane & 7) ^ (row >> 1 & 7));
   }
   // Load I of the block into stage STAGE, by this wave: first its rows, then
   // its weights, then its scales.
   auto load = [&](auto stage, auto I) {
     constexpr int BASE = decltype(stage)::value * T::STAGE, i = decltype(I)::value;
-    const int all = left > 0 ? 0x7fffff00 : 0;  // (past the last block: zeros)
+    auto on_map = [&](int off, int mask) {  // or past the end, which reads zeros
+      return off | (__builtin_amdgcn_sbfe(~mask, tap, 1) & 0x7fffff00);
+    };
     if constexpr (i < T::A_LOADS) {
-      // Off the map: past the end.
-      const int o = off[i] | (__builtin_amdgcn_sbfe(~mask[i], tap, 1) & 0x7fffff00);
-      dma16_at<BASE + T::WAVES * i * 1024>(uniform_rsrc((const void *)xat, all), wave_lds, o);
+      dma16_at<BASE + T::WAVES * i * 1024>(xr, wave_lds, on_map(off[i], mask[i]), xo);
     } else if constexpr (i < T::A_LOADS + T::B_LOADS) {
       constexpr int k = i - T::A_LOADS;
-      dma16_at<BASE + T::B0 + T::WAVES * k * 1024>(uniform_rsrc((const void *)wat, all), wave_lds, woff[k]);
+      int4v wr = xr;
+      wr.x = (int)(long)w;
+      wr.y = (int)((long)w >> 32);
+      dma16_at<BASE + T::B0 + T::WAVES * k * 1024>(wr, wave_lds, woff[k], 0);
     } else {
-      constexpr int k = i - T::A_LOADS - T::B_LOADS;
-      const int piece = wave + T::WAVES * k;
-      const bool rows = piece < T::TM / 64;
-      const int o = rows ? soff[k] | (__builtin_amdgcn_sbfe(~smask[k], tap, 1) & 0x7fffff00) : soff[k];
-      dma4_at<BASE + T::SX0 + T::WAVES * k * 256>(uniform_rsrc((const void *)(rows ? sat : vat), all), wave_lds4, o,
-                                                  rows ? ib & ~3 : 0);
+      constexpr int k = i - T::A_LOADS - T::B_LOADS, AT = BASE + T::SX0 + T::WAVES * k * 256;
+      const bool rows = wave + T::WAVES * k < T::TM / 64;  // (no branch: the products would be moved across it)
+      dma1_at<AT>(rows ? sr : vr, wave_lds4, on_map(soff[k], smask[k]), rows ? so : vo);
     }
   };
   auto advance = [&] {
-    left--;
-    xat += BLOCK8;
-    wat += a.npad * BLOCK8;
-    vat += a.npad * 4;
-    // (Without branches, which the products would be moved across.)
-    const int over = -(int)(++ib == a.cb), wrap = -(int)(kx == 2) & over;
-    ib &= ~over;
-    tap -= over;
-    kx = (kx - over) & ~wrap;
-    xat += (long)over & (wrap ? down : across);
-    sat += (long)over & (wrap ? sdown : a.ss);
+    w += a.npad * BLOCK8;
+    vo += (int)a.npad * 4;
+    const bool over = ++ib == a.cb;
+    tap = over ? tap + 1 : tap;
+    ib = over ? 0 : ib;
+    at_tap();
   };
 
   // Half s of a block: 16-byte slots 4 s + 2 hi, + 1 of each row, at those
@@ -232,7 +240,7 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   };
   int place16[4];
 #pragma unroll
-  for (int k = 0; k < 4; k++) place16[k] = l32 * BLOCK8 + 16 * ((4 * (k >> 1) + 2 * hi + (k & 1)) ^ (l32 & 7));
+  for (int k = 0; k < 4; k++) place16[k] = l32 * BLOCK8 + 16 * ((4 * (k >> 1) + 2 * hi + (k & 1)) ^ (l32 >> 1 & 7));
   const unsigned char *xp = lds + wm * T::FM * 32 * BLOCK8, *wp = lds + T::B0 + wn * T::FN * 32 * BLOCK8;
   const unsigned char *sp = lds + T::SX0 + (wm * T::FM * 32 + l32) * 4, *vp = lds + T::SW0 + (wn * T::FN * 32 + l32) * 4;
   // Fragment I of half s: the rows' first, then the weights'.
@@ -258,14 +266,14 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   };
   floatx16 acc[T::FM][T::FN] = {};
   constexpr int PRODUCTS = T::FM * T::FN;
-  // The products of half a block, beside(k) between them.
+  // The products of half a block, beside(k) after each.
   auto multiply = [&](const Half &h, const Scales &v, auto beside) {
     if constexpr (!EXACT) {
       each<PRODUCTS>([&](auto k) {
         constexpr int i = decltype(k)::value / T::FN, j = decltype(k)::value % T::FN;
-        beside(k);
-        __builtin_amdgcn_sched_barrier(0);
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(h.w[j], h.x[i], acc[i][j], 0, 0, 0, v.w[j], 0, v.x[i]);
+        __builtin_amdgcn_sched_barrier(0);
+        beside(k);
         __builtin_amdgcn_sched_barrier(0);
       });
     } else {
@@ -273,13 +281,13 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
         constexpr int E = 2 * decltype(e)::value;
         bf16x8 x[T::FM], w[T::FN];
 #pragma unroll
-        for (int i = 0; i < T::FM; i++) x[i] = widen8(h.x[i][E], h.x[i][E + 1], scale_power(v.x[i] & 255));
+        for (int i = 0; i < T::FM; i++) x[i] = widen8(h.x[i][E], h.x[i][E + 1], scale_power(v.x[i]));
 #pragma unroll
         for (int j = 0; j < T::FN; j++) w[j] = widen8(h.w[j][E], h.w[j][E + 1], scale_power(v.w[j]));
         each<PRODUCTS>([&](auto k) {
           constexpr int i = decltype(k)::value / T::FN, j = decltype(k)::value % T::FN;
-          if constexpr (E == 0) beside(k);
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[i][j], 0, 0, 0);
+          if constexpr (E == 0) beside(k);
         });
       });
     }
@@ -290,7 +298,7 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   // half's products the next one's first half is read and the block S further
   // loaded into this one's place.  (Blocks past the last are zeros.)
   if (wave < T::TN / 64)  // the epilogue's biases
-    dma4_at<T::BIAS0>(uniform_rsrc((const void *)(a.bias + n0), (a.npad - n0) * 4), wave_lds4, (wave * 64 + lane) * 4, 0);
+    dma_lds4(uniform_rsrc(a.bias + n0, (a.npad - n0) * 4), wave_lds4 + T::BIAS0, (wave * 64 + lane) * 4);
   each<T::S>([&](auto stage) {
     each<T::LOADS>([&](auto i) { load(stage, i); });
     advance();
@@ -300,14 +308,8 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   constexpr int FRAGS = T::FM + T::FN, EARLY = (PRODUCTS + 1) / 2;  // products among which the fragments are read
   Half h0, h1;
   Scales v[T::S];
-  int b = c_begin % a.cb;
   each<FRAGS>([&](auto i) { read(h0, Const<0>{}, Const<0>{}, i); });
   read_scales(v[0], Const<0>{});
-  auto align = [&](Scales &v) {
-#pragma unroll
-    for (int i = 0; i < T::FM; i++) v.x[i] >>= 8 * (b & 3);
-    b = b + 1 == a.cb ? 0 : b + 1;
-  };
   // The products of `now` while half s of stage NEXT is read into `then`, and where `loads`, stage STAGE's next block loaded.
   auto work = [&](const Half &now, const Scales &v, Half &then, auto next, auto s, auto stage, auto loads) {
     multiply(now, v, [&](auto k) {
@@ -322,7 +324,6 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   auto step = [&](auto stage) {
     constexpr int s = decltype(stage)::value;
     const Const<(s + 1) % T::S> next;
-    align(v[s]);
     work(h0, v[s], h1, stage, Const<1>{}, stage, Const<0>{});
     wait_vm<(T::S - 2) * T::LOADS>();
     lds_barrier();
@@ -424,10 +425,10 @@ struct Choice8 {
   int tm, tn;
   double alone[2], among[2], out, out_add;
 };
-constexpr Choice8 CHOICES8[] = {{256, 256, {1.45, 2.9}, {1.45, 2.9}, 8.0, 16.0},
-                                {128, 128, {0.58, 0.90}, {0.50, 0.72}, 3.0, 3.0},
-                                {64, 128, {0.42, 0.68}, {0.34, 0.46}, 1.7, 1.7},
-                                {64, 64, {0.38, 0.60}, {0.22, 0.28}, 1.2, 1.2}};
+constexpr Choice8 CHOICES8[] = {{256, 256, {1.45, 2.9}, {1.45, 2.9}, 8.0, 25.0},
+                                {128, 128, {0.65, 0.90}, {0.50, 0.72}, 3.0, 3.8},
+                                {64, 128, {0.38, 0.68}, {0.27, 0.46}, 1.7, 2.8},
+                                {64, 64, {0.38, 0.60}, {0.22, 0.28}, 1.2, 2.0}};
 
 template <typename T>
 void launch(ien_ctx *ctx, Args8 &a) {
@@ -451,10 +452,15 @@ void run_tiles(ien_ctx *ctx, Args8 &a) {
   a.kchunks = (chunks + ksplit - 1) / ksplit;
   a.part = ctx->splitk;
   a.tile_count = (int *)(ctx->splitk + ctx->splitk_floats);
+  const bool shared = (long)a.tiles_m * a.tiles_n * a.ksplit > ctx->cus;
   switch (tile) {
     case 0: launch<Tile8<4, 4, 2, 2, 2>>(ctx, a); break;
-    case 1: launch<Tile8<2, 2, 2, 2, 2>>(ctx, a); break;
-    case 2: launch<Tile8<1, 2, 2, 2, 3>>(ctx, a); break;
+    case 1:  // (Twice the waves for the residuals' loads: 3x3 256x384 256 -> 256 82 -> 77 us; without, 327 -> 337 us at 16384 rows.)
+      a.add ? launch<Tile8<1, 2, 4, 2, 2>>(ctx, a) : launch<Tile8<2, 2, 2, 2, 2>>(ctx, a);
+      break;
+    case 2:  // (Three workgroups a CU with two stages: 4096 rows 384 -> 1536 12.9 -> 10.5 us; one a CU wants three: 36 blocks deep 16.5, not 23.)
+      shared ? launch<Tile8<1, 2, 2, 2, 2>>(ctx, a) : launch<Tile8<1, 2, 2, 2, 3>>(ctx, a);
+      break;
     default: launch<Tile8<1, 1, 2, 2, 4>>(ctx, a); break;
   }
 }
@@ -546,8 +552,9 @@ ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *in, size_t row0, size_t
   a.vec = w->n % 8 == 0;
   // A tile addresses its rows' values by 31-bit offsets from its first one's.
   IEN_CHECK(in->map.stride < (1u << 20) && in->map.scale_stride < (1u << 20) &&
-                (!a.image || (in->width + 256) * std::max(in->map.stride, in->map.scale_stride) < (1u << 29)),
-            IEN_ERR_INPUT, "rows in 8 bits %zu and %zu bytes apart, %ld to a line of a map", in->map.stride,
+                (!a.image || (in->width + 256) * std::max(in->map.stride, in->map.scale_stride) < (1u << 27)) &&
+                w->taps * w->cb * w->npad < (1l << 28),
+            IEN_ERR_INPUT, "rows in 8 bits %zu and %zu bytes apart, %ld to a line of a map, or too many weights", in->map.stride,
             in->map.scale_stride, a.W);
   run_tiles(ctx, a);
   IEN_HIP(hipGetLastError());

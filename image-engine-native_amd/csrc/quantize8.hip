@@ -178,8 +178,8 @@ ien_status ien_matrix8_new(ien_ctx *ctx, const void *w, ien_wtype wtype, size_t 
   void *raw = nullptr;
   hipError_t e = hipSetDevice(ctx->device);
   if (e == hipSuccess) e = hipMalloc(&raw, bytes);
-  if (e == hipSuccess) e = hipMalloc((void **)&m->d_w, (panels * m->npad + SLACK8) * BLOCK8);
-  if (e == hipSuccess) e = hipMalloc((void **)&m->d_scales, (panels * m->npad + SLACK8) * 4);
+  if (e == hipSuccess) e = hipMalloc((void **)&m->d_w, ((panels + SLACK8) * m->npad + 128) * BLOCK8);
+  if (e == hipSuccess) e = hipMalloc((void **)&m->d_scales, ((panels + SLACK8) * m->npad + 128) * 4);
   if (e == hipSuccess) e = hipMalloc((void **)&m->d_bias, m->npad * 4);
   if (e == hipSuccess) e = hipMemcpyAsync(raw, w, bytes, hipMemcpyHostToDevice, ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(m->d_bias, 0, m->npad * 4, ctx->stream);
