@@ -53,7 +53,7 @@ struct Args8 {
   int f32, exact, act;  // f32 outputs are exact
   const void *add;
   long as;
-  int image, vec;  // a map's pixels; whole eights of outputs
+  int image;  // a map's pixels
   int tiles_m, tiles_n, ksplit, kchunks;
   float *part;
   int *tile_count;
@@ -371,46 +371,45 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
             float4v{v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]};
     __builtin_amdgcn_wave_barrier();
   };
+  const int many = (int)max(min(a.n - nw - col, 8L), 0L);  // this lane's outputs of an eight
+  const bool ragged = nw + COLS > a.n && a.n % 8 != 0;      // (the same for the wave)
+  constexpr int STEP = 64 / EIGHTS;                         // rows between its eights
   with_act8(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < T::FM; i++) {
-      const long r0 = m0 + (wm * T::FM + i) * 32;
-      if (a.vec) {
-        const bool in = nw + col < a.n;
-        Y *y = (Y *)a.y + (r0 + row) * a.ys + nw + col;
-        float old[ITEMS][8];
-        if (a.add) {
-          const Y *add = (const Y *)a.add + (r0 + row) * a.as + nw + col;
-#pragma unroll
-          for (int e = 0; e < ITEMS; e++)
-            if (in && r0 + row + e * (64 / EIGHTS) < a.rows) load8<Y, true>(add + e * (64 / EIGHTS) * a.as, 0, 0, old[e]);
-        }
-        stage_rows(acc[i]);
+      const long r0 = m0 + (wm * T::FM + i) * 32 + row;
+      Y *y = (Y *)a.y + r0 * a.ys + nw + col;
+      float old[ITEMS][8];
+      if (a.add) {
+        const Y *add = (const Y *)a.add + r0 * a.as + nw + col;
 #pragma unroll
         for (int e = 0; e < ITEMS; e++) {
-          if (!in || r0 + row + e * (64 / EIGHTS) >= a.rows) continue;
-          float v[8];
-          take(st + (row + e * (64 / EIGHTS)) * T::PITCH + col, v);
-#pragma unroll
-          for (int k = 0; k < 8; k++) v[k] += bias[k];
-          if (a.add) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] += old[e][k];
-          }
-#pragma unroll
-          for (int k = 0; k < 8; k++) v[k] = act8<decltype(act)::value>(v[k]);
-          store8<Y, true>(y + e * (64 / EIGHTS) * a.ys, 0, 0, v);
+          if (r0 + e * STEP >= a.rows) continue;
+          if (many == 0) continue;
+          if (!ragged || many == 8)
+            load8<Y, true>(add + e * STEP * a.as, 0, 0, old[e]);
+          else
+            load8<Y, false>(add + e * STEP * a.as, 0, many, old[e]);
         }
-      } else {
-        stage_rows(acc[i]);
-        for (int e = lane; e < 32 * COLS; e += 64) {
-          const int r = e / COLS, c = e % COLS;
-          const long n = nw + c;
-          if (r0 + r >= a.rows || n >= a.n) continue;
-          float v = st[r * T::PITCH + c] + ((const float *)(lds + T::BIAS0))[wn * COLS + c];
-          if (a.add) v += (float)((const Y *)a.add)[(r0 + r) * a.as + n];
-          ((Y *)a.y)[(r0 + r) * a.ys + n] = (Y)act8<decltype(act)::value>(v);
+      }
+      stage_rows(acc[i]);
+#pragma unroll
+      for (int e = 0; e < ITEMS; e++) {
+        if (many == 0 || r0 + e * STEP >= a.rows) continue;
+        float v[8];
+        take(st + (row + e * STEP) * T::PITCH + col, v);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] += bias[k];
+        if (a.add) {
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[k] += old[e][k];
         }
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = act8<decltype(act)::value>(v[k]);
+        if (!ragged || many == 8)
+          store8<Y, true>(y + e * STEP * a.ys, 0, 0, v);
+        else
+          store8<Y, false>(y + e * STEP * a.ys, 0, many, v);
       }
       __builtin_amdgcn_wave_barrier();
     }
@@ -549,7 +548,6 @@ ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *in, size_t row0, size_t
   a.add = d_add;
   a.as = (long)add_stride;
   a.image = in->kind == IEN_INPUT_IMAGE;
-  a.vec = w->n % 8 == 0;
   // A tile addresses its rows' values by 31-bit offsets from its first one's.
   IEN_CHECK(in->map.stride < (1u << 20) && in->map.scale_stride < (1u << 20) &&
                 (!a.image || (in->width + 256) * std::max(in->map.stride, in->map.scale_stride) < (1u << 27)) &&
