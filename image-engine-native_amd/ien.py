@@ -248,7 +248,10 @@ def _ptr(t):
 class Context:
     """ien_ctx on one device.  The context's own (non-blocking) HIP stream
     becomes torch's current stream, so torch's copies, fills and events are
-    ordered with the library's launches."""
+    ordered with the library's launches; when it closes, that of the context
+    opened last of those still open (or the default stream) takes its place."""
+
+    _open = []
 
     def __init__(self, device=0):
         import torch
@@ -260,6 +263,7 @@ class Context:
         self.device = device
         self.stream = torch.cuda.ExternalStream(L.ien_stream(h), device=torch.device("cuda", device))
         torch.cuda.set_stream(self.stream)
+        Context._open.append(self)
 
     @property
     def name(self):
@@ -270,7 +274,10 @@ class Context:
             import torch
 
             torch.cuda.synchronize(self.device)
-            torch.cuda.set_stream(torch.cuda.default_stream(self.device))
+            Context._open.remove(self)
+            if torch.cuda.current_stream(self.device) == self.stream:
+                left = [c.stream for c in Context._open if c.device == self.device]
+                torch.cuda.set_stream(left[-1] if left else torch.cuda.default_stream(self.device))
             load().ien_close(self.h)
             self.h = None
 
