@@ -223,8 +223,8 @@ __global__ __launch_bounds__(LANES) void k_norm_stats(NormArgs a) {
 // A lane's eight channels' way from x to y.
 struct Line {
   float mean[8], gain[8], bias[8];
-  __device__ void set(const NormArgs &a, int c0, int at, const float2 *stats) {
-    const int per = a.c / a.groups;
+  // First gamma and beta, so that their loads are under way early, then the statistics.
+  __device__ __forceinline__ Line(const NormArgs &a, int c0, int at) {
 #pragma unroll
     for (int i = 0; i < 8; i++) gain[i] = 1.0f, bias[i] = 0.0f;
     auto get = [&](const float *from, float *to) {
@@ -234,6 +234,9 @@ struct Line {
     };
     if (a.gamma) get(a.gamma, gain);
     if (a.beta) get(a.beta, bias);
+  }
+  __device__ __forceinline__ void set(const NormArgs &a, int at, const float2 *stats) {
+    const int per = a.c / a.groups;
     int g = at / per, in = at - g * per;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -322,6 +325,7 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
       p.eight < p.eights ? (unsigned)((int)min(a.chunk, a.pixels - begin) - p.slot + p.px - 1) / (unsigned)p.px : 0;
   Eight<T> now[BATCH<T>];
   if (count > 0) load_batch<EIGHTS>(now, x, step, last_batch<T>(count), count, at, a.c);
+  Line l(a, 0, at);
 
   const float whole = (float)a.chunk, last = (float)(a.pixels - (a.chunks - 1) * a.chunk);
   for (int g0 = 0; g0 < a.groups; g0 += lanes) {
@@ -347,6 +351,7 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
       __syncthreads();
       s = 0.0f;
       if (row == 0)
+#pragma unroll 8
         for (int k = 0; k < rows; k++) s += sums[k * many + t];
       return s;
     };
@@ -368,8 +373,7 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
   }
 
   if (count <= 0) return;
-  Line l;
-  l.set(a, 0, at, stats);
+  l.set(a, at, stats);
   apply<EIGHTS, T, Y>(a, l, now, x, step, count, r0, p.px, 0, at);
 }
 
@@ -389,6 +393,7 @@ __global__ __launch_bounds__(LANES) void k_norm_one(NormArgs a) {
   const int count = p.eight < p.eights ? (unsigned)((int)a.pixels - p.slot + p.px - 1) / (unsigned)p.px : 0;
   float n = 0.0f, m[8] = {}, q[8] = {};
   Eight<T> now[BATCH<T>];
+  Line l(a, c0, at);
   if (count > 0) {
     gather<EIGHTS>(x, p.px * a.stride, count, at, a.span, n, m, q);
     load_batch<EIGHTS>(now, x, p.px * a.stride, last_batch<T>(count), count, at, a.span);
@@ -398,8 +403,7 @@ __global__ __launch_bounds__(LANES) void k_norm_one(NormArgs a) {
   });
   __syncthreads();
   if (count == 0) return;
-  Line l;
-  l.set(a, c0, at, stats);
+  l.set(a, at, stats);
   apply<EIGHTS, T, Y>(a, l, now, x, p.px * a.stride, count, r0, p.px, c0, at);
 }
 
