@@ -266,7 +266,7 @@ __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, in
   } else {
     Y *y = (Y *)a.y + r * a.ystride + c0;
     if (EIGHTS || at + 8 <= a.span)
-      store8<Y, true>(y, at, a.span, v);
+      stream8(y + at, v);
     else
       store8<Y, false>(y, at, a.span, v);
   }

@@ -407,7 +407,7 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
 #pragma unroll
         for (int k = 0; k < 8; k++) v[k] = act8<decltype(act)::value>(v[k]);
         if (!ragged || many == 8)
-          store8<Y, true>(y + e * STEP * a.ys, 0, 0, v);
+          stream8(y + e * STEP * a.ys, v);
         else
           store8<Y, false>(y + e * STEP * a.ys, 0, many, v);
       }
@@ -427,7 +427,7 @@ struct Choice8 {
 constexpr Choice8 CHOICES8[] = {{256, 256, {1.45, 2.9}, {1.45, 2.9}, 8.0, 25.0},
                                 {128, 128, {0.65, 0.90}, {0.50, 0.72}, 3.0, 3.8},
                                 {64, 128, {0.38, 0.68}, {0.27, 0.46}, 1.7, 2.8},
-                                {64, 64, {0.38, 0.60}, {0.22, 0.28}, 1.2, 2.0}};
+                                {64, 64, {0.38, 0.60}, {0.22, 0.34}, 1.2, 2.0}};
 
 template <typename T>
 void launch(ien_ctx *ctx, Args8 &a) {

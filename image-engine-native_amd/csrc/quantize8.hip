@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void k_dequantize8(Rows8Args q, long rows, lon
         s * __builtin_amdgcn_cvt_f32_fp8(p.y, 0), s * __builtin_amdgcn_cvt_f32_fp8(p.y, 1),
         s * __builtin_amdgcn_cvt_f32_fp8(p.y, 2), s * __builtin_amdgcn_cvt_f32_fp8(p.y, 3)};
     if (EIGHTS || at + 8 <= k)
-      store8<T, true>(y + r * stride, at, k, v);
+      stream8(y + r * stride + at, v);
     else
       store8<T, false>(y + r * stride, at, k, v);
   }
