@@ -292,8 +292,8 @@ typedef struct {
  * rounds to 8 bits again, where a tie that falls the other way counts.  With
  * input->exact, and for f32 outputs always, the products are added in f32, at
  * half the rate.
- * A map's pixels are less than 1 MiB each in bytes, and a line of them (and
- * 256 more) less than 512 MiB.
+ * Rows in 8 bits are less than 1 MiB apart, a line of a map's pixels (and 256
+ * more) less than 128 MiB, and weights less than 32 GiB.
  * d_add (or NULL): rows of out's type, add_stride elements apart; it may be
  * out->data itself, with its stride, which accumulates.  act: NONE, RELU,
  * GELU, SIGMOID or SILU.  out overlaps neither the input nor, otherwise, add. */
