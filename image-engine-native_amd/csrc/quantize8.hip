@@ -10,6 +10,8 @@
 // values written and read back: 97 us, 4.1 TB/s of the f32 values alone and 5.2
 // with the bytes between.
 
+#include <new>
+
 #include "eight_bits.h"
 
 namespace ien {
@@ -173,9 +175,10 @@ ien_status ien_matrix8_new(ien_ctx *ctx, const void *w, ien_wtype wtype, size_t 
                            const float *bias, ien_matrix8 **out) {
   IEN_CHECK(ctx && w && out, IEN_ERR_INPUT, "null argument");
   IEN_CHECK(wtype == IEN_W_F32 || wtype == IEN_W_F16, IEN_ERR_INPUT, "weight type %d", (int)wtype);
-  IEN_CHECK((taps == 1 || taps == 9) && c > 0 && n > 0 && c < (1u << 22) && n < (1u << 22), IEN_ERR_INPUT,
-            "weights of %zu taps x %zu x %zu", taps, c, n);
-  ien_matrix8 *m = new ien_matrix8;
+  IEN_CHECK((taps == 1 || taps == 9) && c > 0 && n > 0 && c < (1u << 22) && n < (1u << 22) && taps * blocks8(c) < 65536,
+            IEN_ERR_INPUT, "weights of %zu taps x %zu x %zu", taps, c, n);
+  ien_matrix8 *m = new (std::nothrow) ien_matrix8;
+  IEN_CHECK(m, IEN_ERR_GPU, "8-bit weights: out of host memory");
   m->ctx = ctx;
   m->taps = taps;
   m->c = c;

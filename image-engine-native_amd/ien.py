@@ -617,9 +617,6 @@ class Rows8:
     data = property(lambda self: self._data)
     scales = property(lambda self: self._scales)
 
-    def struct(self):
-        return self._struct
-
 
 def _row_stride(t):
     """Elements between the rows of a 2-D tensor with contiguous rows (one row: its length)."""

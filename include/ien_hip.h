@@ -263,8 +263,9 @@ ien_status ien_dequantize8(ien_ctx *ctx, const ien_rows8 *x, size_t rows, size_t
 
 /* Weights in 8 bits: row-major (taps c) x n host weights (f32, or f16 bits),
  * taps 1 or 9 (3 x 3, row-major), channels c fastest, plus an optional
- * length-n host bias (kept in f32).  Quantised once, on the device, with a
- * scale for each 128 channels of a tap and output, as ien_quantize8 does. */
+ * length-n host bias (kept in f32); taps ceil(c / 128) under 65536, n under
+ * 2^22.  Quantised once, on the device, with a scale for each 128 channels of
+ * a tap and output, as ien_quantize8 does. */
 typedef struct ien_matrix8 ien_matrix8;
 ien_status ien_matrix8_new(ien_ctx *ctx, const void *w, ien_wtype wtype, size_t taps, size_t c,
                            size_t n, const float *bias, ien_matrix8 **out);

@@ -33,6 +33,11 @@ def test_too_many_weights():
     refused(call(200, 256, npad=1 << 24))
 
 
+def test_too_many_panels():
+    h = ctypes.c_void_p()
+    refused(ien.load().ien_matrix8_new(CTX, P, ien.W_F32, 9, 1 << 20, 8, None, ctypes.byref(h)))
+
+
 def test_bindings_refuse_a_map_that_is_none():
     ctx, q = types.SimpleNamespace(h=None), ien.Rows8(6, 40, device="cpu")
     m = types.SimpleNamespace(h=None, c=40, n=8)
