@@ -73,18 +73,20 @@ struct Place {
   }
 };
 
-// Eight channels of a pixel as they are; past the end zeros.  EIGHTS: c is in
-// eights, and no branch stands between the loads of a batch.
+// Eight channels of a pixel as they are; past the end the last one again (no
+// result is made of those).  EIGHTS: c is in eights, and no branch stands between
+// the loads of a batch.  Otherwise none does either in narrow rows, whose
+// values are read one by one: a branch would wait for the loads before it.
 template <typename T>
 using Eight = T __attribute__((ext_vector_type(8)));
 template <bool EIGHTS, typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T *row, int at, int c) {
   typedef Eight<T> Any __attribute__((aligned(sizeof(T))));
-  if (EIGHTS || at + 8 <= c) return *(const Any *)(row + at);
-  Eight<T> v = {};
+  if (EIGHTS) return *(const Any *)(row + min(at, c - 8));
+  if (c >= 64 && at + 8 <= c) return *(const Any *)(row + at);
+  Eight<T> v;
 #pragma unroll
-  for (int i = 0; i < 8; i++)
-    if (at + i < c) v[i] = row[at + i];
+  for (int i = 0; i < 8; i++) v[i] = row[min(at + i, c - 1)];
   return v;
 }
 
@@ -187,7 +189,7 @@ __device__ __forceinline__ void by_group(const Shared &s, const Place &p, float 
 template <bool EIGHTS, typename T>
 __device__ __forceinline__ void gather(const T *x, long step, int left, int at, int c, float &n, float (&m)[8],
                                        float (&q)[8]) {
-  constexpr int U = sizeof(T) == 2 ? 8 : 4;
+  constexpr int U = (sizeof(T) == 2 ? 8 : 4) / (EIGHTS ? 1 : 2);  // (single values take a register each)
   auto batch = [&](auto all) {
     constexpr bool ALL = decltype(all)::value;
     Eight<T> x8[U];
@@ -258,7 +260,7 @@ __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, in
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      if (!EIGHTS && at + i >= a.span) v[i] = 0.0f;
+      if (at + i >= a.span) v[i] = 0.0f;
       top = fmaxf(top, finite_magnitude(v[i]));
     }
     const int e = exponent8(max16(top));
@@ -275,25 +277,26 @@ __device__ __forceinline__ void put(const NormArgs &a, const Line &l, long r, in
 
 // A lane's `count` pixels r, r + px, ... from x on, `step` apart, from the last:
 // a batch is loaded while the one after it (the first one by the caller) is written.
-template <typename T>
-constexpr int BATCH = sizeof(T) == 2 ? 4 : 2;
 template <bool EIGHTS, typename T>
-__device__ __forceinline__ void load_batch(Eight<T> (&to)[BATCH<T>], const T *x, long step, int k, int count, int at, int c) {
+constexpr int BATCH = (sizeof(T) == 2 ? 4 : 2) / (EIGHTS ? 1 : 2);
+template <bool EIGHTS, typename T>
+__device__ __forceinline__ void load_batch(const T *x, Eight<T> (&to)[BATCH<EIGHTS, T>], long step, int k, int count,
+                                           int at, int c) {
 #pragma unroll
-  for (int u = 0; u < BATCH<T>; u++) to[u] = load_eight<EIGHTS>(x + max(min(k + u, count - 1), 0) * step, at, c);
+  for (int u = 0; u < BATCH<EIGHTS, T>; u++) to[u] = load_eight<EIGHTS>(x + max(min(k + u, count - 1), 0) * step, at, c);
 }
-template <typename T>
+template <bool EIGHTS, typename T>
 __device__ __forceinline__ int last_batch(int count) {
-  return (count - 1) / BATCH<T> * BATCH<T>;
+  return (count - 1) / BATCH<EIGHTS, T> * BATCH<EIGHTS, T>;
 }
 template <bool EIGHTS, typename T, typename Y>
-__device__ __forceinline__ void apply(const NormArgs &a, const Line &l, Eight<T> (&now)[BATCH<T>], const T *x, long step,
+__device__ __forceinline__ void apply(const NormArgs &a, const Line &l, Eight<T> (&now)[BATCH<EIGHTS, T>], const T *x, long step,
                                       int count, long r, int px, int c0, int at) {
-  constexpr int U = BATCH<T>;
+  constexpr int U = BATCH<EIGHTS, T>;
   with_act8(a.act, [&](auto act) {
-    for (int k = last_batch<T>(count); k >= 0; k -= U) {
+    for (int k = last_batch<EIGHTS, T>(count); k >= 0; k -= U) {
       Eight<T> next[U];
-      load_batch<EIGHTS>(next, x, step, k - U, count, at, a.span);
+      load_batch<EIGHTS>(x, next, step, k - U, count, at, a.span);
 #pragma unroll
       for (int u = 0; u < U; u++) {
         float v[8];
@@ -324,8 +327,8 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
   const T *x = (const T *)a.x + r0 * a.stride;
   const int count =
       p.eight < p.eights ? (unsigned)((int)min(a.chunk, a.pixels - begin) - p.slot + p.px - 1) / (unsigned)p.px : 0;
-  Eight<T> now[BATCH<T>];
-  if (count > 0) load_batch<EIGHTS>(now, x, step, last_batch<T>(count), count, at, a.c);
+  Eight<T> now[BATCH<EIGHTS, T>];
+  if (count > 0) load_batch<EIGHTS>(x, now, step, last_batch<EIGHTS, T>(count), count, at, a.c);
   Line l(a, 0, at);
 
   const float whole = (float)a.chunk, last = (float)(a.pixels - (a.chunks - 1) * a.chunk);
@@ -350,10 +353,16 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
       __syncthreads();
       sums[t] = s;
       __syncthreads();
+      int width = 1;
+      while (width * 2 < rows) width *= 2;
+      for (; width >= 16; width /= 2) {  // (halved down to 16, then one lane's sum)
+        if (row < width && row + width < rows) sums[t] = s += sums[t + width * many];
+        __syncthreads();
+      }
       s = 0.0f;
       if (row == 0)
 #pragma unroll 8
-        for (int k = 0; k < rows; k++) s += sums[k * many + t];
+        for (int k = 0; k < min(rows, 16); k++) s += sums[k * many + t];
       return s;
     };
     float s = 0.0f;
@@ -393,11 +402,11 @@ __global__ __launch_bounds__(LANES) void k_norm_one(NormArgs a) {
   const T *x = (const T *)a.x + r0 * a.stride + c0;
   const int count = p.eight < p.eights ? (unsigned)((int)a.pixels - p.slot + p.px - 1) / (unsigned)p.px : 0;
   float n = 0.0f, m[8] = {}, q[8] = {};
-  Eight<T> now[BATCH<T>];
+  Eight<T> now[BATCH<EIGHTS, T>];
   Line l(a, c0, at);
   if (count > 0) {
     gather<EIGHTS>(x, p.px * a.stride, count, at, a.span, n, m, q);
-    load_batch<EIGHTS>(now, x, p.px * a.stride, last_batch<T>(count), count, at, a.span);
+    load_batch<EIGHTS>(x, now, p.px * a.stride, last_batch<EIGHTS, T>(count), count, at, a.span);
   }
   by_group(s, p, n, m, q, a.span, per, [&](int g, float mean, float squares) {
     stats[g] = {mean, 1.0f / sqrtf(squares / ((float)a.pixels * per) + a.eps)};
@@ -448,8 +457,7 @@ ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_b
       hipLaunchKernelGGL((k_norm_apply<T, Y, E>), grid, dim3(lanes), 2 * lanes * 4 + a.groups * sizeof(float2), ctx->stream, a);
     }
   };
-  // (Lanes past a row in 8 bits write zeros: they are no whole eights.)
-  const bool in_eights = a.c % (y_bytes == 1 ? 128 : 8) == 0;
+  const bool in_eights = a.c % 8 == 0;
   auto go = [&](auto t, auto u, long many) {
     in_eights ? go_eights(t, u, Act<1>{}, many) : go_eights(t, u, Act<0>{}, many);
   };
