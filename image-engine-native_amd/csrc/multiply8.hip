@@ -10,13 +10,12 @@
 // The 8-bit instructions line the products of a few neighbouring values up on
 // some 16 bits before they are added (measured: 2^16 + 1 inside one lane's
 // values loses the 1; sums of 64 random products are off by 1.4e-5 of
-// themselves, whatever their accumulator holds).  That is a fortieth of an f16
-// output's own rounding, and as much as f32 outputs would be off in all.
-// Those, and f16 outputs on request, take their operands as bf16, which holds
-// e4m3 values under any of the scales exactly, and the bf16 instructions
-// (6e-9), at half the rate.  (Rounded to 8 bits again after a norm, f16 results
-// off by 1.4e-5 gave a residual block of 64 x 64 x 512 an error of 4.6e-4 in
-// place of 2.2e-4.)
+// themselves, whatever their accumulator holds).  That is no sum in f32, and
+// left to a caller who asks for it (`fast`, f16 outputs).  All others take their
+// operands as bf16, which holds e4m3 values under any of the scales exactly,
+// and the bf16 instructions (6e-9), at half the rate.  (Rounded to 8 bits again
+// after a norm, f16 results off by 1.4e-5 gave a residual block of 64 x 64 x 512
+// an error of 4.6e-4 in place of 2.2e-4.)
 //
 // A workgroup of four waves computes a tile of rows x outputs, a block of 128
 // deep at a time through a ring of stages in LDS that buffer loads fill without
@@ -49,7 +48,7 @@ struct Args8 {
   long n, npad;
   void *y;
   long ys;
-  int f32, exact, act;  // f32 outputs are exact
+  int f32, exact, act;  // f32 outputs, sums in f32 (f32 outputs always)
   const void *add;
   long as;
   int image;  // a map's pixels
@@ -542,7 +541,7 @@ ien_status ien_multiply8(ien_ctx *ctx, const ien_input8 *in, size_t row0, size_t
   a.y = out->data;
   a.ys = (long)out->stride;
   a.f32 = out->type == IEN_OUT_F32;
-  a.exact = a.f32 || in->exact;
+  a.exact = a.f32 || !in->fast;
   a.act = act;
   a.add = d_add;
   a.as = (long)add_stride;

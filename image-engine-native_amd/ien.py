@@ -111,7 +111,7 @@ class Input8(ctypes.Structure):
     """ien_input8."""
     _fields_ = [("kind", ctypes.c_int), ("map", Rows8Struct), ("images", ctypes.c_size_t),
                 ("height", ctypes.c_size_t), ("width", ctypes.c_size_t), ("step", ctypes.c_size_t),
-                ("exact", ctypes.c_int)]
+                ("fast", ctypes.c_int)]
 
 
 class Tensor(ctypes.Structure):
@@ -720,23 +720,23 @@ def _multiply8(ctx, x, shape, row0, matrix, out, act, add, exact):
         add_rows, add_n, add_at, add_kind, add_stride = _rows_of(add)
         if add_rows != rows or add_n != n or add_kind != kind:
             raise ValueError("what is added has the output's shape and type")
-    status = (_lib or load()).ien_multiply8(ctx.h, _INPUT8(shape[0], *x._fields, *shape[1:], 1 if exact else 0), row0, rows, matrix.h,
+    status = (_lib or load()).ien_multiply8(ctx.h, _INPUT8(shape[0], *x._fields, *shape[1:], 0 if exact else 1), row0, rows, matrix.h,
                                             _OUTPUT(at, stride, NHWC, kind), act, add_at, add_stride)
     if status:
         check(status)
 
 
-def multiply8(ctx, x, matrix, out, act=ACT_NONE, add=None, row0=0, exact=False):
+def multiply8(ctx, x, matrix, out, act=ACT_NONE, add=None, row0=0, exact=True):
     """out = act(x . w + bias + add): rows row0 .. of the Rows8 x, as many as
-    out (rows x n, f16 or f32) has; `add` like out, or out itself.  exact: f16
-    outputs from sums as exact as f32 ones', at half the rate, for results that
-    are rounded to 8 bits again."""
+    out (rows x n, f16 or f32) has; `add` like out, or out itself.  exact=False:
+    f16 outputs from the coarser sums of the 8-bit matrix instructions, at twice
+    the rate (ien_input8's `fast`); f32 outputs are exact either way."""
     if row0 < 0 or row0 + out.shape[0] > x.rows:
         raise ValueError(f"rows {row0} .. {row0 + out.shape[0]} of {x.rows}")
     _multiply8(ctx, x, (INPUT_ROWS, 1, 1, x.rows, 1), row0, matrix, out, act, add, exact)
 
 
-def conv8(ctx, x, images, height, width, matrix, out, step=1, act=ACT_NONE, add=None, row0=0, exact=False):
+def conv8(ctx, x, images, height, width, matrix, out, step=1, act=ACT_NONE, add=None, row0=0, exact=True):
     """The same for a 3 x 3 (9 taps) or 1 x 1 convolution of `images` maps of
     height x width pixels in 8 bits, zero padding: output pixels row0 .., as
     many as out has rows."""

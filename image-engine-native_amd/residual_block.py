@@ -39,8 +39,7 @@ class ResidualBlock8:
         out = torch.empty_like(x) if out is None else out
         shape = images, height, width
         ien.group_norm(self.ctx, x, images, self.groups, *self.norms[0], q, eps=self.eps, act=ien.ACT_SILU)
-        # Exact sums: this result is rounded to 8 bits again after the next norm.
-        ien.conv8(self.ctx, q, *shape, self.convs[0], h, exact=True)
+        ien.conv8(self.ctx, q, *shape, self.convs[0], h)
         ien.group_norm(self.ctx, h, images, self.groups, *self.norms[1], q, eps=self.eps, act=ien.ACT_SILU)
         ien.conv8(self.ctx, q, *shape, self.convs[1], out, add=x)
         return out

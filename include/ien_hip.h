@@ -280,19 +280,18 @@ typedef struct {
   ien_input_kind kind;
   ien_rows8 map;
   size_t images, height, width, step;
-  int exact; /* f16 outputs: exact sums of products too, see ien_multiply8 */
+  int fast; /* f16 outputs: coarser sums of products at twice the rate, see ien_multiply8 */
 } ien_input8;
 
 /* out[r] = act(input[r] . w + bias + add[r]) for rows row0 .. row0 + rows of
  * the input (IMAGE: of its output pixels, images x ceil(height / step) x
  * ceil(width / step)), into f16 or f32 NHWC rows `out->stride` elements apart
- * (row row0 at out->data; add's rows likewise).  Sums are f32, rounded once.
- * The 8-bit matrix instructions that f16 outputs take line neighbouring
- * products up on some 16 bits before they are added, which puts a sum 1.5e-5
- * of itself off: less than the f16 rounding after it, unless a later step
- * rounds to 8 bits again, where a tie that falls the other way counts.  With
- * input->exact, and for f32 outputs always, the products are added in f32, at
- * half the rate.
+ * (row row0 at out->data; add's rows likewise).  Products are added in f32,
+ * and their sum is rounded once.
+ * With input->fast (f16 outputs; f32 ones ignore it) the 8-bit matrix
+ * instructions add them, at twice the rate: those line neighbouring products
+ * up on fewer bits first, which puts a sum of alike products 1.5e-5 of itself
+ * off.
  * Rows in 8 bits are less than 1 MiB apart, a line of a map's pixels (and 256
  * more) less than 128 MiB, and weights less than 32 GiB.
  * d_add (or NULL): rows of out's type, add_stride elements apart; it may be
