@@ -46,3 +46,40 @@ def test_small_products_of_a_map(ctx):
     y = torch.full((2 * 8 * 24, 40), 9.0, dtype=torch.float16, device="cuda")
     ien.conv8(ctx, rows8_of(*E.quantize(x), 128), 2, 8, 24, ien.Matrix8(ctx, w, taps=9), y)
     assert bool((y == 0.25).all())
+
+
+def exponents(data, scales):
+    """The powers of two of bytes under their scales, [rows, k]: at least -6 before the scale."""
+    e = np.maximum(np.frexp(np.nan_to_num(E.E4M3[data]))[1] - 1, -6)
+    e = np.where(E.E4M3[data] == 0, -6, e)
+    return e + np.repeat(scales.astype(int) - 127, 128, 1)
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 128, 24), (37, 1152, 72), (300, 512, 136), (4096, 256, 136)])
+def test_fast_sums(ctx, rows, k, n):
+    """exact=False, where neighbours cancel and values lie far apart: each eight
+    products are off by at most 8 times 2^-13 of the largest one's power of two, the
+    sums by a step of f32 each, the result by half a step of f16."""
+    import ien
+    import torch
+
+    rng = np.random.default_rng(rows + k)
+    x = (rng.standard_normal((rows, k)) * 2.0 ** rng.integers(-9, 9, (rows, k))).astype(np.float32)
+    w = (rng.standard_normal((k, n)) * 2.0 ** rng.integers(-4, 4, (k, n))).astype(np.float32)
+    x[:, 1::2] = x[:, ::2] * (1 + 2.0**-4 * rng.standard_normal((rows, k // 2)))
+    w[1::2] = -w[::2]
+    data, scales = E.quantize(x)
+    m = ien.Matrix8(ctx, w)
+    y = torch.full((rows, n), 9.0, dtype=torch.float16, device="cuda")
+    ien.multiply8(ctx, rows8_of(data, scales, k), m, y, exact=False)
+    wdata, wscales = E.quantize(np.ascontiguousarray(w.T))
+    x8, w8 = E.values(data, scales, k), E.values(wdata, wscales, k).T
+    want = x8 @ w8
+    ex, ew = exponents(data, scales).reshape(rows, -1, 8), exponents(wdata, wscales).reshape(n, -1, 8)
+    off = np.zeros((rows, n))
+    for g in range(k // 8):
+        off += 2.0 ** (ex[:, None, g] + ew[None, :, g]).max(2)
+    tol = 8 * 2.0**-13 * off + (k + 2) * 2.0**-23 * (np.abs(x8) @ np.abs(w8)) + 2.0**-11 * np.abs(want) + 2.0**-25
+    with np.errstate(over="ignore"):
+        assert (np.abs(want) + tol < 65504).all()
+    assert (np.abs(y.double().cpu().numpy() - want) <= tol).all()
