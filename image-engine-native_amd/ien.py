@@ -592,21 +592,25 @@ class Swin:
 
 class Rows8:
     """ien_rows8 over torch tensors: `rows` rows of k values in 8 bits (data:
-    uint8 [rows, stride], scales: uint8 [rows, scale_stride]), made here
-    unless given.  The tensors stay this object's (their addresses are read
-    once, here); another Rows8 takes other ones, views of these among them."""
+    uint8 [rows, at least ien_rows8_stride(k)], scales: uint8 [rows, at least
+    ien_rows8_scale_stride(k)]), made here unless given.  The tensors stay this
+    object's (their addresses are read once, here); another Rows8 takes other
+    ones, views of these among them."""
 
     def __init__(self, rows, k, data=None, scales=None, device="cuda"):
         import torch
 
         L = load()
+        widths = L.ien_rows8_stride(k), L.ien_rows8_scale_stride(k)
         if data is None:
-            data = torch.empty(rows, L.ien_rows8_stride(k), dtype=torch.uint8, device=device)
+            data = torch.empty(rows, widths[0], dtype=torch.uint8, device=device)
         if scales is None:
-            scales = torch.empty(rows, L.ien_rows8_scale_stride(k), dtype=torch.uint8, device=data.device)
-        for t in (data, scales):
+            scales = torch.empty(rows, widths[1], dtype=torch.uint8, device=data.device)
+        for t, width in zip((data, scales), widths):
             if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
                 raise ValueError("rows in 8 bits are uint8 tensors of rows x bytes")
+            if rows and t.shape[1] < width:
+                raise ValueError(f"rows of {k} values in 8 bits take {width} bytes, not {t.shape[1]}")
         if data.device != scales.device:
             raise ValueError(f"rows in 8 bits on {data.device} and {scales.device}")
         self.rows, self.k, self._data, self._scales = rows, k, data, scales
