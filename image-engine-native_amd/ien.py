@@ -615,6 +615,7 @@ class Rows8:
             raise ValueError(f"rows in 8 bits on {data.device} and {scales.device}")
         self.rows, self.k, self._data, self._scales = rows, k, data, scales
         self._fields = data.data_ptr(), _row_stride(data), scales.data_ptr(), _row_stride(scales)
+        self._device = data.get_device()
         self._struct = Rows8Struct(*self._fields)
         self._at = ctypes.addressof(self._struct)
 
@@ -645,8 +646,8 @@ def _out_type(dtype):
     return _OUT_TYPES[dtype]
 
 
-def _rows_of(t):
-    """(rows, columns, address, type, stride) of a tensor of rows on the GPU."""
+def _rows_of(ctx, t):
+    """(rows, columns, address, type, stride) of a tensor of rows on the context's GPU."""
     shape, strides = t.shape, t.stride()
     if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
         raise ValueError("rows x channels with contiguous channels expected")
@@ -654,14 +655,22 @@ def _rows_of(t):
     stride = strides[0]
     if not t.is_cuda:
         raise ValueError(f"a tensor on the GPU expected, not on {t.device}")
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, t.device)
     return rows, c, t.data_ptr(), _out_type(t.dtype), stride if rows > 1 or stride > c else c
+
+
+def _elsewhere(ctx, device):
+    return ValueError(f"a tensor on the context's GPU {ctx.device} expected, not on {device}")
 
 
 def quantize8(ctx, x, out):
     """Rows x k (f16 or f32 tensor) into the Rows8 `out`."""
-    rows, k, at, kind, stride = _rows_of(x)
+    rows, k, at, kind, stride = _rows_of(ctx, x)
     if rows != out.rows or k != out.k:
         raise ValueError(f"{tuple(x.shape)} into {out.rows} rows of {out.k}")
+    if out._device != ctx.device:
+        raise _elsewhere(ctx, out.data.device)
     status = (_lib or load()).ien_quantize8(ctx.h, at, kind, rows, k, stride, out._at)
     if status:
         check(status)
@@ -669,9 +678,11 @@ def quantize8(ctx, x, out):
 
 def dequantize8(ctx, x, y):
     """The values of the Rows8 `x` into the rows x k tensor y (f16 or f32)."""
-    rows, k, at, kind, stride = _rows_of(y)
+    rows, k, at, kind, stride = _rows_of(ctx, y)
     if rows != x.rows or k != x.k:
         raise ValueError(f"{x.rows} rows of {x.k} into {tuple(y.shape)}")
+    if x._device != ctx.device:
+        raise _elsewhere(ctx, x.data.device)
     status = (_lib or load()).ien_dequantize8(ctx.h, x._at, rows, k, at, kind, stride)
     if status:
         check(status)
@@ -715,13 +726,17 @@ _INPUT8, _OUTPUT = struct.Struct("@iPNPNNNNNi").pack, struct.Struct("@PNii").pac
 
 
 def _multiply8(ctx, x, shape, row0, matrix, out, act, add, exact):
-    rows, n, at, kind, stride = _rows_of(out)
+    rows, n, at, kind, stride = _rows_of(ctx, out)
     if x.k != matrix.c or n != matrix.n:
         raise ValueError(f"rows of {x.k} by {matrix.c} x {matrix.n} into {tuple(out.shape)}")
+    if x._device != ctx.device:
+        raise _elsewhere(ctx, x.data.device)
+    if matrix.ctx.device != ctx.device:
+        raise _elsewhere(ctx, f"GPU {matrix.ctx.device}")
     add_at = None
     add_stride = 0
     if add is not None:
-        add_rows, add_n, add_at, add_kind, add_stride = _rows_of(add)
+        add_rows, add_n, add_at, add_kind, add_stride = _rows_of(ctx, add)
         if add_rows != rows or add_n != n or add_kind != kind:
             raise ValueError("what is added has the output's shape and type")
     status = (_lib or load()).ien_multiply8(ctx.h, _INPUT8(shape[0], *x._fields, *shape[1:], 0 if exact else 1), row0, rows, matrix.h,
@@ -749,12 +764,14 @@ def conv8(ctx, x, images, height, width, matrix, out, step=1, act=ACT_NONE, add=
     _multiply8(ctx, x, (INPUT_IMAGE, images, height, width, step), row0, matrix, out, act, add, exact)
 
 
-def _channels_of(t, c):
-    """The address of c f32 values on the GPU, or None."""
+def _channels_of(ctx, t, c):
+    """The address of c f32 values on the context's GPU, or None."""
     if t is None:
         return None
     if t.shape != (c,) or not t.is_cuda or not t.is_contiguous() or _out_type(t.dtype) != OUT_F32:
         raise ValueError(f"gamma and beta are {c} contiguous f32 values on the GPU")
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, t.device)
     return t.data_ptr()
 
 
@@ -762,22 +779,24 @@ def group_norm(ctx, x, images, groups, gamma, beta, y, eps=1e-5, act=ACT_NONE):
     """act(group norm) of `images` maps of x.shape[0] / images pixels (x: rows x
     channels, f16 or f32) into y: a tensor of x's shape (f16 or f32, x itself
     too), or a Rows8.  gamma, beta: f32 tensors, or None for 1 and 0."""
-    rows, c, at, kind, stride = _rows_of(x)
+    rows, c, at, kind, stride = _rows_of(ctx, x)
     if images < 1 or rows % images:
         raise ValueError(f"{rows} pixels in {images} maps")
     if isinstance(y, Rows8):
         if y.rows != rows or y.k != c:
             raise ValueError("the result has the input's rows and channels")
+        if y._device != ctx.device:
+            raise _elsewhere(ctx, y.data.device)
         status = (_lib or load()).ien_group_norm8(
-            ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(gamma, c), _channels_of(beta, c),
-            eps, act, y._at)
+            ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(ctx, gamma, c),
+            _channels_of(ctx, beta, c), eps, act, y._at)
     else:
-        y_rows, y_c, y_at, y_kind, y_stride = _rows_of(y)
+        y_rows, y_c, y_at, y_kind, y_stride = _rows_of(ctx, y)
         if y_rows != rows or y_c != c:
             raise ValueError("the result has the input's rows and channels")
         status = (_lib or load()).ien_group_norm(
-            ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(gamma, c), _channels_of(beta, c),
-            eps, act, y_at, y_kind, y_stride)
+            ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(ctx, gamma, c),
+            _channels_of(ctx, beta, c), eps, act, y_at, y_kind, y_stride)
     if status:
         check(status)
 

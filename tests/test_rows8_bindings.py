@@ -26,3 +26,74 @@ def test_rows8_takes_wide_enough_tensors():
     q = ien.Rows8(6, 640, data=byte_rows(6, 640, 1024), scales=byte_rows(6, 8))
     assert q._fields[1] == 1024 and q._fields[3] == 8
     assert ien.Rows8(0, 640, data=byte_rows(0, 640), scales=byte_rows(0, 8)).rows == 0
+
+
+class OnGpu:
+    """What the bindings read of a tensor on GPU `index`; its address is never followed."""
+
+    def __init__(self, rows, c, index=0, dtype=torch.float16, flat=False):
+        self.shape, self._strides = ((c,), (1,)) if flat else ((rows, c), (c, 1))
+        self.index, self.dtype, self.is_cuda, self.device = index, dtype, True, f"cuda:{index}"
+
+    def stride(self):
+        return self._strides
+
+    def data_ptr(self):
+        return 0x10000
+
+    def get_device(self):
+        return self.index
+
+    def is_contiguous(self):
+        return True
+
+
+class Somewhere(ien.Rows8):
+    """Rows on GPU `index` (-1: the host) without tensors there."""
+
+    def __init__(self, rows, k, index):
+        super().__init__(rows, k, device="cpu")
+        self._device = index
+
+
+CTX = type("Context", (), dict(h=None, device=0))()
+OTHER = type("Context", (), dict(h=None, device=1))()
+
+
+def calls(x, q, gamma=None, matrix_ctx=CTX):
+    m = type("Matrix8", (), dict(h=None, c=40, n=40, taps=1, ctx=matrix_ctx))()
+    return [lambda: ien.quantize8(CTX, x, q), lambda: ien.dequantize8(CTX, q, x),
+            lambda: ien.multiply8(CTX, q, m, x), lambda: ien.conv8(CTX, q, 1, 2, 3, m, x),
+            lambda: ien.group_norm(CTX, x, 1, 8, gamma, None, q), lambda: ien.group_norm(CTX, x, 1, 8, None, gamma, q)]
+
+
+@pytest.mark.parametrize("index", [-1, 1])
+def test_rows8_of_the_host_or_another_gpu(index):
+    for call in calls(OnGpu(6, 40), Somewhere(6, 40, index)):
+        with pytest.raises(ValueError, match="GPU 0"):
+            call()
+
+
+def test_tensors_of_another_gpu():
+    here, there = OnGpu(6, 40), OnGpu(6, 40, 1)
+    for call in calls(there, Somewhere(6, 40, 0)):
+        with pytest.raises(ValueError, match="GPU 0"):
+            call()
+    for call in calls(here, Somewhere(6, 40, 0), OnGpu(1, 40, 1, torch.float32, flat=True))[4:]:
+        with pytest.raises(ValueError, match="GPU 0"):
+            call()
+    for call in calls(here, Somewhere(6, 40, 0), matrix_ctx=OTHER)[2:4]:
+        with pytest.raises(ValueError, match="GPU 0"):
+            call()
+    m = type("Matrix8", (), dict(h=None, c=40, n=40, taps=1, ctx=CTX))()
+    for call in (lambda: ien.multiply8(CTX, Somewhere(6, 40, 0), m, here, add=there),
+                 lambda: ien.group_norm(CTX, here, 1, 8, None, None, there)):
+        with pytest.raises(ValueError, match="GPU 0"):
+            call()
+
+
+def test_tensors_of_the_contexts_gpu_reach_the_library():
+    """(Which refuses: these contexts hold none of its own.)"""
+    for call in calls(OnGpu(6, 40), Somewhere(6, 40, 0), OnGpu(1, 40, 0, torch.float32, flat=True)):
+        with pytest.raises(ien.IenError):
+            call()
