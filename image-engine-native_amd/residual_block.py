@@ -20,22 +20,30 @@ import ien
 class ResidualBlock8:
     """The weights (f32 or f16 numpy, (9 c) x c with the taps row-major and
     the channels fastest, and c biases) of two convolutions, quantised once,
-    and the f32 gains (gamma, beta: torch, on the GPU) of two group norms."""
+    and the f32 gains (gamma, beta: torch, on the GPU) of two group norms.
+
+    The first run of each number of rows makes the two maps between its steps
+    (3 c bytes a row, and the scales); they stay the block's until free(), so a
+    captured run has them for as long as the block lives.  Runs share them:
+    like all calls of a context, which share its workspace, those of one block
+    follow each other, a graph's replays among them."""
 
     def __init__(self, ctx, c, groups, norms, convs, eps=1e-5):
         self.ctx, self.c, self.groups, self.norms, self.eps = ctx, c, groups, norms, eps
         self.convs = [ien.Matrix8(ctx, w, b, taps=9) for w, b in convs]
-        self._work = None
+        self._work = {}  # rows: the map in 8 bits, the map between the halves
 
     def run(self, x, images, height, width, out=None):
-        """f16 rows x channels (a pixel a row, one map after the other) into
-        `out` (or a new tensor; not x itself), in the order of the context's
-        stream."""
+        """f16 or f32 rows x channels (a pixel a row, one map after the other)
+        into `out` (or a new tensor; not x itself), in the order of the
+        context's stream."""
         import torch
 
-        if self._work is None or self._work[0].rows != x.shape[0]:
-            self._work = ien.Rows8(x.shape[0], self.c), torch.empty(x.shape[0], self.c, dtype=torch.float16, device=x.device)
-        q, h = self._work
+        rows = x.shape[0]
+        if rows not in self._work:
+            self._work[rows] = (ien.Rows8(rows, self.c, device=x.device),
+                                torch.empty(rows, self.c, dtype=torch.float16, device=x.device))
+        q, h = self._work[rows]
         out = torch.empty_like(x) if out is None else out
         shape = images, height, width
         ien.group_norm(self.ctx, x, images, self.groups, *self.norms[0], q, eps=self.eps, act=ien.ACT_SILU)
@@ -45,6 +53,7 @@ class ResidualBlock8:
         return out
 
     def free(self):
+        self._work.clear()
         for m in self.convs:
             m.free()
 
