@@ -94,7 +94,8 @@ __device__ __forceinline__ Eight<T> load_eight(const T *row, int at, int c) {
 // statistics.
 template <bool ALL, int U>
 __device__ __forceinline__ void take(const float (&v)[U][8], int many, float &n, float (&m)[8], float (&q)[8]) {
-  const float k = ALL ? (float)U : (float)many, w = share(k, n + k), nw = n * w;
+  // (The first batch is taken as it is: k rcp(k) may be a step off 1.)
+  const float k = ALL ? (float)U : (float)many, w = n > 0.0f ? share(k, n + k) : 1.0f, nw = n * w;
   float counts[U];
 #pragma unroll
   for (int u = 0; u < U; u++) counts[u] = u < many ? 1.0f : 0.0f;
@@ -161,9 +162,10 @@ __device__ __forceinline__ void by_group(const Shared &s, const Place &p, float 
   auto at = [&](int r) { return (r & (runs - 1)) * s.lanes + r / runs; };
   if (many <= 8) {
     for (int g = t; g < span / per; g += s.lanes) {
+      const float base = s.m[at(g * many)];  // (sums from it on: of equal means exact)
       float mean = 0.0f, squares = 0.0f;
-      for (int r = 0; r < many; r++) mean += s.m[at(g * many + r)];
-      mean /= (float)many;
+      for (int r = 1; r < many; r++) mean += s.m[at(g * many + r)] - base;
+      mean = base + mean / (float)many;
       for (int r = 0; r < many; r++) {
         const float d = s.m[at(g * many + r)] - mean;
         squares += s.q[at(g * many + r)] + each * d * d;
@@ -172,9 +174,10 @@ __device__ __forceinline__ void by_group(const Shared &s, const Place &p, float 
     }
   } else {
     for (int g = t >> 6; g < span / per; g += s.lanes >> 6) {
+      const float base = s.m[at(g * many)];
       float mean = 0.0f, squares = 0.0f;
-      for (int r = t & 63; r < many; r += 64) mean += s.m[at(g * many + r)];
-      mean = group_sum<64>(mean) / (float)many;
+      for (int r = t & 63; r < many; r += 64) mean += s.m[at(g * many + r)] - base;
+      mean = base + group_sum<64>(mean) / (float)many;
       for (int r = t & 63; r < many; r += 64) {
         const float d = s.m[at(g * many + r)] - mean;
         squares += s.q[at(g * many + r)] + each * d * d;
