@@ -31,6 +31,9 @@ inline size_t blocks8(size_t k) { return (k + BLOCK8 - 1) / BLOCK8; }
 // Rows in 8 bits that an entry point was handed, or its refusal.
 ien_status check_rows8(const ien_rows8 *r, size_t k, const char *what);
 
+// quantize8.hip: workgroups for rows of that many blocks in all.
+unsigned quantize8_grid(long blocks);
+
 // multiply8.hip: 64 x the tile + the splits of the depth of a product of `rows`
 // rows, `chunks` blocks deep, n outputs.
 int multiply8_choice(int cus, long workspace, long rows, long n, int chunks, bool exact, bool add);
