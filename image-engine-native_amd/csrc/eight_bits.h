@@ -34,6 +34,19 @@ ien_status check_rows8(const ien_rows8 *r, size_t k, const char *what);
 // quantize8.hip: workgroups for rows of that many blocks in all.
 unsigned quantize8_grid(long blocks);
 
+// group_norm.hip: the launches of a norm of `images` maps of `pixels` pixels, c
+// channels in `groups` groups, into results of y_bytes.
+struct NormPlan {
+  long one;     // one launch (or two, over `chunks` parts of an image of `chunk` pixels)
+  long span;    // channels a workgroup handles (c, or a part in one launch)
+  long px;      // pixels side by side in one launch
+  long chunks, chunk;
+  long lanes;   // of a workgroup
+  long groups;  // workgroups an image
+  long images;  // of a turn: no launch has 2^32 lanes, and their parts fit the workspace
+};
+NormPlan norm_plan(int cus, long workspace, long images, long pixels, int c, int groups, int y_bytes);
+
 // multiply8.hip: 64 x the tile + the splits of the depth of a product of `rows`
 // rows, `chunks` blocks deep, n outputs.
 int multiply8_choice(int cus, long workspace, long rows, long n, int chunks, bool exact, bool add);

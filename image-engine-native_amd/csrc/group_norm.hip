@@ -19,6 +19,8 @@
 // 5.3 TB/s of the three passes.  Maps of a few hundred pixels take one launch, a
 // workgroup a few groups (16 x 16 x 512: 7.4 us).
 
+#include <algorithm>
+
 #include "eight_bits.h"
 
 namespace ien {
@@ -429,33 +431,24 @@ int smallest_span(int c, int per, int unit) {
 
 ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_bytes) {
   const int per = a.c / a.groups;
-  // One launch where a lane's share is a few pixels.
-  const int wide = smallest_span(a.c, per, 128);
-  a.px = std::min(64, LANES / ((wide + 127) / 128 * 16));
-  const bool one = a.pixels <= 8 * a.px;
-  a.span = !one ? a.c : y_bytes == 1 ? wide : smallest_span(a.c, per, 8);
-  const int eights = (a.span + 7) / 8, one_lanes = ((y_bytes == 1 ? (eights + 15) / 16 * 16 : eights) * a.px + 63) / 64 * 64;
-  // Otherwise a workgroup a part of at least four rounds of pixels: one for each
-  // CU of a long map; of a shorter one, whose second pass spends most of its time on
-  // joining the parts, one for every other CU.
-  const int lanes = eights <= 512 ? 512 : LANES, px = lanes / eights;
-  const long rounds = (a.pixels + px - 1) / px, most_parts = images * a.pixels * eights > 2048L * ctx->cus ? ctx->cus : ctx->cus / 2;
-  const long parts = std::max(1L, std::min((rounds + 3) / 4, most_parts / images));
-  a.chunk = std::min((rounds + parts - 1) / parts, (1L << 30) / px) * px;  // (counted in 32 bits)
-  a.chunks = (int)((a.pixels + a.chunk - 1) / a.chunk);
+  const NormPlan plan = norm_plan(ctx->cus, (long)ctx->splitk_floats, images, a.pixels, a.c, a.groups, y_bytes);
+  a.span = (int)plan.span;
+  a.px = (int)plan.px;
+  a.chunks = (int)plan.chunks;
+  a.chunk = plan.chunk;
   a.part = (float2 *)ctx->splitk;
-  const long most = one ? 1L << 16 : std::max(1L, (long)(ctx->splitk_floats / 2) / ((long)a.chunks * a.groups));
+  const int lanes = (int)plan.lanes;
   const void *x = a.x;
   uint8_t *y = (uint8_t *)a.y, *scales = a.scales;
   auto go_eights = [&](auto t, auto u, auto e, long many) {
     using T = decltype(t);
     using Y = decltype(u);
     constexpr bool E = decltype(e)::value;
-    if (one) {
-      const size_t shared = shared_floats(one_lanes) * 4 + a.span / per * sizeof(float2);
-      hipLaunchKernelGGL((k_norm_one<T, Y, E>), dim3((unsigned)(many * (a.c / a.span))), dim3(one_lanes), shared, ctx->stream, a);
+    const dim3 grid((unsigned)(many * plan.groups));
+    if (plan.one) {
+      const size_t shared = shared_floats(lanes) * 4 + a.span / per * sizeof(float2);
+      hipLaunchKernelGGL((k_norm_one<T, Y, E>), grid, dim3(lanes), shared, ctx->stream, a);
     } else {
-      const dim3 grid((unsigned)(many * a.chunks));
       hipLaunchKernelGGL((k_norm_stats<T, E>), grid, dim3(lanes), shared_floats(lanes) * 4, ctx->stream, a);
       hipLaunchKernelGGL((k_norm_apply<T, Y, E>), grid, dim3(lanes), 2 * lanes * 4 + a.groups * sizeof(float2), ctx->stream, a);
     }
@@ -465,8 +458,8 @@ ien_status run(ien_ctx *ctx, NormArgs a, long images, ien_out_type type, int y_b
     in_eights ? go_eights(t, u, Act<1>{}, many) : go_eights(t, u, Act<0>{}, many);
   };
   const int x_bytes = type == IEN_OUT_F16 ? 2 : 4;
-  for (long i = 0; i < images; i += most) {  // (one turn but for a great many images)
-    const long many = std::min(most, images - i), r = i * a.pixels;
+  for (long i = 0; i < images; i += plan.images) {  // (one turn but for a great many images)
+    const long many = std::min(plan.images, images - i), r = i * a.pixels;
     a.x = (const uint8_t *)x + r * a.stride * x_bytes;
     a.y = y + r * a.ystride * y_bytes;
     a.scales = scales + r * a.scale_stride;
@@ -506,6 +499,38 @@ ien_status describe(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t ima
 }
 
 }  // namespace
+
+NormPlan norm_plan(int cus, long workspace, long images, long pixels, int c, int groups, int y_bytes) {
+  NormPlan p{};
+  const int per = c / groups;
+  // One launch where a lane's share is a few pixels.
+  const int wide = smallest_span(c, per, 128);
+  p.px = std::min(64, LANES / ((wide + 127) / 128 * 16));
+  p.one = pixels <= 8 * p.px;
+  p.span = !p.one ? c : y_bytes == 1 ? wide : smallest_span(c, per, 8);
+  const long eights = (p.span + 7) / 8;
+  if (p.one) {
+    p.lanes = ((y_bytes == 1 ? (eights + 15) / 16 * 16 : eights) * p.px + 63) / 64 * 64;
+    p.chunks = 1;
+    p.chunk = pixels;
+    p.groups = c / p.span;
+  } else {
+    // A workgroup a part of at least four rounds of pixels: one for each CU of a
+    // long map; of a shorter one, whose second pass spends most of its time on
+    // joining the parts, one for every other CU.
+    p.lanes = eights <= 512 ? 512 : LANES;
+    const long px = p.lanes / eights, rounds = (pixels + px - 1) / px;
+    const long most_parts = images * pixels * eights > 2048L * cus ? cus : cus / 2;
+    const long parts = std::max(1L, std::min((rounds + 3) / 4, most_parts / images));
+    p.chunk = std::min((rounds + parts - 1) / parts, (1L << 30) / px) * px;  // (counted in 32 bits)
+    p.chunks = (pixels + p.chunk - 1) / p.chunk;
+    p.groups = p.chunks;
+  }
+  const long fit = p.one ? images : workspace / 2 / (p.chunks * groups);
+  p.images = std::max(1L, std::min({images, fit, (1L << 31) / (p.groups * p.lanes)}));
+  return p;
+}
+
 }  // namespace ien
 
 using namespace ien;

@@ -15,3 +15,38 @@ def test_quantize8(blocks):
     grid = _function("_ZN3ien14quantize8_gridEl", ctypes.c_long, restype=ctypes.c_uint)(blocks)
     assert 1 <= grid and grid * 256 < LANES
     assert grid == min(-(-blocks // 16), 1 << 20)  # one turn, but for more than 2 GiB of blocks
+
+
+class NormPlan(ctypes.Structure):
+    """eight_bits.h NormPlan."""
+    _fields_ = [(n, ctypes.c_long) for n in ("one", "span", "px", "chunks", "chunk", "lanes", "groups", "images")]
+
+
+CUS, WORKSPACE = 256, 8 << 20  # MI355X; the context's workspace in floats
+
+
+def norm_plan(images, pixels, c, groups, y_bytes):
+    f = _function("_ZN3ien9norm_planEillliii", ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_long, ctypes.c_int,
+                  ctypes.c_int, ctypes.c_int, restype=NormPlan)
+    return f(CUS, WORKSPACE, images, pixels, c, groups, y_bytes)
+
+
+@pytest.mark.parametrize("y_bytes", [1, 2, 4])
+@pytest.mark.parametrize("c,groups", [(1, 1), (7, 1), (8, 1), (64, 8), (512, 32), (640, 32), (2056, 8), (4090, 10), (4104, 1), (8184, 1023),
+                                      (8191, 8191), (8192, 1), (8192, 64), (8192, 1024), (8192, 8192)])
+def test_group_norm(c, groups, y_bytes):
+    for images in (1, 2, 255, 256, 257, 65535, 65536, 65537, 2**20 - 1):
+        for pixels in (1, 2, 8, 9, 512, 513, 5000, 2**20 + 1, 2**32, 2**40 - 1):
+            p = norm_plan(images, pixels, c, groups, y_bytes)
+            assert 1 <= p.images <= images and 64 <= p.lanes <= 1024 and p.lanes % 64 == 0
+            assert p.images * p.groups * p.lanes < LANES
+            assert p.chunks * p.chunk >= pixels and (p.chunks - 1) * p.chunk < pixels
+            assert p.span % (c // groups) == 0 and c % p.span == 0
+            if p.one:
+                assert p.groups == c // p.span and p.px * -(-p.span // 8) <= p.lanes
+                assert 68 * p.lanes + 8 * p.span // (c // groups) <= 160 << 10  # LDS
+            else:
+                assert p.groups == p.chunks and p.chunk <= 1 << 30 and 8 * p.lanes + 8 * groups <= 160 << 10
+                # (One image's parts fit the workspace, but where no card's memory holds it.)
+                if pixels * c < 2**40:
+                    assert 2 * p.images * p.chunks * groups <= WORKSPACE

@@ -28,3 +28,31 @@ def test_quantize8_in_turns(ctx):
     assert bool(((y - x).abs() <= tol).all())
     del x, q, y, tol
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("images,pixels,c,groups", [(65600, 1, 8192, 1024), (70000, 2, 512, 64)])
+@pytest.mark.parametrize("into", ["float16", "8 bits"])
+def test_group_norm_of_many_maps(ctx, images, pixels, c, groups, into):
+    """More workgroups than a launch has: maps at both ends and where turns meet have the
+    bits that they have alone."""
+    import ien
+    import torch
+
+    x = torch.randn(images * pixels, c, device="cuda").half()
+
+    def run(x, images):
+        if into == "8 bits":
+            y = ien.Rows8(images * pixels, c)
+            ien.group_norm(ctx, x, images, groups, None, None, y, act=ien.ACT_SILU)
+            return y.data, y.scales[:, :c // 128]
+        y = torch.empty_like(x)
+        ien.group_norm(ctx, x, images, groups, None, None, y, act=ien.ACT_SILU)
+        return (y,)
+
+    whole = run(x, images)
+    for begin in (0, 32768 - 20, 65536 - 40, images - 50):
+        rows = slice(begin * pixels, (begin + 50) * pixels)
+        for w, p in zip(whole, run(x[rows].contiguous(), 50)):
+            assert torch.equal(w[rows], p)
+    del x, whole
+    torch.cuda.empty_cache()
