@@ -50,6 +50,8 @@ NormPlan norm_plan(int cus, long workspace, long images, long pixels, int c, int
 // multiply8.hip: 64 x the tile + the splits of the depth of a product of `rows`
 // rows, `chunks` blocks deep, n outputs.
 int multiply8_choice(int cus, long workspace, long rows, long n, int chunks, bool exact, bool add);
+// The rows of one launch of that tile, at most.
+long multiply8_part(int tile, long n);
 
 typedef int int2v __attribute__((ext_vector_type(2)));
 

@@ -29,6 +29,8 @@
 // idle.  8192 x 8192 -> 8192: 411 us, 2.67 PFLOP/s; 16384 rows 2048 -> 8192 249
 // to 259 us, 202 without the epilogue.
 
+#include <algorithm>
+
 #include "eight_bits.h"
 
 namespace ien {
@@ -440,10 +442,8 @@ void launch(ien_ctx *ctx, Args8 &a) {
     hipLaunchKernelGGL((k_tile8<T, false, _Float16>), grid, dim3(T::THREADS), 0, ctx->stream, a);
 }
 
-void run_tiles(ien_ctx *ctx, Args8 &a) {
+void run_part(ien_ctx *ctx, Args8 &a, int tile, int ksplit) {
   const int chunks = a.taps * a.cb;
-  const int plan = multiply8_choice(ctx->cus, (long)ctx->splitk_floats, a.rows, a.n, chunks, a.exact, a.add);
-  const int tile = plan / 64, ksplit = plan % 64;
   const Choice8 &c = CHOICES8[tile];
   a.tiles_m = (int)((a.rows + c.tm - 1) / c.tm);
   a.tiles_n = (int)((a.n + c.tn - 1) / c.tn);
@@ -464,7 +464,26 @@ void run_tiles(ien_ctx *ctx, Args8 &a) {
   }
 }
 
+void run_tiles(ien_ctx *ctx, const Args8 &a) {
+  const int plan = multiply8_choice(ctx->cus, (long)ctx->splitk_floats, a.rows, a.n, a.taps * a.cb, a.exact, a.add);
+  const long part = multiply8_part(plan / 64, a.n);
+  for (long r = 0; r < a.rows; r += part) {  // (one turn but for some 10^10 outputs)
+    Args8 p = a;
+    p.row0 += r;
+    p.rows = std::min(part, a.rows - r);
+    p.y = (uint8_t *)a.y + r * a.ys * (a.f32 ? 4 : 2);
+    if (a.add) p.add = (const uint8_t *)a.add + r * a.as * (a.f32 ? 4 : 2);
+    run_part(ctx, p, plan / 64, plan % 64);
+  }
+}
+
 }  // namespace
+
+// 2^21 tiles, which at 512 lanes are 2^30: a launch counts its lanes in 32 bits.
+long multiply8_part(int tile, long n) {
+  const Choice8 &c = CHOICES8[tile];
+  return std::max((1L << 21) / ((n + c.tn - 1) / c.tn), 1L) * c.tm;
+}
 
 // The tile (times 64) and in how many splits of the depth: by the estimated
 // time.  Few tiles leave CUs idle, which splits fill for a pass through device

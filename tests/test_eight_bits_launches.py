@@ -50,3 +50,26 @@ def test_group_norm(c, groups, y_bytes):
                 # (One image's parts fit the workspace, but where no card's memory holds it.)
                 if pixels * c < 2**40:
                     assert 2 * p.images * p.chunks * groups <= WORKSPACE
+
+
+def multiply8_plan(rows, n, chunks, exact, add):
+    choice = _function("_ZN3ien16multiply8_choiceEilllibb", ctypes.c_int, ctypes.c_long, ctypes.c_long, ctypes.c_long,
+                       ctypes.c_int, ctypes.c_bool, ctypes.c_bool)
+    tile, splits = divmod(choice(CUS, WORKSPACE, rows, n, chunks, exact, add), 64)
+    return tile, splits, _function("_ZN3ien14multiply8_partEil", ctypes.c_int, ctypes.c_long, restype=ctypes.c_long)(tile, n)
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("add", [False, True])
+def test_multiply8(exact, add):
+    tiles = [(256, 256), (128, 128), (64, 128), (64, 64)]
+    for rows in (1, 64, 65, 4096, 2**20, 2**24, 2**27 + 1, 2**30, 2**33, 2**40 - 1):
+        for n in (1, 8, 64, 65, 129, 8192, 100000, 2**22 - 1):
+            for chunks in (1, 9, 64, 1000):
+                tile, splits, part = multiply8_plan(rows, n, chunks, exact, add)
+                tm, tn = tiles[tile]
+                assert part >= tm and part % tm == 0
+                across = -(-n // tn)
+                assert -(-min(part, rows) // tm) * across * splits * 512 < LANES
+                if -(-rows // tm) * across <= 2**21:
+                    assert part >= rows  # one launch

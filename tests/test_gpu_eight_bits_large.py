@@ -56,3 +56,34 @@ def test_group_norm_of_many_maps(ctx, images, pixels, c, groups, into):
             assert torch.equal(w[rows], p)
     del x, whole
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,add", [("float16", True), ("float32", False)])
+def test_multiply8_in_parts(ctx, dtype, add):
+    """More tiles than a launch has (17 GB of rows): rows at both ends and where the
+    parts meet have the bits that they have alone."""
+    import ien
+    import numpy as np
+    import torch
+
+    rows, k, n, dtype = (1 << 27) + 300, 24, 8, getattr(torch, dtype)
+    data = torch.randint(0, 120, (4096, 128), dtype=torch.uint8, device="cuda")
+    data[:, k:] = 0
+    data = data.repeat(rows // 4096 + 1, 1)[:rows]
+    q = ien.Rows8(rows, k, data=data)
+    q.scales.fill_(124)
+    rng = np.random.default_rng(1)
+    m = ien.Matrix8(ctx, rng.standard_normal((k, n)).astype(np.float32), rng.standard_normal(n).astype(np.float32))
+    y = torch.full((rows, n), float("nan"), dtype=dtype, device="cuda")
+    old = torch.randn(rows, n, device="cuda").to(dtype) if add else None
+    ien.multiply8(ctx, q, m, y, add=old)
+    for begin in (0, (1 << 27) - 200, rows - 250):
+        part = slice(begin, begin + 250)
+        p = ien.Rows8(250, k, data=data[part].contiguous())
+        p.scales.fill_(124)
+        z = torch.empty(250, n, dtype=dtype, device="cuda")
+        ien.multiply8(ctx, p, m, z, add=old[part].contiguous() if add else None)
+        assert torch.equal(y[part], z)
+    assert not bool(y.isnan().any())
+    del data, q, y, old
+    torch.cuda.empty_cache()
