@@ -14,8 +14,8 @@
 // loses bits by that: sums of 64 random products are off by 1.4e-5 of themselves,
 // and by all of themselves where large products cancel.  That is no sum in f32, and
 // left to a caller who asks for it (`fast`, f16 outputs).  All others take their
-// operands as bf16, which holds e4m3 values under any of the scales exactly,
-// and the bf16 instructions (6e-9), at half the rate.  (Rounded to 8 bits again
+// operands as bf16, which holds e4m3 values under scales 3 .. 246 exactly (past
+// those it ends: 2^128, 2^-133), and the bf16 instructions (6e-9), at half the rate.  (Rounded to 8 bits again
 // after a norm, f16 results off by 1.4e-5 gave a residual block of 64 x 64 x 512
 // an error of 4.6e-4 in place of 2.2e-4.)
 //

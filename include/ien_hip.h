@@ -256,7 +256,8 @@ size_t ien_rows8_scale_stride(size_t k); /* 4 ceil(k / 512) */
 ien_status ien_quantize8(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t rows, size_t k,
                          size_t stride, const ien_rows8 *out);
 /* The values that rows in 8 bits stand for, as f16 or f32 rows `stride`
- * elements apart (f32 holds each exactly; f16 rounds to nearest even, past
+ * elements apart (f32 holds each exactly, but for 2^128 and more, which scales
+ * from 247 on reach and which become infinity; f16 rounds to nearest even, past
  * 65504 to infinity). */
 ien_status ien_dequantize8(ien_ctx *ctx, const ien_rows8 *x, size_t rows, size_t k, void *d_y,
                            ien_out_type type, size_t stride);
@@ -287,7 +288,9 @@ typedef struct {
  * the input (IMAGE: of its output pixels, images x ceil(height / step) x
  * ceil(width / step)), into f16 or f32 NHWC rows `out->stride` elements apart
  * (row row0 at out->data; add's rows likewise).  Products are added in f32,
- * and their sum is rounded once.
+ * and their sum is rounded once.  Their operands are taken as bf16, which holds
+ * values under scales 3 .. 246 exactly: of the others, values of 2^128 and more
+ * become infinity, and small ones the nearest multiple of 2^-133.
  * With input->fast (f16 outputs; f32 ones ignore it) the 8-bit matrix
  * instructions add them, at twice the rate.  Those cut each aligned eight
  * products off towards zero at 2^-13 of the power of two of the largest one
