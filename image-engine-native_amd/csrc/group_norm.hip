@@ -317,7 +317,9 @@ __device__ __forceinline__ void apply(const NormArgs &a, const Line &l, Eight<T>
 
 // The parts' statistics joined, and the same part of the pixels again, from its
 // end.  The parts' means are summed from the first one's on, then the squares
-// about their mean; all but the last part hold a.chunk pixels.
+// about their mean; all but the last part hold a.chunk pixels.  A lane may have
+// some hundred parts to sum (one a group, where there are thousands), in f64: one
+// after the other in f32 they left means 2e-6 of a deviation off.
 template <typename T, typename Y, bool EIGHTS>
 __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
   constexpr int HERE = 16;  // parts a lane keeps for the second sum
@@ -370,19 +372,19 @@ __global__ __launch_bounds__(LANES) void k_norm_apply(NormArgs a) {
         for (int k = 0; k < min(rows, 16); k++) s += sums[k * many + t];
       return s;
     };
-    float s = 0.0f;
-    if (row < rows) each([&](float2 x, float n) { s += n * (x.x - base); });
-    s = sum(s);
+    double own = 0.0;
+    if (row < rows) each([&](float2 x, float n) { own += n * (x.x - base); });
+    float s = sum((float)own);
     if (row == 0) means[t] = base + s / (float)a.pixels;
     __syncthreads();
     const float mean = means[g];
-    s = 0.0f;
+    own = 0.0;
     if (row < rows)
       each([&](float2 x, float n) {
         const float d = x.x - mean;
-        s += n > 0.0f ? x.y + (n * per) * d * d : 0.0f;
+        own += n > 0.0f ? x.y + (n * per) * d * d : 0.0f;
       });
-    s = sum(s);
+    s = sum((float)own);
     if (row == 0) stats[g0 + t] = {mean, 1.0f / sqrtf(s / ((float)a.pixels * per) + a.eps)};
     __syncthreads();
   }
