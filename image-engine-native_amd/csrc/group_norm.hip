@@ -517,13 +517,12 @@ NormPlan norm_plan(int cus, long workspace, long images, long pixels, int c, int
     p.chunk = pixels;
     p.groups = c / p.span;
   } else {
-    // A workgroup a part of at least four rounds of pixels: one for each CU of a
-    // long map; of a shorter one, whose second pass spends most of its time on
-    // joining the parts, one for every other CU.
+    // A workgroup a part of at least four rounds of pixels, one for each CU where there
+    // are as many (one for every other CU: 64 x 96 x 640 14.4 -> 15.2 us, into 8
+    // bits 15.3 -> 17.2, 128 x 128 x 512 16.1 -> 19.2; 64 x 64 x 512, which has 128, 12.9).
     p.lanes = eights <= 512 ? 512 : LANES;
     const long px = p.lanes / eights, rounds = (pixels + px - 1) / px;
-    const long most_parts = images * pixels * eights > 2048L * cus ? cus : cus / 2;
-    const long parts = std::max(1L, std::min((rounds + 3) / 4, most_parts / images));
+    const long parts = std::max(1L, std::min((rounds + 3) / 4, cus / images));
     p.chunk = std::min((rounds + parts - 1) / parts, (1L << 30) / px) * px;  // (counted in 32 bits)
     p.chunks = (pixels + p.chunk - 1) / p.chunk;
     p.groups = p.chunks;

@@ -73,3 +73,9 @@ def test_multiply8(exact, add):
                 assert -(-min(part, rows) // tm) * across * splits * 512 < LANES
                 if -(-rows // tm) * across <= 2**21:
                     assert part >= rows  # one launch
+
+
+def test_a_part_of_a_norm_for_each_cu():
+    for pixels, c, chunks in ((6144, 640, 256), (16384, 512, 256), (4096, 512, 128), (131072, 64, 256)):
+        assert norm_plan(1, pixels, c, 32, 2).chunks == chunks
+    assert norm_plan(4, 16384, 512, 32, 2).chunks == 64
