@@ -454,8 +454,12 @@ void run_part(ien_ctx *ctx, Args8 &a, int tile, int ksplit) {
   const bool shared = (long)a.tiles_m * a.tiles_n * a.ksplit > ctx->cus;
   switch (tile) {
     case 0: launch<Tile8<4, 4, 2, 2, 2>>(ctx, a); break;
-    case 1:  // (Twice the waves for the residuals' loads: 3x3 256x384 256 -> 256 82 -> 77 us; without, 327 -> 337 us at 16384 rows.)
-      a.add ? launch<Tile8<1, 2, 4, 2, 2>>(ctx, a) : launch<Tile8<2, 2, 2, 2, 2>>(ctx, a);
+    case 1:
+      // Twice the waves: fast sums, for the residuals' loads (4096 rows 384 -> 1536 11.3 -> 9.9 us, 3x3 256x384 128 ->
+      // 128 27.2 -> 23.6; without a residual 16384 rows 2048 -> 8192 293 -> 296).  Exact ones, where a CU has one
+      // workgroup (2048 rows 8192 -> 2048 68.3 -> 63.8, with a residual 1024 rows 4096 -> 4096 38.9 -> 36.6);
+      // among others they lose (3x3 256x384 256 -> 256 97 -> 115, with a residual 102 -> 125).
+      (a.exact ? !shared : a.add != nullptr) ? launch<Tile8<1, 2, 4, 2, 2>>(ctx, a) : launch<Tile8<2, 2, 2, 2, 2>>(ctx, a);
       break;
     case 2:  // (Three workgroups a CU with two stages: 4096 rows 384 -> 1536 12.9 -> 10.5 us; one a CU wants three: 36 blocks deep 16.5, not 23.)
       shared ? launch<Tile8<1, 2, 2, 2, 2>>(ctx, a) : launch<Tile8<1, 2, 2, 2, 3>>(ctx, a);
