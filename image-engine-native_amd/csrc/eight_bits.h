@@ -141,7 +141,7 @@ __device__ __forceinline__ void store8(T *row, long at, long c, const float *v) 
 
 // Eight results of a row.  In f16 past the caches' order of use, for what no
 // cache would hold until it is read (it would put out what is still to be read:
-// 16384 rows 2048 -> 8192 295 -> 248 us, the norm of 512 x 768 x 128 64 -> 54).
+// 16384 rows 2048 -> 8192 with fast sums 295 -> 248 us, the norm of 512 x 768 x 128 64 -> 54).
 // f32 results go in two halves of a line a wave, which the caches have to join
 // (without them 98304 rows of 512 98 -> 115 us).
 template <typename T>

@@ -17,7 +17,9 @@
 // its end, so that some of it is still in the L2 of its XCD; the rest comes from
 // the memory-side cache where x fits that.  512 x 768 x 128 in f16: 21 + 37 us,
 // 5.3 TB/s of the three passes.  Maps of a few hundred pixels take one launch, a
-// workgroup a few groups (16 x 16 x 512: 7.4 us).
+// workgroup a few groups (16 x 16 x 512: 7.2 us).  Lanes to spare are what narrow
+// rows cost, most into 8 bits, where a pixel takes 16 (50000 x 8: 14.7 us into f16,
+// 55.5 into 8 bits).
 
 #include <algorithm>
 

@@ -22,12 +22,14 @@
 // A workgroup of four waves computes a tile of rows x outputs, a block of 128
 // deep at a time through a ring of stages in LDS that buffer loads fill without
 // registers; the 3 x 3 taps are the blocks' order, each lane's row at the tap's
-// pixel or, off the map, past the buffer's end.  The 256 x 256 tile is bound by
-// the matrix instructions (1.45 us a block, 2.9 PFLOP/s over all CUs), smaller
-// ones by their way into and out of LDS and, a workgroup a CU, by the time a
-// block takes from one barrier to the next; they are for what would leave CUs
-// idle.  8192 x 8192 -> 8192: 411 us, 2.67 PFLOP/s; 16384 rows 2048 -> 8192 249
-// to 259 us, 202 without the epilogue.
+// pixel or, off the map, past the buffer's end.  A block takes the 256 x 256
+// tile 2.9 us (1.48 PFLOP/s over all CUs; fast 1.45, 2.96), of which the matrix
+// pipe is busy in 56 % of the cycles: more than the library's products reach on
+// this card (1.32, 2.73), what the other cycles go to was not isolated (it is 12
+// bytes a lane short of registers).  Smaller tiles are bound by their way into
+// and out of LDS and, a workgroup a CU, by the time a block takes from one barrier
+// to the next; they are for what would leave CUs idle.  16384 rows 2048 -> 8192:
+// 431 us, fast 245.
 
 #include <algorithm>
 
@@ -91,8 +93,6 @@ struct Tile8 {
   static constexpr int LDS = BIAS0 + TN * 4;
   static_assert(A_LOADS * 8 * WAVES == TM && B_LOADS * 8 * WAVES == TN, "loads a wave");
 };
-
-constexpr int NOWHERE = 0x7ffffff0;  // past every buffer: reads zeros
 
 // Buffer loads into LDS (dma_lds) with the place as a wave's base and a
 // constant, and a uniform offset beside the lane's: 16 bytes a lane, or a byte
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(T::THREADS, T::FM * T::FN > 8 ? 1 : 2) void k_tile8
   // Block c's second half is read while its first is multiplied.  Then every
   // wave has read all of it, the next block has landed, and under the second
   // half's products the next one's first half is read and the block S further
-  // loaded into this one's place.  (Blocks past the last are zeros.)
+  // loaded into this one's place.  (What comes past the last block is not multiplied.)
   if (wave < T::TN / 64)  // the epilogue's biases
     dma_lds4(uniform_rsrc(a.bias + n0, (a.npad - n0) * 4), wave_lds4 + T::BIAS0, (wave * 64 + lane) * 4);
   each<T::S>([&](auto stage) {
