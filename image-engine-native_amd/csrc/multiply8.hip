@@ -461,7 +461,9 @@ void run_part(ien_ctx *ctx, Args8 &a, int tile, int ksplit) {
       // among others they lose (3x3 256x384 256 -> 256 97 -> 115, with a residual 102 -> 125).
       (a.exact ? !shared : a.add != nullptr) ? launch<Tile8<1, 2, 4, 2, 2>>(ctx, a) : launch<Tile8<2, 2, 2, 2, 2>>(ctx, a);
       break;
-    case 2:  // (Three workgroups a CU with two stages: 4096 rows 384 -> 1536 12.9 -> 10.5 us; one a CU wants three: 36 blocks deep 16.5, not 23.)
+    case 2:
+      // Three workgroups a CU with two stages, where there are as many: 4096 rows 384 -> 1536 11.0 -> 10.0 us (fast 9.4 ->
+      // 7.9).  One a CU wants three: 3x3 64x64 512 -> 512 with a residual 26.8 -> 25.0 (fast 21.5 -> 17.2).
       shared ? launch<Tile8<1, 2, 2, 2, 2>>(ctx, a) : launch<Tile8<1, 2, 2, 2, 3>>(ctx, a);
       break;
     default: launch<Tile8<1, 1, 2, 2, 4>>(ctx, a); break;
