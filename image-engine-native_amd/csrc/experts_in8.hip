@@ -1,0 +1,81 @@
+// experts_in8.hip -- the experts' first product (ien_experts_in8): the rows of
+// each expert's tokens, gathered by the plan, times its weights, with biases, an
+// activation or a gate, and rounding to 8 bits in the epilogue.  Tiles are
+// ien_multiply8's (tile8.h): a tile is up to 64, 128 or 256 pairs of one expert.
+
+#include "tile8.h"
+
+namespace ien {
+namespace {
+
+template <typename T, Kind8 KIND>
+void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, int size) {
+  a.tiles_n = (int)((a.npad + T::TN - 1) / T::TN);
+  a.list = (const ExpertTile *)(r->d_plan + p.tiles[size]);
+  a.total = r->d_plan + p.totals + size;
+  const dim3 grid((unsigned)(p.most[size] * a.tiles_n));
+  if (a.exact)
+    hipLaunchKernelGGL((k_tile8<T, true, _Float16, KIND>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL((k_tile8<T, false, _Float16, KIND>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+}
+
+}  // namespace
+}  // namespace ien
+
+using namespace ien;
+
+extern "C" ien_status ien_experts_in8(ien_ctx *ctx, const ien_rows8 *x, const ien_routes *routes,
+                                      const ien_experts8 *w, ien_act act, int fast, const ien_rows8 *out) {
+  IEN_CHECK(ctx && w && w->d_w, IEN_ERR_INPUT, "null argument");
+  IEN_CHECK(act8_known(act), IEN_ERR_INPUT, "experts_in8 takes no activation %d", (int)act);
+  ien_status s = check_routes(routes, "experts_in8");
+  if (s != IEN_OK) return s;
+  IEN_CHECK(routes->experts == w->experts, IEN_ERR_INPUT, "routes to %zu experts of %zu", routes->experts, w->experts);
+  if (routes->tokens == 0) return IEN_OK;
+  s = check_rows8(x, w->c, "experts_in8");
+  if (s != IEN_OK) return s;
+  s = check_rows8(out, w->n, "experts_in8");
+  if (s != IEN_OK) return s;
+  IEN_CHECK(x->stride < (1u << 20) && x->scale_stride < (1u << 20) && out->stride < (1u << 20) &&
+                out->scale_stride < (1u << 20) && routes->tokens * std::max(x->stride, x->scale_stride) < 0x7fffff00,
+            IEN_ERR_INPUT, "experts_in8: %zu rows %zu and %zu bytes apart, results %zu and %zu", routes->tokens,
+            x->stride, x->scale_stride, out->stride, out->scale_stride);
+  const PlanLayout p = plan_layout(routes->tokens, routes->experts, routes->top);
+  Args8 a{};
+  a.x = x->data;
+  a.xs = (long)x->stride;
+  a.scales = x->scales;
+  a.ss = (long)x->scale_stride;
+  a.taps = 1;
+  a.step = 1;
+  a.images = a.H = a.OH = 1;
+  a.cb = w->cb;
+  a.w = w->d_w;
+  a.ws = w->d_scales;
+  a.bias = w->d_bias;
+  a.n = (long)w->n;
+  a.npad = w->npad;
+  a.exact = !fast;
+  a.act = act;
+  a.ksplit = 1;
+  a.kchunks = w->cb;
+  a.order = routes->d_plan + p.order;
+  a.top = (int)routes->top;
+  a.q = out->data;
+  a.qstride = (long)out->stride;
+  a.qs = out->scales;
+  a.qsstride = (long)out->scale_stride;
+  const long pairs = (long)(routes->tokens * routes->top), mean = pairs / std::min(pairs, (long)routes->experts);
+  if (w->gated) {
+    if (mean >= 512) launch<Tile8<4, 4, 2, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 3);
+    else if (mean >= 96) launch<Tile8<2, 4, 2, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 2);
+    else launch<Tile8<1, 4, 2, 2, 3>, EXPERTS_GATED8>(ctx, a, routes, p, 1);
+  } else {
+    if (mean >= 512) launch<Tile8<4, 4, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 3);
+    else if (mean >= 96) launch<Tile8<2, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 2);
+    else launch<Tile8<1, 2, 2, 2, 3>, EXPERTS_ACT8>(ctx, a, routes, p, 1);
+  }
+  IEN_HIP(hipGetLastError());
+  return IEN_OK;
+}

@@ -1,0 +1,141 @@
+// experts_out8.hip -- the experts' second product and each token's weighted sum
+// of it (ien_experts_out8): the rows of the plan times their experts' weights in
+// ien_multiply8's tiles (tile8.h), then, a token after another, its pairs' rows
+// by their weights onto the residual.  The sum is a pass of its own, so that it
+// takes the slots in order: what arrives first decides nothing.
+
+#include "tile8.h"
+
+namespace ien {
+namespace {
+
+template <typename T>
+void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, int size) {
+  a.tiles_n = (int)((a.n + T::TN - 1) / T::TN);
+  a.list = (const ExpertTile *)(r->d_plan + p.tiles[size]);
+  a.total = r->d_plan + p.totals + size;
+  const dim3 grid((unsigned)(p.most[size] * a.tiles_n));
+  if (a.f32)
+    hipLaunchKernelGGL((k_tile8<T, true, float, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  else if (a.exact)
+    hipLaunchKernelGGL((k_tile8<T, true, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL((k_tile8<T, false, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+}
+
+struct CombineArgs {
+  const void *parts;
+  long pitch;
+  const int *place;
+  const float *weight;
+  const void *add;
+  long as;
+  void *y;
+  long ys;
+  long tokens, n;
+  int top;
+};
+
+// A lane eight outputs of a token; rows of parts are whole eights.
+template <typename Y>
+__global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
+  const long eights = (a.n + 7) / 8, total = a.tokens * eights;
+  for (long item = (long)blockIdx.x * 256 + threadIdx.x; item < total; item += (long)gridDim.x * 256) {
+    const long t = item / eights, at = (item - t * eights) * 8;
+    const bool whole = at + 8 <= a.n;
+    float v[8] = {};
+    for (int k = 0; k < a.top; k++) {
+      const int place = a.place[t * a.top + k];
+      if (place < 0) continue;
+      const float w = a.weight[t * a.top + k];
+      float part[8];
+      load8<Y, true>((const Y *)a.parts + place * a.pitch, at, 0, part);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = fmaf(w, part[i], v[i]);
+    }
+    if (a.add) {
+      float old[8];
+      if (whole)
+        load8<Y, true>((const Y *)a.add + t * a.as, at, 0, old);
+      else
+        load8<Y, false>((const Y *)a.add + t * a.as, at, a.n, old);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] += old[i];
+    }
+    Y *y = (Y *)a.y + t * a.ys;
+    if (whole)
+      stream8(y + at, v);
+    else
+      store8<Y, false>(y, at, a.n, v);
+  }
+}
+
+}  // namespace
+}  // namespace ien
+
+using namespace ien;
+
+extern "C" {
+
+size_t ien_experts_parts(const ien_routes *routes, const ien_experts8 *w) {
+  if (!w || check_routes(routes, "experts_parts") != IEN_OK) return 0;
+  return routes->tokens * routes->top * ((w->n + 7) / 8 * 8);
+}
+
+ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *routes, const ien_experts8 *w,
+                            int fast, void *d_parts, const void *d_add, size_t add_stride, const ien_output *out) {
+  IEN_CHECK(ctx && w && w->d_w && out, IEN_ERR_INPUT, "null argument");
+  IEN_CHECK(!w->gated, IEN_ERR_INPUT, "experts_out8 takes no gated weights");
+  IEN_CHECK(out->type == IEN_OUT_F16 || out->type == IEN_OUT_F32, IEN_ERR_INPUT, "type %d", (int)out->type);
+  IEN_CHECK(out->layout == IEN_LAYOUT_NHWC, IEN_ERR_INPUT, "experts_out8 writes NHWC rows");
+  ien_status s = check_routes(routes, "experts_out8");
+  if (s != IEN_OK) return s;
+  IEN_CHECK(routes->experts == w->experts, IEN_ERR_INPUT, "routes to %zu experts of %zu", routes->experts, w->experts);
+  if (routes->tokens == 0) return IEN_OK;
+  s = check_rows8(h, w->c, "experts_out8");
+  if (s != IEN_OK) return s;
+  IEN_CHECK(out->data && out->stride >= w->n && (!d_add || add_stride >= w->n), IEN_ERR_INPUT,
+            "no output, or rows %zu and %zu apart for n = %zu", out->stride, add_stride, w->n);
+  IEN_CHECK(d_parts && ((uintptr_t)d_parts & 15) == 0, IEN_ERR_INPUT, "experts_out8: no parts, or unaligned");
+  IEN_CHECK(h->stride < (1u << 20) && h->scale_stride < (1u << 20), IEN_ERR_INPUT,
+            "experts_out8: rows in 8 bits %zu and %zu bytes apart", h->stride, h->scale_stride);
+  const PlanLayout p = plan_layout(routes->tokens, routes->experts, routes->top);
+  Args8 a{};
+  a.x = h->data;
+  a.xs = (long)h->stride;
+  a.scales = h->scales;
+  a.ss = (long)h->scale_stride;
+  a.taps = 1;
+  a.step = 1;
+  a.images = a.H = a.OH = 1;
+  a.cb = w->cb;
+  a.w = w->d_w;
+  a.ws = w->d_scales;
+  a.bias = w->d_bias;
+  a.n = (long)w->n;
+  a.npad = w->npad;
+  a.y = d_parts;
+  a.ys = (long)((w->n + 7) / 8 * 8);
+  a.f32 = out->type == IEN_OUT_F32;
+  a.exact = a.f32 || !fast;
+  a.act = IEN_ACT_NONE;
+  a.ksplit = 1;
+  a.kchunks = w->cb;
+  const long pairs = (long)(routes->tokens * routes->top), mean = pairs / std::min(pairs, (long)routes->experts);
+  if (mean >= 512) launch<Tile8<4, 4, 2, 2, 2>>(ctx, a, routes, p, 3);
+  else if (mean >= 96) launch<Tile8<2, 2, 2, 2, 2>>(ctx, a, routes, p, 2);
+  else launch<Tile8<1, 2, 2, 2, 3>>(ctx, a, routes, p, 1);
+  IEN_HIP(hipGetLastError());
+  CombineArgs c{d_parts, a.ys, routes->d_plan + p.place, routes->d_weight, d_add, (long)add_stride, out->data,
+                (long)out->stride, (long)routes->tokens, a.n, (int)routes->top};
+  const long items = c.tokens * ((c.n + 7) / 8);
+  const dim3 grid((unsigned)std::min((items + 255) / 256, 1L << 20));
+  if (a.f32)
+    hipLaunchKernelGGL(k_combine<float>, grid, dim3(256), 0, ctx->stream, c);
+  else
+    hipLaunchKernelGGL(k_combine<_Float16>, grid, dim3(256), 0, ctx->stream, c);
+  IEN_HIP(hipGetLastError());
+  return IEN_OK;
+}
+
+}  // extern "C"

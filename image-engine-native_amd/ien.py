@@ -23,6 +23,7 @@ NHWC, NCHW = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_PRELU, ACT_SIGMOID, ACT_SILU = range(6)
 OUT_F16, OUT_F32 = 0, 1
 MODEL_REALESRGAN, MODEL_SCUNET, MODEL_LAMA, MODEL_BIREFNET = 0, 1, 2, 3
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 # Every symbol include/ien_hip.h declares.
 EXPORTS = (
@@ -45,6 +46,8 @@ EXPORTS = (
     "ien_spectral_run",
     "ien_rows8_stride", "ien_rows8_scale_stride", "ien_quantize8", "ien_dequantize8", "ien_matrix8_new",
     "ien_matrix8_free", "ien_multiply8", "ien_group_norm", "ien_group_norm8",
+    "ien_rms_norm", "ien_routes_ints", "ien_routes_order", "ien_route", "ien_routes_plan", "ien_experts8_new",
+    "ien_experts8_free", "ien_experts_in8", "ien_experts_parts", "ien_experts_out8",
 )
 
 
@@ -112,6 +115,18 @@ class Input8(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int), ("map", Rows8Struct), ("images", ctypes.c_size_t),
                 ("height", ctypes.c_size_t), ("width", ctypes.c_size_t), ("step", ctypes.c_size_t),
                 ("fast", ctypes.c_int)]
+
+
+class RoutesStruct(ctypes.Structure):
+    """ien_routes."""
+    _fields_ = [("tokens", ctypes.c_size_t), ("experts", ctypes.c_size_t), ("top", ctypes.c_size_t),
+                ("index", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("plan", ctypes.c_void_p)]
+
+
+class Router(ctypes.Structure):
+    """ien_router."""
+    _fields_ = [("score", ctypes.c_int), ("bias", ctypes.c_void_p), ("groups", ctypes.c_size_t), ("kept", ctypes.c_size_t),
+                ("group_top", ctypes.c_size_t), ("renormalise", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
 class Tensor(ctypes.Structure):
@@ -229,6 +244,20 @@ def load():
         L.ien_multiply8.argtypes = [vp, vp, sz, sz, vp, vp, i, vp, sz]
         L.ien_group_norm.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, vp, i, sz]
         L.ien_group_norm8.argtypes = [vp, vp, i, sz, sz, sz, sz, sz, vp, vp, fl, i, vp]
+        L.ien_rms_norm.argtypes = [vp, vp, i, sz, sz, sz, vp, i, sz, vp, sz, vp, fl, vp, i, sz, vp]
+        L.ien_routes_ints.argtypes = [sz, sz, sz]
+        L.ien_routes_ints.restype = sz
+        L.ien_routes_order.argtypes = [sz]
+        L.ien_routes_order.restype = sz
+        L.ien_route.argtypes = [vp, vp, i, sz, vp, vp]
+        L.ien_routes_plan.argtypes = [vp, vp]
+        L.ien_experts8_new.argtypes = [vp, vp, i, sz, sz, sz, i, vp, ctypes.POINTER(vp)]
+        L.ien_experts8_free.argtypes = [vp]
+        L.ien_experts8_free.restype = None
+        L.ien_experts_in8.argtypes = [vp, vp, vp, vp, i, i, vp]
+        L.ien_experts_parts.argtypes = [vp, vp]
+        L.ien_experts_parts.restype = sz
+        L.ien_experts_out8.argtypes = [vp, vp, vp, vp, i, vp, vp, sz, vp]
         for name in EXPORTS:
             getattr(L, name)
         _lib = L
@@ -797,6 +826,199 @@ def group_norm(ctx, x, images, groups, gamma, beta, y, eps=1e-5, act=ACT_NONE):
         status = (_lib or load()).ien_group_norm(
             ctx.h, at, kind, images, rows // images, c, stride, groups, _channels_of(ctx, gamma, c),
             _channels_of(ctx, beta, c), eps, act, y_at, y_kind, y_stride)
+    if status:
+        check(status)
+
+
+def rms_norm(ctx, x, gamma, y=None, rows8=None, add=None, total=None, eps=1e-6):
+    """The sum of the rows x and `add` (rows x channels, f16 or f32 each) into
+    `total` (x's type; x or add itself too), and its root-mean-square norm times
+    gamma (f32 tensor, or None for 1) into y (f16 or f32) and the Rows8 rows8;
+    add, total, y and rows8 may each be None."""
+    rows, c, at, kind, stride = _rows_of(ctx, x)
+    add_at = total_at = y_at = out = None
+    add_kind = y_kind = add_stride = total_stride = y_stride = 0
+    if add is not None:
+        n, k, add_at, add_kind, add_stride = _rows_of(ctx, add)
+        if n != rows or k != c:
+            raise ValueError("what is added has the input's rows and channels")
+    if total is not None:
+        n, k, total_at, total_kind, total_stride = _rows_of(ctx, total)
+        if n != rows or k != c or total_kind != kind:
+            raise ValueError("the sum has the input's rows, channels and type")
+    if y is not None:
+        n, k, y_at, y_kind, y_stride = _rows_of(ctx, y)
+        if n != rows or k != c:
+            raise ValueError("the result has the input's rows and channels")
+    if rows8 is not None:
+        if rows8.rows != rows or rows8.k != c:
+            raise ValueError("the result has the input's rows and channels")
+        if rows8._device != ctx.device:
+            raise _elsewhere(ctx, rows8.data.device)
+        out = rows8._at
+    status = (_lib or load()).ien_rms_norm(ctx.h, at, kind, rows, c, stride, add_at, add_kind, add_stride, total_at,
+                                           total_stride, _channels_of(ctx, gamma, c), eps, y_at, y_kind, y_stride, out)
+    if status:
+        check(status)
+
+
+class Routes:
+    """ien_routes: each token's experts, best first (`index`: int32, tokens x
+    top, -1 for none) and their weights (f32), and the plan that the experts'
+    products go by.  The tensors are made here, or given; the plan is route's or
+    plan_routes' to fill, again whenever the index changes.  `offsets`: the
+    first pair (token x top + slot) of each expert in `order`, which holds the
+    pairs in the order of their experts."""
+
+    def __init__(self, tokens, experts, top, index=None, weight=None, device="cuda"):
+        import torch
+
+        L = load()
+        ints = L.ien_routes_ints(tokens, experts, top)
+        if not ints:
+            raise ValueError(f"{tokens} tokens with {top} of {experts} experts")
+        if index is not None or weight is not None:
+            device = (index if index is not None else weight).device
+        if index is None:
+            index = torch.empty(tokens, top, dtype=torch.int32, device=device)
+        if weight is None:
+            weight = torch.empty(tokens, top, dtype=torch.float32, device=device)
+        for t, dtype in ((index, torch.int32), (weight, torch.float32)):
+            if t.shape != (tokens, top) or t.dtype != dtype or not t.is_contiguous() or t.device != index.device:
+                raise ValueError(f"the experts and weights are contiguous int32 and f32 tensors of {tokens} x {top} on one device")
+        plan = torch.zeros(ints, dtype=torch.int32, device=index.device)  # (zeros: a plan of no pairs)
+        self.tokens, self.experts, self.top = tokens, experts, top
+        self._index, self._weight, self._plan = index, weight, plan
+        first = L.ien_routes_order(experts)
+        self.offsets, self.order = plan[:experts + 1], plan[first:first + tokens * top]
+        self._device = index.get_device()
+        self._struct = RoutesStruct(tokens, experts, top, index.data_ptr(), weight.data_ptr(), plan.data_ptr())
+        self._at = ctypes.addressof(self._struct)
+
+    index = property(lambda self: self._index)
+    weight = property(lambda self: self._weight)
+
+
+def plan_routes(ctx, routes):
+    """The plan of the experts in routes.index (values outside 0 .. experts - 1: none)."""
+    if routes._device != ctx.device:
+        raise _elsewhere(ctx, routes.index.device)
+    check((_lib or load()).ien_routes_plan(ctx.h, routes._at))
+
+
+# ien_router as bytes.
+_ROUTER = struct.Struct("@iPNNNif").pack
+
+
+def route(ctx, logits, routes, score=SCORE_SOFTMAX, bias=None, groups=1, kept=None, group_top=1, renormalise=True, scale=1.0):
+    """Each token's experts and weights from its logits (tokens x experts, f16
+    or f32), and their plan, into `routes`: see ien_router.  kept: all groups by
+    default."""
+    tokens, experts, at, kind, stride = _rows_of(ctx, logits)
+    if tokens != routes.tokens or experts != routes.experts:
+        raise ValueError(f"{tuple(logits.shape)} logits for {routes.tokens} tokens of {routes.experts} experts")
+    if routes._device != ctx.device:
+        raise _elsewhere(ctx, routes.index.device)
+    if groups < 1 or group_top < 1 or (kept is not None and kept < 1):
+        raise ValueError(f"{kept} of {groups} groups by their {group_top} best")
+    how = _ROUTER(score, _channels_of(ctx, bias, experts) or 0, groups, groups if kept is None else kept, group_top,
+                  1 if renormalise else 0, scale)
+    status = (_lib or load()).ien_route(ctx.h, at, kind, stride, how, routes._at)
+    if status:
+        check(status)
+
+
+class Experts8:
+    """ien_experts8: experts x c x n weights (f32 or f16; torch on the context's
+    GPU, or numpy) and experts x n biases in 8 bits.  gated: n / 2 outputs, the
+    activation of the first half of the columns times the second half."""
+
+    def __init__(self, ctx, w, bias=None, gated=False):
+        import torch
+
+        device = torch.device("cuda", ctx.device)
+
+        def held(t, types):
+            t = t if isinstance(t, torch.Tensor) else torch.from_numpy(t)
+            if t.is_cuda and t.get_device() != ctx.device:
+                raise _elsewhere(ctx, t.device)
+            return t.to(device, t.dtype if t.dtype in types else torch.float32).contiguous()
+
+        if len(w.shape) != 3 or (bias is not None and tuple(bias.shape) != (w.shape[0], w.shape[2])):
+            raise ValueError("weights are experts x c x n, biases experts x n")
+        w = held(w, (torch.float16, torch.float32))
+        b = None if bias is None else held(bias, (torch.float32,))
+        torch.cuda.current_stream(device).synchronize()  # (they may have been made on another stream than the context's)
+        experts, c, n = w.shape
+        h = ctypes.c_void_p()
+        check(load().ien_experts8_new(ctx.h, _ptr(w), W_F16 if w.dtype == torch.float16 else W_F32, experts, c, n,
+                                      1 if gated else 0, _ptr(b), ctypes.byref(h)))
+        self.h, self.experts, self.c, self.n, self.gated, self.ctx = h, experts, c, n // 2 if gated else n, gated, ctx
+
+    def free(self):
+        if self.h:
+            load().ien_experts8_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _experts_of(ctx, rows8, rows, routes, matrix):
+    if rows8.k != matrix.c or rows8.rows != rows or routes.experts != matrix.experts:
+        raise ValueError(f"{rows8.rows} rows of {rows8.k} by {matrix.experts} experts of {matrix.c} x {matrix.n}, routes of "
+                         f"{routes.tokens} tokens to {routes.top} of {routes.experts}")
+    if rows8._device != ctx.device:
+        raise _elsewhere(ctx, rows8.data.device)
+    if routes._device != ctx.device:
+        raise _elsewhere(ctx, routes.index.device)
+    if matrix.ctx.device != ctx.device:
+        raise _elsewhere(ctx, f"GPU {matrix.ctx.device}")
+
+
+def experts_in8(ctx, x, routes, matrix, out, act=ACT_NONE, exact=True):
+    """The Rows8 out (tokens x top rows, in the order of routes.order) from the
+    Rows8 x (a row a token): act(x . w + bias) of each pair's expert, of gated
+    weights act(gate) x up.  exact=False: the coarser sums of multiply8."""
+    _experts_of(ctx, x, routes.tokens, routes, matrix)
+    if out.rows != routes.tokens * routes.top or out.k != matrix.n:
+        raise ValueError(f"{routes.tokens} x {routes.top} rows of {matrix.n} into {out.rows} of {out.k}")
+    if out._device != ctx.device:
+        raise _elsewhere(ctx, out.data.device)
+    status = (_lib or load()).ien_experts_in8(ctx.h, x._at, routes._at, matrix.h, act, 0 if exact else 1, out._at)
+    if status:
+        check(status)
+
+
+def expert_parts(routes, matrix, dtype):
+    """What experts_out8 writes its products to, of the result's type."""
+    import torch
+
+    return torch.empty(load().ien_experts_parts(routes._at, matrix.h), dtype=dtype, device=routes.index.device)
+
+
+def experts_out8(ctx, h, routes, matrix, parts, out, add=None, exact=True):
+    """out (tokens x n, f16 or f32) = add + each token's sum of weight x (h . w +
+    bias) over its pairs' rows of the Rows8 h (as experts_in8 leaves them);
+    `add` like out, or out itself; parts: expert_parts(routes, matrix, out's type)."""
+    _experts_of(ctx, h, routes.tokens * routes.top, routes, matrix)
+    rows, n, at, kind, stride = _rows_of(ctx, out)
+    if rows != routes.tokens or n != matrix.n:
+        raise ValueError(f"{routes.tokens} rows of {matrix.n} into {tuple(out.shape)}")
+    if parts.dtype != out.dtype or not parts.is_contiguous() or parts.get_device() != ctx.device \
+            or parts.numel() < rows * routes.top * (-(-n // 8) * 8):
+        raise ValueError("parts are what expert_parts makes for the result's type")
+    add_at = None
+    add_stride = 0
+    if add is not None:
+        add_rows, add_n, add_at, add_kind, add_stride = _rows_of(ctx, add)
+        if add_rows != rows or add_n != n or add_kind != kind:
+            raise ValueError("what is added has the output's shape and type")
+    status = (_lib or load()).ien_experts_out8(ctx.h, h._at, routes._at, matrix.h, 0 if exact else 1, parts.data_ptr(),
+                                               add_at, add_stride, _OUTPUT(at, stride, NHWC, kind))
     if status:
         check(status)
 

@@ -101,7 +101,7 @@ typedef enum {
   IEN_ACT_GELU = 2,
   IEN_ACT_PRELU = 3,
   IEN_ACT_SIGMOID = 4,
-  IEN_ACT_SILU = 5 /* v sigmoid(v): ien_group_norm{,8} and ien_multiply8 only */
+  IEN_ACT_SILU = 5 /* v sigmoid(v): ien_group_norm{,8}, ien_multiply8 and ien_experts_in8 only */
 } ien_act;
 
 /* The left operand of a product (gemm.rs:289-304).  `data` is device f16.
@@ -325,6 +325,101 @@ ien_status ien_group_norm8(ien_ctx *ctx, const void *d_x, ien_out_type type, siz
                            size_t pixels, size_t c, size_t stride, size_t groups,
                            const float *d_gamma, const float *d_beta, float eps, ien_act act,
                            const ien_rows8 *out);
+
+/* ---- root-mean-square norm, routing to experts, their products ----------
+ * No counterpart in the reference: the second half of a transformer block
+ * whose MLP is one of many for each token, x + sum over a token's experts of
+ * weight expert(norm(x)), with the products' operands in 8 bits. */
+
+/* Rows of c values (f16 or f32 by `type`, c at most 8192): the sum s = x +
+ * add in f32 (d_add or NULL; f16 or f32 by add_type), and its norm
+ *   y = s / sqrt(mean(s^2) + eps) gamma[c]
+ * (gamma device f32 or NULL for 1; the mean of squares in f64).  Written are,
+ * where not NULL: the sum to d_sum, rows of `type` sum_stride elements apart;
+ * y to d_y (f16 or f32 by y_type); and y in 8 bits to `out8`, as
+ * ien_quantize8 of the f32 results.  The norm is of the f32 sum, not of what
+ * d_sum holds of it.  d_sum and d_y may each be d_x or d_add itself with its
+ * type and stride. */
+ien_status ien_rms_norm(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t rows, size_t c,
+                        size_t stride, const void *d_add, ien_out_type add_type, size_t add_stride,
+                        void *d_sum, size_t sum_stride, const float *d_gamma, float eps, void *d_y,
+                        ien_out_type y_type, size_t y_stride, const ien_rows8 *out8);
+
+/* The experts of each token, device memory.  A pair is a token and one of its
+ * experts: token x top + slot.  d_index: an expert a pair, or any value that
+ * is none (-1 from ien_route) for a pair without one; d_weight: its weight.
+ * d_plan: ien_routes_ints(tokens, experts, top) ints, 16-byte aligned, which
+ * the calls below share: the first pair of each expert among the pairs in the
+ * order of their experts (experts + 1 ints, the last the number of pairs that
+ * have one), then from int ien_routes_order(experts) on the pairs in that
+ * order (equal experts by pair, pairs without one last), then what only they
+ * read.  Up to 1024 experts, 16 a token, 2^28 pairs. */
+typedef struct {
+  size_t tokens, experts, top;
+  int32_t *d_index;
+  float *d_weight;
+  int32_t *d_plan;
+} ien_routes;
+size_t ien_routes_ints(size_t tokens, size_t experts, size_t top);
+size_t ien_routes_order(size_t experts); /* 4 ceil((experts + 1) / 4) */
+
+/* A router's scores of its logits: their softmax or each one's logistic
+ * function.  Experts are chosen by score + bias (device f32 or NULL): of
+ * `groups` groups of consecutive experts the `kept` ones with the largest sum
+ * of their group_top (1 or 2) largest choices, of those groups' experts the
+ * `top` largest, largest first; equal ones by the lowest index.  Experts
+ * whose logit or bias is NaN or -infinity are never chosen; where fewer than
+ * `top` are left, the pairs past them have expert -1 and weight 0.  Weights
+ * are the scores (without bias), divided by their sum over the token's experts
+ * when `renormalise` (0 where that is 0), times scale.  Choices that f32
+ * cannot tell apart are compared in f64. */
+typedef enum { IEN_SCORE_SOFTMAX = 0, IEN_SCORE_SIGMOID = 1 } ien_score;
+typedef struct {
+  ien_score score;
+  const float *d_bias;
+  size_t groups, kept, group_top;
+  int renormalise;
+  float scale;
+} ien_router;
+/* Logits: routes->tokens rows of routes->experts values (f16 or f32 by
+ * `type`), stride elements apart.  Fills the index, the weights and the plan. */
+ien_status ien_route(ien_ctx *ctx, const void *d_logits, ien_out_type type, size_t stride,
+                     const ien_router *how, const ien_routes *routes);
+/* The plan of an index that the caller made. */
+ien_status ien_routes_plan(ien_ctx *ctx, const ien_routes *routes);
+
+/* The experts' weights in 8 bits: `experts` row-major c x n matrices, one
+ * after the other, and n biases each (or NULL), in DEVICE memory (f32 or f16
+ * weights, f32 biases; read before the call returns).  Quantised once, with a
+ * scale for each 128 channels of an output, as ien_quantize8 does.  gated: n
+ * is even and the outputs are n / 2, act(first half) x second half.
+ * experts ceil(c / 128) under 65536, c and n under 2^22. */
+typedef struct ien_experts8 ien_experts8;
+ien_status ien_experts8_new(ien_ctx *ctx, const void *d_w, ien_wtype wtype, size_t experts, size_t c,
+                            size_t n, int gated, const float *d_bias, ien_experts8 **out);
+void ien_experts8_free(ien_experts8 *m);
+
+/* The experts' first product: for the pair at place p of the plan's order, of
+ * token t and expert e, row p of `out` is act(x[t] . w[e] + bias[e]) (gated:
+ * see above), in 8 bits as ien_quantize8 of the f32 results.  x: tokens rows of
+ * c values, out: tokens x top rows of the outputs; rows of pairs without an
+ * expert are left as they were.  Sums as in ien_multiply8, `fast` too.
+ * x takes less than 2 GiB, its rows and out's are less than 1 MiB apart.
+ * act: NONE, RELU, GELU, SIGMOID or SILU.  out does not overlap x. */
+ien_status ien_experts_in8(ien_ctx *ctx, const ien_rows8 *x, const ien_routes *routes,
+                           const ien_experts8 *w, ien_act act, int fast, const ien_rows8 *out);
+
+/* The second: y[t] = add[t] + the sum over token t's pairs, of expert e and
+ * at place p, of weight x (h[p] . w[e] + bias[e]), slot by slot in f32.  h:
+ * tokens x top rows of c values; out: tokens rows (f16 or f32 NHWC); d_add (or
+ * NULL): rows of out's type, which may be out->data itself with its stride.
+ * w is not gated.  d_parts: ien_experts_parts(routes, w) values of out's type,
+ * 16-byte aligned, the pairs' products (rounded to it: an f16 result wants
+ * products within f16).  `fast` (f16 results): as in ien_multiply8. */
+size_t ien_experts_parts(const ien_routes *routes, const ien_experts8 *w);
+ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *routes,
+                            const ien_experts8 *w, int fast, void *d_parts, const void *d_add,
+                            size_t add_stride, const ien_output *out);
 
 /* ---- resampling and padding ------------------------------------------- */
 
