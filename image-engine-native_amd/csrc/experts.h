@@ -35,15 +35,17 @@ struct ExpertTile {
 
 // Where a plan's parts lie, in ints.
 struct PlanLayout {
-  long offsets, order, place;      // experts + 1; pairs; pairs (a pair's place in the order, -1 for none)
-  long totals, firsts;             // tiles of each size; [size][expert]: the expert's first tile
-  long tiles[TILE_SIZES];          // ExpertTile each
-  long most[TILE_SIZES];           // of them, at most
-  long parts, chunk, chunks;       // [chunk][experts + 1] counts of the pairs' chunks
+  long offsets, order, place;  // experts + 1; pairs; pairs (a pair's place in the order, -1 for none)
+  long totals;                 // tiles of each size
+  long tiles[TILE_SIZES];      // ExpertTile each
+  long most[TILE_SIZES];       // of them, at most
+  long parts, pitch;           // [chunk][pitch] counts of the chunks' pairs by expert, and without one
+  long chunk, chunks;          // tokens
   long ints;
 };
 
-// Pairs are counted in chunks of at least 2048, at most 1024 of them.
+// Tokens are counted in chunks of 64s, at most 256 of them (every workgroup that
+// places a chunk's pairs adds all chunks' counts).
 inline PlanLayout plan_layout(size_t tokens, size_t experts, size_t top) {
   const long pairs = (long)(tokens * top), e = (long)experts;
   auto whole = [](long n) { return (n + 3) / 4 * 4; };
@@ -51,18 +53,17 @@ inline PlanLayout plan_layout(size_t tokens, size_t experts, size_t top) {
   p.order = whole(e + 1);
   p.place = p.order + whole(pairs);
   p.totals = p.place + whole(pairs);
-  p.firsts = p.totals + TILE_SIZES;
-  long at = p.firsts + whole(TILE_SIZES * e);
+  long at = p.totals + TILE_SIZES;
   for (int s = 0; s < TILE_SIZES; s++) {
     p.tiles[s] = at;
     p.most[s] = pairs / TILE_ROWS[s] + std::min(pairs, e);
     at += 4 * p.most[s];
   }
-  p.chunk = std::max(2048L, (pairs + 1023) / 1024);
-  p.chunk = (p.chunk + 255) / 256 * 256;
-  p.chunks = std::max(1L, (pairs + p.chunk - 1) / p.chunk);
+  p.chunk = 64 * std::max(1L, ((long)tokens + 64 * 256 - 1) / (64 * 256));
+  p.chunks = std::max(1L, ((long)tokens + p.chunk - 1) / p.chunk);
   p.parts = at;
-  p.ints = at + whole(p.chunks * (e + 1));
+  p.pitch = whole(e + 1);
+  p.ints = at + p.chunks * p.pitch;
   return p;
 }
 

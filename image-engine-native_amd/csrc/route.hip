@@ -2,16 +2,20 @@
 // tokens and experts in the order of the experts (ien_route, ien_routes_plan).
 //
 // Choosing.  16 lanes hold a token's scores (64 where there are more than 256
-// experts) and find the largest choice among them, top times.  Choices are
-// compared in f64: two that differ by less than a step of f32 are still told
-// apart, and the order of the sums decides nothing.
+// experts), and the largest choice among them is found top times: the largest
+// value, then the lowest index that has it.  Without a bias choices are in the
+// order of the logits, which are compared themselves.  With one they are f32
+// sums that are off by some steps: where two that matter (neighbours among the
+// chosen, the last chosen and the next, the last group kept and the first not)
+// are nearer than that, the token is chosen again in f64.
 //
 // Planning is a counting sort that keeps the order of equal experts and adds
-// nothing atomically across workgroups, so it is the same every time: counts of
-// each chunk of the pairs, the chunks' sums for each expert, then every pair's
-// place, a wave taking its part of the chunk 64 pairs at a time (a pair's rank
-// among them is the number of lanes before it with its expert).  Plans of one
-// chunk take one launch.
+// nothing atomically across workgroups, so it is the same every time.  The
+// workgroups that choose count their chunk's pairs by expert; those that place a
+// chunk's pairs add the counts of all chunks (at most 256, from the caches)
+// themselves and then take the pairs 64 at a time a wave, a pair's rank among them
+// being the number of lanes before it with its expert.  Two launches; up to 64
+// tokens take one.
 
 #include <algorithm>
 
@@ -33,254 +37,150 @@ ien_status check_routes(const ien_routes *r, const char *what) {
 
 namespace {
 
-struct RouteArgs {
-  const void *logits;
-  long stride, tokens;
-  int experts, top;
-  const float *bias;
-  int softmax, groups, kept, group_top, renormalise;
-  float scale;
-  int *index;
-  float *weight;
-};
-
-// (a, i) before (b, j): the larger choice, of equal ones the lower index.
-__device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
-
-// L lanes a token, V experts a lane: expert l + L i.
-template <typename X, int L, int V>
-__global__ __launch_bounds__(256) void k_route(RouteArgs a) {
-  constexpr int TOKENS = 256 / L;
-  extern __shared__ double shared[];  // grouped: [token][experts] choices, then [token][groups] ranks
-  const int lane = threadIdx.x % L, slot = threadIdx.x / L, experts = a.experts;
-  const long first = (long)blockIdx.x * TOKENS, t = min(first + slot, a.tokens - 1);
-  const bool some = first + slot < a.tokens;
-  const double none = -__builtin_inf();
-  double s[V], c[V];
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int e = lane + L * i;
-    s[i] = e < experts ? (double)((const X *)a.logits)[t * a.stride + e] : none;
-    if (!(s[i] > none)) s[i] = none;  // (NaN too)
-    c[i] = s[i];
-  }
-  if (a.softmax) {
-    double m = none;
-#pragma unroll
-    for (int i = 0; i < V; i++) m = fmax(m, s[i]);
-#pragma unroll
-    for (int k = 1; k < L; k *= 2) m = fmax(m, __shfl_xor(m, k));
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-      s[i] = s[i] == m ? 1.0 : exp(s[i] - m);  // (infinite ones share all; closed ones are 0)
-      if (c[i] == none) s[i] = 0.0;
-      sum += s[i];
-    }
-#pragma unroll
-    for (int k = 1; k < L; k *= 2) sum += __shfl_xor(sum, k);
-#pragma unroll
-    for (int i = 0; i < V; i++) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) s[i] = 1.0 / (1.0 + exp(-s[i]));
-  }
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int e = lane + L * i;
-    const float b = a.bias && e < experts ? a.bias[e] : 0.0f;
-    c[i] = c[i] == none || !(b > -__builtin_inff()) ? none : s[i] + (double)b;
-  }
-  if (a.kept < a.groups) {
-    double *choices = shared + slot * experts, *ranks = shared + TOKENS * experts + slot * a.groups;
-    const int per = experts / a.groups;
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      if (lane + L * i < experts) choices[lane + L * i] = c[i];
-    __syncthreads();
-    for (int g = lane; g < a.groups; g += L) {
-      double best = none, next = none;
-      for (int e = g * per; e < (g + 1) * per; e++) {
-        const double v = choices[e];
-        next = fmax(next, fmin(best, v));
-        best = fmax(best, v);
-      }
-      ranks[g] = a.group_top == 2 && next > none ? best + next : best;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-      const int e = lane + L * i;
-      if (e >= experts) continue;
-      const int mine = e / per;
-      const double rank = ranks[mine];
-      int ahead = 0;
-      for (int g = 0; g < a.groups; g++) ahead += before(ranks[g], g, rank, mine);
-      if (ahead >= a.kept) c[i] = none;
-    }
-  }
-  // Slot k's expert and score stay with lane k.
-  int chosen = -1;
-  double score = 0.0, total = 0.0;
-  for (int k = 0; k < a.top; k++) {
-    double best = none, its = 0.0;
-    int at = 1 << 30;
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      if (c[i] > best) best = c[i], at = lane + L * i, its = s[i];
-#pragma unroll
-    for (int m = 1; m < L; m *= 2) {
-      const double other = __shfl_xor(best, m), score_of = __shfl_xor(its, m);
-      const int there = __shfl_xor(at, m);
-      if (before(other, there, best, at)) best = other, at = there, its = score_of;
-    }
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      if (lane + L * i == at) c[i] = none;
-    total += its;
-    if (lane == k && best > none) chosen = at, score = its;
-  }
-  if (some && lane < a.top) {
-    a.index[t * a.top + lane] = chosen;
-    const double w = !a.renormalise ? score : total > 0.0 ? score / total : 0.0;
-    a.weight[t * a.top + lane] = (float)(w * (double)a.scale);
-  }
-}
+// ---- the plan ------------------------------------------------------------------
 
 struct PlanArgs {
   const int *index;
   int *plan;
-  long pairs;
-  int experts;
+  long tokens;
+  int experts, top;
   PlanLayout at;
 };
 
-constexpr int WAVES = 4;
+constexpr int PLACE_WAVES = 8, PLACE_LANES = 64 * PLACE_WAVES;
 
-__device__ __forceinline__ int expert_of(const PlanArgs &a, long pair) {
-  const int e = a.index[pair];
-  return (unsigned)e < (unsigned)a.experts ? e : a.experts;
+// What placing a chunk's pairs keeps in LDS, for n = experts + 1 bins: counts of
+// each wave's pairs, of the chunks before, of all; the offsets; the first tiles of
+// each size; a scan's sums.
+struct PlaceShared {
+  int *bins, *before, *total, *offsets, *firsts, *sums;
+  __device__ PlaceShared(int *p, int n)
+      : bins(p), before(bins + PLACE_WAVES * n), total(before + n), offsets(total + n), firsts(offsets + n),
+        sums(firsts + TILE_SIZES * n) {}
+};
+constexpr size_t place_ints(size_t n) { return (PLACE_WAVES + 3 + TILE_SIZES) * n + PLACE_WAVES * (TILE_SIZES + 1); }
+
+__device__ __forceinline__ int bin_of(int expert, int experts) {
+  return (unsigned)expert < (unsigned)experts ? expert : experts;
 }
 
-// Exclusive sums of n (at most 1025) counts in LDS, in place, by 256 threads;
-// every thread gets the sum of all.
-__device__ int scan_counts(int *v, int n, int *work) {
-  constexpr int EACH = (MAX_EXPERTS + 1 + 255) / 256;
-  int mine[EACH], sum = 0;
+// The offsets and each size's first tiles from the total counts, by the first
+// PLACE_LANES threads; into the plan too where `write`.
+__device__ void lay_out(const PlanArgs &a, const PlaceShared &s, bool write) {
+  constexpr int EACH = ((int)MAX_EXPERTS + 1 + PLACE_LANES - 1) / PLACE_LANES, SUMS = TILE_SIZES + 1;
+  const int n = a.experts + 1, tid = threadIdx.x, lane = tid & 63;
+  int count[EACH], run[SUMS] = {}, own[SUMS];
+  if (tid < PLACE_LANES) {
 #pragma unroll
-  for (int i = 0; i < EACH; i++) {
-    const int at = threadIdx.x * EACH + i;
-    mine[i] = at < n ? v[at] : 0;
-    sum += mine[i];
-  }
-  int before = sum;
+    for (int i = 0; i < EACH; i++) {
+      const int e = tid * EACH + i;
+      count[i] = e < n ? s.total[e] : 0;
+      run[0] += count[i];
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    const int o = __shfl_up(before, m);
-    if ((int)(threadIdx.x & 63) >= m) before += o;
-  }
-  if ((threadIdx.x & 63) == 63) work[threadIdx.x / 64] = before;
-  __syncthreads();
-  int base = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; w++) {
-    if (w < (int)threadIdx.x / 64) base += work[w];
-    all += work[w];
-  }
-  int run = base + before - sum;
-#pragma unroll
-  for (int i = 0; i < EACH; i++) {
-    const int at = threadIdx.x * EACH + i;
-    if (at < n) v[at] = run;
-    run += mine[i];
-  }
-  __syncthreads();
-  return all;
-}
-
-// Offsets, and the tiles of each size, from the counts of experts + 1 bins in LDS
-// (which become the offsets).
-__device__ void lay_out(const PlanArgs &a, int *counts, int *firsts, int *work) {
-  for (int s = 0; s < TILE_SIZES; s++) {
-    for (int e = threadIdx.x; e < a.experts; e += 256) firsts[e] = (counts[e] + TILE_ROWS[s] - 1) / TILE_ROWS[s];
-    __syncthreads();
-    const int all = scan_counts(firsts, a.experts, work);
-    for (int e = threadIdx.x; e < a.experts; e += 256) a.plan[a.at.firsts + (long)s * a.experts + e] = firsts[e];
-    if (threadIdx.x == 0) a.plan[a.at.totals + s] = all;
-    __syncthreads();
-  }
-  scan_counts(counts, a.experts + 1, work);
-  for (int e = threadIdx.x; e <= a.experts; e += 256) a.plan[a.at.offsets + e] = counts[e];
-  __syncthreads();
-}
-
-// Counts of the chunk's pairs by expert, a wave its part: [wave][bin] in LDS.
-__device__ void count_chunk(const PlanArgs &a, int *bins, long begin, long end) {
-  const int n = a.experts + 1, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < WAVES * n; i += 256) bins[i] = 0;
-  __syncthreads();
-  const long part = a.at.chunk / WAVES, from = begin + wave * part, to = min(from + part, end);
-  for (long p = from + lane; p < to; p += 64) atomicAdd(bins + wave * n + expert_of(a, p), 1);
-  __syncthreads();
-}
-
-__global__ __launch_bounds__(256) void k_plan_count(PlanArgs a) {
-  extern __shared__ int lds[];
-  const int n = a.experts + 1;
-  const long begin = (long)blockIdx.x * a.at.chunk;
-  count_chunk(a, lds, begin, min(begin + a.at.chunk, a.pairs));
-  for (int e = threadIdx.x; e < n; e += 256)
-    a.plan[a.at.parts + (long)blockIdx.x * n + e] = lds[e] + lds[n + e] + lds[2 * n + e] + lds[3 * n + e];
-}
-
-// Each chunk's counts become the counts of the chunks before it; then the offsets and tiles.
-__global__ __launch_bounds__(256) void k_plan_sum(PlanArgs a) {
-  extern __shared__ int lds[];
-  const int n = a.experts + 1;
-  for (int e = threadIdx.x; e < n; e += 256) {
-    int *parts = a.plan + a.at.parts + e, run = 0;
-    for (long c = 0; c < a.at.chunks; c++) {
-      const int count = parts[c * n];
-      parts[c * n] = run;
-      run += count;
+      for (int k = 0; k < TILE_SIZES; k++)
+        if (e < a.experts) run[k + 1] += (count[i] + TILE_ROWS[k] - 1) / TILE_ROWS[k];
     }
-    lds[e] = run;
+#pragma unroll
+    for (int k = 0; k < SUMS; k++) {
+      own[k] = run[k];
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const int o = __shfl_up(run[k], m);
+        if (lane >= m) run[k] += o;
+      }
+      if (lane == 63) s.sums[tid / 64 * SUMS + k] = run[k];
+    }
   }
   __syncthreads();
-  lay_out(a, lds, lds + n, lds + 2 * n);
+  if (tid < PLACE_LANES) {
+#pragma unroll
+    for (int k = 0; k < SUMS; k++) {
+      run[k] -= own[k];
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < PLACE_WAVES; w++) {
+        const int sum = s.sums[w * SUMS + k];
+        if (w < tid / 64) run[k] += sum;
+        all += sum;
+      }
+      if (write && k > 0 && tid == 0) a.plan[a.at.totals + k - 1] = all;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const int e = tid * EACH + i;
+      if (e >= n) break;
+      s.offsets[e] = run[0];
+      if (write) a.plan[a.at.offsets + e] = run[0];
+      run[0] += count[i];
+#pragma unroll
+      for (int k = 0; k < TILE_SIZES; k++) {
+        s.firsts[k * n + e] = run[k + 1];
+        run[k + 1] += (count[i] + TILE_ROWS[k] - 1) / TILE_ROWS[k];
+      }
+    }
+  }
+  __syncthreads();
 }
 
-// The places of a chunk's pairs.  ONE: the only chunk, which does the rest too.
-template <bool ONE>
-__global__ __launch_bounds__(256) void k_plan_place(PlanArgs a) {
-  extern __shared__ int lds[];
-  const int n = a.experts + 1, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-  int *bins = lds, *counts = lds + WAVES * n, *firsts = counts + n, *work = firsts + n;
-  const long begin = (long)blockIdx.x * a.at.chunk, end = min(begin + a.at.chunk, a.pairs);
-  count_chunk(a, bins, begin, end);
+// The places of a chunk's pairs, by the first PLACE_WAVES waves, each a part of them
+// (expert(p): pair p's of the chunk).  ONE: the only chunk.
+template <bool ONE, typename F>
+__device__ void place_pairs(const PlanArgs &a, const PlaceShared &s, F expert) {
+  const int n = a.experts + 1, tid = threadIdx.x, wave = tid / 64, lane = tid & 63;
+  const long begin = (long)blockIdx.x * a.at.chunk * a.top;
+  const int pairs = (int)(min((blockIdx.x + 1) * a.at.chunk, a.tokens) * a.top - begin);
+  const int part = (pairs + 64 * PLACE_WAVES - 1) / (64 * PLACE_WAVES) * 64;
+  const int from = min(wave * part, pairs), to = wave < PLACE_WAVES ? min(from + part, pairs) : from;
+  for (int i = tid; i < (PLACE_WAVES + 2) * n; i += blockDim.x) s.bins[i] = 0;  // (before and total too)
+  __syncthreads();
+  for (int p = from + lane; p < to; p += 64) atomicAdd(s.bins + wave * n + expert(p), 1);
+  if constexpr (!ONE) {
+    // Four bins a thread, chunks side by side.
+    const int fours = (int)a.at.pitch / 4, groups = (int)blockDim.x / fours, four = tid % fours, group = tid / fours;
+    int4v before{}, total{};
+    if (group < groups) {
+#pragma unroll 8
+      for (int c = group; c < (int)a.at.chunks; c += groups) {
+        const int4v v = *(const int4v *)(a.plan + a.at.parts + (long)c * a.at.pitch + 4 * four);
+        total += v;
+        if (c < (int)blockIdx.x) before += v;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (4 * four + i < n) {
+          atomicAdd(s.before + 4 * four + i, before[i]);
+          atomicAdd(s.total + 4 * four + i, total[i]);
+        }
+    }
+  }
+  __syncthreads();
   if constexpr (ONE) {
-    for (int e = threadIdx.x; e < n; e += 256) counts[e] = bins[e] + bins[n + e] + bins[2 * n + e] + bins[3 * n + e];
+    for (int e = tid; e < n; e += blockDim.x) {
+      int sum = 0;
+      for (int w = 0; w < PLACE_WAVES; w++) sum += s.bins[w * n + e];
+      s.total[e] = sum;
+    }
     __syncthreads();
-    lay_out(a, counts, firsts, work);
   }
-  // A wave's next place of each expert.
-  for (int e = threadIdx.x; e < n; e += 256) {
-    int run = ONE ? counts[e] : a.plan[a.at.offsets + e] + a.plan[a.at.parts + (long)blockIdx.x * n + e];
-    for (int w = 0; w < WAVES; w++) {
-      const int count = bins[w * n + e];
-      bins[w * n + e] = run;
+  lay_out(a, s, blockIdx.x == 0);
+  // Each wave's next place of each expert.
+  for (int e = tid; e < n; e += blockDim.x) {
+    int run = s.offsets[e] + s.before[e];
+    for (int w = 0; w < PLACE_WAVES; w++) {
+      const int count = s.bins[w * n + e];
+      s.bins[w * n + e] = run;
       run += count;
     }
   }
   __syncthreads();
-  const long part = a.at.chunk / WAVES, from = begin + wave * part, to = min(from + part, end);
-  int *next = bins + wave * n;
-  for (long p0 = from; p0 < to; p0 += 64) {
-    const long p = p0 + lane;
+  int *next = s.bins + wave * n;
+  const int bits = 32 - __clz(a.experts);
+  for (int p0 = from; p0 < to; p0 += 64) {
+    const int p = p0 + lane;
     const bool some = p < to;
-    const int e = some ? expert_of(a, p) : -1;
+    const int e = some ? expert(p) : 0;
     unsigned long long same = __ballot(some);
-    for (int bit = 0; bit < 11; bit++) {
+    for (int bit = 0; bit < bits; bit++) {
       const unsigned long long set = __ballot(e >> bit & 1);
       same &= e >> bit & 1 ? set : ~set;
     }
@@ -290,48 +190,400 @@ __global__ __launch_bounds__(256) void k_plan_place(PlanArgs a) {
     __builtin_amdgcn_wave_barrier();
     if (!some) continue;
     const int at = first + rank;
-    a.plan[a.at.order + at] = (int)p;
-    a.plan[a.at.place + p] = e < a.experts ? at : -1;
+    a.plan[a.at.order + at] = (int)(begin + p);
+    a.plan[a.at.place + begin + p] = e < a.experts ? at : -1;
     if (e == a.experts) continue;
     // A tile begins at every TILE_ROWS-th pair of an expert.
-    const int begins = ONE ? counts[e] : a.plan[a.at.offsets + e], ends = ONE ? counts[e + 1] : a.plan[a.at.offsets + e + 1];
-    for (int s = 0; s < TILE_SIZES; s++) {
-      if ((at - begins) % TILE_ROWS[s] != 0) continue;
-      const int tile = a.plan[a.at.firsts + (long)s * a.experts + e] + (at - begins) / TILE_ROWS[s];
-      *(int4v *)(a.plan + a.at.tiles[s] + 4l * tile) = int4v{e, at, min(at + TILE_ROWS[s], ends), 0};
-    }
+    const int row = at - s.offsets[e];
+#pragma unroll
+    for (int k = 0; k < TILE_SIZES; k++)
+      if (row % TILE_ROWS[k] == 0)
+        *(int4v *)(a.plan + a.at.tiles[k] + 4l * (s.firsts[k * n + e] + row / TILE_ROWS[k])) =
+            int4v{e, at, min(at + TILE_ROWS[k], s.offsets[e + 1]), 0};
   }
 }
 
-ien_status plan(ien_ctx *ctx, const ien_routes *r) {
-  PlanArgs a{r->d_index, r->d_plan, (long)(r->tokens * r->top), (int)r->experts,
-             plan_layout(r->tokens, r->experts, r->top)};
-  const int n = a.experts + 1;
-  const size_t lds = (size_t)((WAVES + 2) * n + WAVES) * 4;
-  const dim3 grid((unsigned)a.at.chunks);
-  if (a.at.chunks == 1) {
-    hipLaunchKernelGGL(k_plan_place<true>, grid, dim3(256), lds, ctx->stream, a);
-  } else {
-    hipLaunchKernelGGL(k_plan_count, grid, dim3(256), lds, ctx->stream, a);
-    hipLaunchKernelGGL(k_plan_sum, dim3(1), dim3(256), lds, ctx->stream, a);
-    hipLaunchKernelGGL(k_plan_place<false>, grid, dim3(256), lds, ctx->stream, a);
+__global__ __launch_bounds__(256) void k_plan_count(PlanArgs a) {
+  __shared__ int bins[MAX_EXPERTS + 4];
+  for (int e = threadIdx.x; e < (int)a.at.pitch; e += 256) bins[e] = 0;
+  __syncthreads();
+  const long begin = (long)blockIdx.x * a.at.chunk * a.top, end = min((blockIdx.x + 1) * a.at.chunk, a.tokens) * a.top;
+  for (long p = begin + threadIdx.x; p < end; p += 256) atomicAdd(bins + bin_of(a.index[p], a.experts), 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < (int)a.at.pitch; e += 256) a.plan[a.at.parts + blockIdx.x * a.at.pitch + e] = bins[e];
+}
+
+template <bool ONE>
+__global__ __launch_bounds__(PLACE_LANES) void k_plan_place(PlanArgs a) {
+  extern __shared__ int lds[];
+  const int *index = a.index + (long)blockIdx.x * a.at.chunk * a.top;
+  place_pairs<ONE>(a, PlaceShared(lds, a.experts + 1), [&](int p) { return bin_of(index[p], a.experts); });
+}
+
+// ---- choosing ------------------------------------------------------------------
+
+struct RouteArgs {
+  const void *logits;
+  long stride;
+  const float *bias;
+  int softmax, groups, kept, group_top, renormalise;
+  int by_logit;      // choices are in the order of the logits
+  unsigned magic;    // e / (experts a group) = e magic >> 22
+  float scale;
+  int *index;
+  float *weight;
+  PlanArgs plan;
+};
+
+constexpr float NONE = -__builtin_inff();
+
+// f(v, v of lane xor 1, 2, 4, ..) over each group of L lanes.
+template <int L, typename F>
+__device__ __forceinline__ void over_lanes(F f) {
+  f([](float v) { return dpp_from<0xB1>(v); });
+  f([](float v) { return dpp_from<0x4E>(v); });
+  f([](float v) { return dpp_from<0x141>(v); });
+  f([](float v) { return dpp_from<0x140>(v); });
+  if constexpr (L == 64) {
+    f([](float v) { return __shfl_xor(v, 16); });
+    f([](float v) { return __shfl_xor(v, 32); });
   }
-  IEN_HIP(hipGetLastError());
-  return IEN_OK;
+}
+template <int L>
+__device__ __forceinline__ float largest(float v) {
+  over_lanes<L>([&](auto other) { v = fmaxf(v, other(v)); });
+  return v;
+}
+template <int L>
+__device__ __forceinline__ int least(int v) {
+  over_lanes<L>([&](auto other) { v = min(v, __float_as_int(other(__int_as_float(v)))); });
+  return v;
+}
+
+// e^x: the hardware's power of two of the rounded x log2(e), times what the rounding left (some 2 steps of f32).
+__device__ __forceinline__ float exp_f(float x) {
+  const float hi = x * 1.44269502f, lo = fmaf(x, 1.44269502f, -hi) + x * 1.92596303e-8f;
+  const float r = __builtin_amdgcn_exp2f(hi);
+  return r > 0.0f ? fmaf(r * lo, 0.693147181f, r) : r;
+}
+
+// How near two choices may come before f32 cannot tell them apart.  A score is off by at
+// most 27 2^-24: the rounding of its argument, which moves it by d e^-d 2^-24 < 2^-25, 3
+// steps of the exponential, 20 of the sum, 2 of the quotient; a choice by half a step of itself more, a
+// group's rank by twice that.  The difference of two is off by twice as much.
+__device__ __forceinline__ float margin(float choice) { return 0x1p-17f + fabsf(choice) * 0x1p-22f; }
+
+__device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
+
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// One token's choice in f64 (by_logit: as it is) and its weights, by its L lanes: lane
+// k's is slot k's expert and weight.
+template <typename X, int L, int V>
+__device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, int lane, double *ranks, int &chosen,
+                                           float &weight) {
+  const int experts = a.plan.experts, top = a.plan.top;
+  const double none = -__builtin_inf();
+  auto logit = [&](int e) {
+    const double v = e < experts ? (double)row[e] : none;
+    return v > none ? v : none;  // (NaN too)
+  };
+  double m = none, sum = 0.0;
+  if (a.softmax) {
+    for (int e = lane; e < experts; e += L) m = fmax(m, logit(e));
+#pragma unroll
+    for (int k = 1; k < L; k *= 2) m = fmax(m, __shfl_xor(m, k));
+  }
+  auto score = [&](double v) {
+    if (v == none) return 0.0;
+    if (!a.softmax) return 1.0 / (1.0 + exp(-v));
+    return v == m ? 1.0 : exp(v - m);  // (infinite ones share all)
+  };
+  double c[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    c[i] = score(logit(lane + L * i));
+    sum += c[i];
+  }
+  if (a.softmax) {
+#pragma unroll
+    for (int k = 1; k < L; k *= 2) sum += __shfl_xor(sum, k);
+  } else {
+    sum = 1.0;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int e = lane + L * i;
+    const float b = a.bias && e < experts ? a.bias[e] : 0.0f;
+    c[i] = logit(e) == none || !(b > NONE) ? none : c[i] / sum + (double)b;
+  }
+  if (a.kept < a.groups) {
+    for (int g = 0; g < a.groups; g++) {
+      double best = none, next = none;
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (((lane + L * i) * a.magic) >> 22 == (unsigned)g) next = fmax(next, fmin(best, c[i])), best = fmax(best, c[i]);
+#pragma unroll
+      for (int k = 1; k < L; k *= 2) {
+        const double b = __shfl_xor(best, k), n = __shfl_xor(next, k);
+        next = fmax(fmax(next, n), fmin(best, b));
+        best = fmax(best, b);
+      }
+      if (lane == 0) ranks[g] = a.group_top == 2 && next > none ? best + next : best;
+    }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      if (lane + L * i >= experts) continue;
+      const int mine = (lane + L * i) * a.magic >> 22;
+      const double rank = ranks[mine];
+      int ahead = 0;
+      for (int g = 0; g < a.groups; g++) ahead += before(ranks[g], g, rank, mine);
+      if (ahead >= a.kept) c[i] = none;
+    }
+    wave_fence();
+  }
+  if (!a.by_logit) chosen = -1;
+  for (int k = 0; k < (a.by_logit ? 0 : top); k++) {
+    double best = none;
+    int at = 1 << 30;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (c[i] > best) best = c[i], at = lane + L * i;
+#pragma unroll
+    for (int n = 1; n < L; n *= 2) {
+      const double other = __shfl_xor(best, n);
+      const int there = __shfl_xor(at, n);
+      if (before(other, there, best, at)) best = other, at = there;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (lane + L * i == at) c[i] = none;
+    if (lane == k && best > none) chosen = at;
+  }
+  const double s = chosen >= 0 ? score(logit(chosen)) / sum : 0.0;
+  double total = s;
+#pragma unroll
+  for (int k = 1; k < L; k *= 2) total += __shfl_xor(total, k);
+  const double w = !a.renormalise ? s : total > 0.0 ? s / total : 0.0;
+  weight = (float)(w * (double)a.scale);
+}
+
+constexpr int route_lanes(int l) { return l == 16 ? 1024 : 512; }  // of a workgroup (64 lanes a token: f64 ranks of all groups fit)
+
+// L lanes a token, V experts a lane: expert l + L i.  A workgroup takes a chunk of
+// tokens, so many at a time.  ONE: the only chunk, whose pairs it places too.
+template <typename X, int L, int V, bool ONE>
+__global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
+  constexpr int LANES = route_lanes(L), TOKENS = LANES / L;
+  extern __shared__ int lds[];
+  const int experts = a.plan.experts, top = a.plan.top, n = experts + 1;
+  const int lane = threadIdx.x % L, slot = threadIdx.x / L;
+  int *bins = lds;                                      // the chunk's counts; ONE: its pairs' experts
+  const int held = ONE ? 64 * top : (int)a.plan.at.pitch;
+  float *ranks = (float *)(lds + (held + 3) / 4 * 4);  // [token][groups]; f64 of one token a wave
+  if constexpr (!ONE) {
+    for (int e = threadIdx.x; e < held; e += LANES) bins[e] = 0;
+    __syncthreads();
+  }
+  float b[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    b[i] = a.bias && lane + L * i < experts ? a.bias[lane + L * i] : 0.0f;
+    if (!(b[i] > NONE)) b[i] = NONE;
+  }
+  const long begin = (long)blockIdx.x * a.plan.at.chunk, end = min(begin + a.plan.at.chunk, a.plan.tokens);
+  for (long t0 = begin; t0 < end; t0 += TOKENS) {
+    const long t = min(t0 + slot, end - 1);
+    const bool some = t0 + slot < end;
+    const X *row = (const X *)a.logits + t * a.stride;
+    float s[V], c[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int e = lane + L * i;
+      const float v = e < experts ? (float)row[e] : NONE;
+      c[i] = v > NONE ? v : NONE;  // (NaN too)
+    }
+    float sum = 1.0f;
+    if (a.softmax) {
+      float m = NONE;
+#pragma unroll
+      for (int i = 0; i < V; i++) m = fmaxf(m, c[i]);
+      m = largest<L>(m);
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        s[i] = c[i] == NONE ? 0.0f : c[i] == m ? 1.0f : exp_f(c[i] - m);  // (infinite ones share all)
+        sum += s[i];
+      }
+      sum = group_sum<L>(sum);
+      const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; i++) s[i] *= inv;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float e = exp_f(-fabsf(c[i]));
+        s[i] = (c[i] < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
+      }
+    }
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < V; i++) c[i] = c[i] == NONE || b[i] == NONE ? NONE : s[i] + b[i];
+    } else if (!a.by_logit) {
+#pragma unroll
+      for (int i = 0; i < V; i++) c[i] = c[i] == NONE ? NONE : s[i];
+    }
+    bool unclear = false;
+    if (a.kept < a.groups) {
+      float *mine = ranks + (L == 16 ? 1 : 2) * slot * a.groups;
+      const int per = experts / a.groups;
+      auto rank_of = [&](int g, float best, float next) {
+        over_lanes<L>([&](auto other) {
+          const float b2 = other(best), n2 = other(next);
+          next = fmaxf(fmaxf(next, n2), fminf(best, b2));
+          best = fmaxf(best, b2);
+        });
+        if (lane == 0) mine[g] = a.group_top == 2 && next > NONE ? best + next : best;
+      };
+      if (per % L == 0) {  // a group is some of every lane's experts, one after another
+        float best = NONE, next = NONE;
+        int g = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          next = fmaxf(next, fminf(best, c[i]));
+          best = fmaxf(best, c[i]);
+          if ((i + 1) * L == (g + 1) * per) {
+            rank_of(g++, best, next);
+            best = next = NONE;
+          }
+        }
+      } else {
+        for (int g = 0; g < a.groups; g++) {
+          float best = NONE, next = NONE;
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            const float v = (lane + L * i) * a.magic >> 22 == (unsigned)g ? c[i] : NONE;
+            next = fmaxf(next, fminf(best, v));
+            best = fmaxf(best, v);
+          }
+          rank_of(g, best, next);
+        }
+      }
+      wave_fence();
+      // The groups kept, and how near the last of them and the first of the others are.
+      unsigned long long keep = 0;  // of this lane's groups lane + L j
+      float low = __builtin_inff(), high = NONE;
+      for (int j = 0; lane + L * j < a.groups; j++) {
+        const float rank = mine[lane + L * j];
+        int ahead = 0;
+        for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
+        if (ahead < a.kept)
+          keep |= 1ull << j, low = fminf(low, rank);
+        else
+          high = fmaxf(high, rank);
+      }
+      over_lanes<L>([&](auto other) { low = fminf(low, other(low)), high = fmaxf(high, other(high)); });
+      unclear = !a.by_logit && high > NONE && low - high < margin(low);
+      wave_fence();
+      for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = keep >> j & 1 ? 1.0f : 0.0f;
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (lane + L * i < experts && mine[(lane + L * i) * a.magic >> 22] == 0.0f) c[i] = NONE;
+      wave_fence();
+    }
+    // Slot k's expert and score stay with lane k.
+    int chosen = -1;
+    bool any = false;
+    float score = 0.0f, total = 0.0f, last = __builtin_inff();
+    for (int k = 0; k <= top; k++) {
+      float best = NONE;
+#pragma unroll
+      for (int i = 0; i < V; i++) best = fmaxf(best, c[i]);
+      best = largest<L>(best);
+      if (best > NONE && last - best < margin(best)) unclear = true;
+      last = best;
+      any = any || best > NONE;
+      if (k == top) break;
+      int at = 1 << 30;
+      float its = 0.0f;
+#pragma unroll
+      for (int i = V - 1; i >= 0; i--)
+        if (c[i] == best) at = lane + L * i, its = s[i];
+      const int first = least<L>(at);
+      const bool owner = first == at;
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (first == lane + L * i) c[i] = NONE;
+      its = group_sum<L>(owner && best > NONE ? its : 0.0f);
+      total += its;
+      if (lane == k && best > NONE) chosen = first, score = its;
+    }
+    float weight = (!a.renormalise ? score : total > 0.0f ? score / total : 0.0f) * a.scale;
+    // (f32 scores that vanish: their shares need not.)
+    unclear = (unclear && !a.by_logit) || (a.renormalise && total < 1e-30f && any);
+    if (__ballot(unclear)) {
+      for (int k = 0; k < 64 / L; k++)
+        if (unclear && slot % (64 / L) == k)
+          choose_f64<X, L, V>(a, row, lane, (double *)(ranks + (L == 16 ? slot / 4 * 4 : 2 * slot) * a.groups), chosen, weight);
+    }
+    if (some && lane < top) {
+      const long pair = t * top + lane;
+      a.index[pair] = chosen;
+      a.weight[pair] = weight;
+      if constexpr (ONE)
+        bins[pair] = bin_of(chosen, experts);
+      else
+        atomicAdd(bins + bin_of(chosen, experts), 1);
+    }
+    wave_fence();  // (the ranks' next token)
+  }
+  __syncthreads();
+  if constexpr (ONE)
+    place_pairs<true>(a.plan, PlaceShared(lds + (held + 3) / 4 * 4, n), [&](int p) { return bins[p]; });
+  else
+    for (int e = threadIdx.x; e < held; e += LANES) a.plan.plan[a.plan.at.parts + blockIdx.x * a.plan.at.pitch + e] = bins[e];
+}
+
+void launch_place(ien_ctx *ctx, const PlanArgs &a) {
+  const size_t lds = place_ints((size_t)a.experts + 1) * 4;
+  if (a.at.chunks == 1)
+    hipLaunchKernelGGL(k_plan_place<true>, dim3(1), dim3(PLACE_LANES), lds, ctx->stream, a);
+  else
+    hipLaunchKernelGGL(k_plan_place<false>, dim3((unsigned)a.at.chunks), dim3(PLACE_LANES), lds, ctx->stream, a);
+}
+
+template <typename X, int L, int V>
+void launch_route(ien_ctx *ctx, const RouteArgs &a) {
+  const PlanArgs &p = a.plan;
+  const bool one = p.at.chunks == 1;
+  const size_t held = one ? 64 * (size_t)p.top : (size_t)p.at.pitch;
+  size_t ints = a.kept < a.groups ? (size_t)(route_lanes(L) / L) * a.groups * (L == 16 ? 1 : 2) : 0;
+  if (one) ints = std::max(ints, place_ints((size_t)p.experts + 1));
+  const size_t lds = ((held + 3) / 4 * 4 + ints) * 4;
+  if (one)
+    hipLaunchKernelGGL((k_route<X, L, V, true>), dim3(1), dim3(route_lanes(L)), lds, ctx->stream, a);
+  else
+    hipLaunchKernelGGL((k_route<X, L, V, false>), dim3((unsigned)p.at.chunks), dim3(route_lanes(L)), lds, ctx->stream, a);
 }
 
 template <typename X>
 void route(ien_ctx *ctx, const RouteArgs &a) {
-  auto go = [&](auto kernel, int lanes) {
-    const int tokens = 256 / lanes;
-    const size_t lds = a.kept < a.groups ? (size_t)tokens * (a.experts + a.groups) * sizeof(double) : 0;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.tokens + tokens - 1) / tokens)), dim3(256), lds, ctx->stream, a);
-  };
-  if (a.experts <= 16) go(k_route<X, 16, 1>, 16);
-  else if (a.experts <= 64) go(k_route<X, 16, 4>, 16);
-  else if (a.experts <= 128) go(k_route<X, 16, 8>, 16);
-  else if (a.experts <= 256) go(k_route<X, 16, 16>, 16);
-  else go(k_route<X, 64, 16>, 64);
+  const int experts = a.plan.experts;
+  if (experts <= 16) launch_route<X, 16, 1>(ctx, a);
+  else if (experts <= 64) launch_route<X, 16, 4>(ctx, a);
+  else if (experts <= 128) launch_route<X, 16, 8>(ctx, a);
+  else if (experts <= 256) launch_route<X, 16, 16>(ctx, a);
+  else launch_route<X, 64, 16>(ctx, a);
+}
+
+PlanArgs plan_args(const ien_routes *r) {
+  return {r->d_index, r->d_plan, (long)r->tokens, (int)r->experts, (int)r->top,
+          plan_layout(r->tokens, r->experts, r->top)};
 }
 
 }  // namespace
@@ -352,7 +604,14 @@ ien_status ien_routes_plan(ien_ctx *ctx, const ien_routes *routes) {
   IEN_CHECK(ctx, IEN_ERR_INPUT, "no context");
   const ien_status s = check_routes(routes, "routes_plan");
   if (s != IEN_OK || routes->tokens == 0) return s;
-  return plan(ctx, routes);
+  const PlanArgs a = plan_args(routes);
+  if (a.at.chunks > 1) {
+    hipLaunchKernelGGL(k_plan_count, dim3((unsigned)a.at.chunks), dim3(256), 0, ctx->stream, a);
+    IEN_HIP(hipGetLastError());
+  }
+  launch_place(ctx, a);
+  IEN_HIP(hipGetLastError());
+  return IEN_OK;
 }
 
 ien_status ien_route(ien_ctx *ctx, const void *d_logits, ien_out_type type, size_t stride, const ien_router *how,
@@ -370,15 +629,20 @@ ien_status ien_route(ien_ctx *ctx, const void *d_logits, ien_out_type type, size
   if (routes->tokens == 0) return IEN_OK;
   IEN_CHECK(d_logits && stride >= routes->experts, IEN_ERR_INPUT, "no logits, or %zu apart for %zu experts", stride,
             routes->experts);
-  RouteArgs a{d_logits, (long)stride, (long)routes->tokens, (int)routes->experts, (int)routes->top, how->d_bias,
-              how->score == IEN_SCORE_SOFTMAX, (int)how->groups, (int)how->kept, (int)how->group_top,
-              how->renormalise, how->scale, routes->d_index, routes->d_weight};
+  const unsigned per = (unsigned)(routes->experts / how->groups);
+  const bool grouped = how->kept < how->groups;
+  // (e magic is e / per + e (magic - 2^22 / per) / 2^22, and e per < 2^22: the second part is under 1 / per.)
+  RouteArgs a{d_logits, (long)stride, how->d_bias, how->score == IEN_SCORE_SOFTMAX, (int)how->groups, (int)how->kept,
+              (int)how->group_top, how->renormalise, !how->d_bias && !(grouped && how->group_top == 2),
+              ((1u << 22) + per - 1) / per, how->scale, routes->d_index, routes->d_weight, plan_args(routes)};
   if (type == IEN_OUT_F16)
     route<_Float16>(ctx, a);
   else
     route<float>(ctx, a);
   IEN_HIP(hipGetLastError());
-  return plan(ctx, routes);
+  if (a.plan.at.chunks > 1) launch_place(ctx, a.plan);
+  IEN_HIP(hipGetLastError());
+  return IEN_OK;
 }
 
 }  // extern "C"

@@ -371,8 +371,9 @@ size_t ien_routes_order(size_t experts); /* 4 ceil((experts + 1) / 4) */
  * whose logit or bias is NaN or -infinity are never chosen; where fewer than
  * `top` are left, the pairs past them have expert -1 and weight 0.  Weights
  * are the scores (without bias), divided by their sum over the token's experts
- * when `renormalise` (0 where that is 0), times scale.  Choices that f32
- * cannot tell apart are compared in f64. */
+ * when `renormalise` (0 where that is 0), times scale.  Without a bias, and
+ * groups by one choice, choices are in the order of the logits; others that
+ * f32 cannot tell apart are compared in f64. */
 typedef enum { IEN_SCORE_SOFTMAX = 0, IEN_SCORE_SIGMOID = 1 } ien_score;
 typedef struct {
   ien_score score;
