@@ -67,6 +67,10 @@ inline PlanLayout plan_layout(size_t tokens, size_t experts, size_t top) {
   return p;
 }
 
+// experts_in8.hip, experts_out8.hip: the tile of a product.
+int experts_in_choice(int cus, long pairs, long experts, long npad, int chunks, int gated);
+int experts_out_choice(long pairs, long experts, int chunks);
+
 // The routes that an entry point was handed, or its refusal.
 ien_status check_routes(const ien_routes *r, const char *what);
 

@@ -3,7 +3,10 @@
 // activation or a gate, and rounding to 8 bits in the epilogue.  Tiles are
 // ien_multiply8's (tile8.h): a tile is up to 64, 128 or 256 pairs of one expert.
 
-#include "tile8.h"
+#include <algorithm>
+#include <cmath>
+
+#include "few8.h"
 
 namespace ien {
 namespace {
@@ -21,6 +24,33 @@ void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, in
 }
 
 }  // namespace
+
+// The size of tile (TILE_ROWS) for that many pairs, columns in whole 128s and blocks
+// of depth.  Where an expert has few rows its weights are what is read, and waves that
+// read them straight into registers beat a tile's stages: gated, four rows an expert
+// 26.8 us against 28.3, eight 34.1 against 29.4 (1024 -> 2 x 1024, 64 experts); plain,
+// one row 8.0 against 9.4, two 16.3 against 14.9.
+// Plain tiles: two workgroups a CU of 128 x 128 outputs or three of 64 x 128, which
+// take 1.1 times as long a row but leave fewer idle (us, rows an expert 128: 40.2 and
+// 31.8, 512: 26.3 and 25.2, 1024: 42.0 and 43.4, 2048: 333 and 365).
+// Gated ones are 256 columns wide, a workgroup a CU: by the rounds of workgroups and
+// what a round was measured at, a block and at its end.
+int experts_in_choice(int cus, long pairs, long experts, long npad, int chunks, int gated) {
+  const long active = std::min(pairs, experts), mean = pairs / active;
+  if (mean <= (gated ? 4 : 1)) return 0;
+  if (!gated) return mean >= 640 ? 2 : 1;
+  constexpr double BLOCK_US[] = {0.85, 1.65, 2.95}, END_US[] = {4.5, 4.3, 6.3};
+  int best = 1;
+  double best_us = 1e30;
+  for (int size = 1; size < TILE_SIZES; size++) {
+    // An expert's last tile is part of one: 0.6 of a tile more for each, as loads differ.
+    const double tiles = ((double)pairs / TILE_ROWS[size] + 0.6 * (double)active) * (double)((npad + 255) / 256);
+    const double us = std::ceil(tiles / cus) * (BLOCK_US[size - 1] * chunks + END_US[size - 1]);
+    if (us < best_us) best_us = us, best = size;
+  }
+  return best;
+}
+
 }  // namespace ien
 
 using namespace ien;
@@ -66,15 +96,21 @@ extern "C" ien_status ien_experts_in8(ien_ctx *ctx, const ien_rows8 *x, const ie
   a.qstride = (long)out->stride;
   a.qs = out->scales;
   a.qsstride = (long)out->scale_stride;
-  const long pairs = (long)(routes->tokens * routes->top), mean = pairs / std::min(pairs, (long)routes->experts);
-  if (w->gated) {
-    if (mean >= 512) launch<Tile8<4, 4, 2, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 3);
-    else if (mean >= 96) launch<Tile8<2, 4, 2, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 2);
-    else launch<Tile8<1, 4, 2, 2, 3>, EXPERTS_GATED8>(ctx, a, routes, p, 1);
-  } else {
-    if (mean >= 512) launch<Tile8<4, 4, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 3);
-    else if (mean >= 96) launch<Tile8<2, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 2);
-    else launch<Tile8<1, 2, 2, 2, 3>, EXPERTS_ACT8>(ctx, a, routes, p, 1);
+  const long pairs = (long)(routes->tokens * routes->top);
+  switch (experts_in_choice(ctx->cus, pairs, (long)routes->experts, a.npad, a.cb, w->gated)) {
+    case 0:
+      w->gated ? launch_few<EXPERTS_GATED8, float, 8, 1>(ctx, a, routes, p)
+               : launch_few<EXPERTS_ACT8, float, 8, 1>(ctx, a, routes, p);
+      break;
+    case 1:
+      w->gated ? launch<Tile8<1, 4, 2, 2, 3>, EXPERTS_GATED8>(ctx, a, routes, p, 1)
+               : launch<Tile8<1, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 1);
+      break;
+    case 2:
+      w->gated ? launch<Tile8<1, 4, 4, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 2)
+               : launch<Tile8<2, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 2);
+      break;
+    default: launch<Tile8<2, 4, 4, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 3); break;
   }
   IEN_HIP(hipGetLastError());
   return IEN_OK;

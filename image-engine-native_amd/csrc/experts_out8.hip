@@ -4,7 +4,9 @@
 // by their weights onto the residual.  The sum is a pass of its own, so that it
 // takes the slots in order: what arrives first decides nothing.
 
-#include "tile8.h"
+#include <algorithm>
+
+#include "few8.h"
 
 namespace ien {
 namespace {
@@ -21,6 +23,14 @@ void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, in
     hipLaunchKernelGGL((k_tile8<T, true, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
   else
     hipLaunchKernelGGL((k_tile8<T, false, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+}
+
+template <int WN, int WK>
+void few(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p) {
+  if (a.f32)
+    launch_few<EXPERTS_ROWS8, float, WN, WK>(ctx, a, r, p);
+  else
+    launch_few<EXPERTS_ROWS8, _Float16, WN, WK>(ctx, a, r, p);
 }
 
 struct CombineArgs {
@@ -71,6 +81,20 @@ __global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
 }
 
 }  // namespace
+
+// The size of tile (TILE_ROWS), 0 and 3 for few rows an expert: waves that read the
+// weights straight into registers, two shares of the depth beside each other, or four
+// where a share then has four blocks at least (us, with the sum's pass; 2048 -> 1024: one
+// row of 8 experts 9.4, two shares 11.6, tiles of 64 rows 18.1; 1024 -> 1024: two rows of 56
+// experts 15.9, four shares 23.8, tiles 18.2; four rows 19.4 and 19.0).  Else two
+// workgroups a CU of 128 x 128 outputs or three of 64 x 128 (rows an expert 128: 39.5 and
+// 35.1, 512: 21.3 and 21.3, 1024: 34.9 and 41.8, 2048: 287 and 316).
+int experts_out_choice(long pairs, long experts, int chunks) {
+  const long mean = pairs / std::min(pairs, experts);
+  if (mean < 3) return chunks >= 16 ? 3 : 0;
+  return mean >= 400 ? 2 : 1;
+}
+
 }  // namespace ien
 
 using namespace ien;
@@ -121,10 +145,13 @@ ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *
   a.act = IEN_ACT_NONE;
   a.ksplit = 1;
   a.kchunks = w->cb;
-  const long pairs = (long)(routes->tokens * routes->top), mean = pairs / std::min(pairs, (long)routes->experts);
-  if (mean >= 512) launch<Tile8<4, 4, 2, 2, 2>>(ctx, a, routes, p, 3);
-  else if (mean >= 96) launch<Tile8<2, 2, 2, 2, 2>>(ctx, a, routes, p, 2);
-  else launch<Tile8<1, 2, 2, 2, 3>>(ctx, a, routes, p, 1);
+  const long pairs = (long)(routes->tokens * routes->top);
+  switch (experts_out_choice(pairs, (long)routes->experts, a.cb)) {
+    case 0: few<4, 2>(ctx, a, routes, p); break;
+    case 1: launch<Tile8<1, 2, 2, 2, 2>>(ctx, a, routes, p, 1); break;
+    case 2: launch<Tile8<2, 2, 2, 2, 2>>(ctx, a, routes, p, 2); break;
+    default: few<2, 4>(ctx, a, routes, p); break;
+  }
   IEN_HIP(hipGetLastError());
   CombineArgs c{d_parts, a.ys, routes->d_plan + p.place, routes->d_weight, d_add, (long)add_stride, out->data,
                 (long)out->stride, (long)routes->tokens, a.n, (int)routes->top};

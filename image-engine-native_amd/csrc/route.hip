@@ -267,12 +267,6 @@ __device__ __forceinline__ float exp_f(float x) {
   return r > 0.0f ? fmaf(r * lo, 0.693147181f, r) : r;
 }
 
-// How near two choices may come before f32 cannot tell them apart.  A score is off by at
-// most 27 2^-24: the rounding of its argument, which moves it by d e^-d 2^-24 < 2^-25, 3
-// steps of the exponential, 20 of the sum, 2 of the quotient; a choice by half a step of itself more, a
-// group's rank by twice that.  The difference of two is off by twice as much.
-__device__ __forceinline__ float margin(float choice) { return 0x1p-17f + fabsf(choice) * 0x1p-22f; }
-
 __device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
 
 __device__ __forceinline__ void wave_fence() {
@@ -280,11 +274,12 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// One token's choice in f64 (by_logit: as it is) and its weights, by its L lanes: lane
-// k's is slot k's expert and weight.
-template <typename X, int L, int V>
-__device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, int lane, double *ranks, int &chosen,
-                                           float &weight) {
+// One token's choice in f64 (by_logit: as it is, in `chosen`) and its weights, by a
+// whole wave, V experts a lane: lane k's is slot k's expert and weight.
+template <typename X, int V>
+__device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, double *ranks, int &chosen, float &weight) {
+  constexpr int L = 64;
+  const int lane = threadIdx.x & 63;
   const int experts = a.plan.experts, top = a.plan.top;
   const double none = -__builtin_inf();
   auto logit = [&](int e) {
@@ -364,7 +359,7 @@ __device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, int
       if (lane + L * i == at) c[i] = none;
     if (lane == k && best > none) chosen = at;
   }
-  const double s = chosen >= 0 ? score(logit(chosen)) / sum : 0.0;
+  const double s = lane < top && chosen >= 0 ? score(logit(chosen)) / sum : 0.0;
   double total = s;
 #pragma unroll
   for (int k = 1; k < L; k *= 2) total += __shfl_xor(total, k);
@@ -389,12 +384,14 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     for (int e = threadIdx.x; e < held; e += LANES) bins[e] = 0;
     __syncthreads();
   }
-  float b[V];
+  float b[V], choice_size = 1.0f;  // (no choice is larger)
 #pragma unroll
   for (int i = 0; i < V; i++) {
     b[i] = a.bias && lane + L * i < experts ? a.bias[lane + L * i] : 0.0f;
     if (!(b[i] > NONE)) b[i] = NONE;
+    if (fabsf(b[i]) < __builtin_inff()) choice_size = fmaxf(choice_size, 1.0f + fabsf(b[i]));
   }
+  choice_size = largest<L>(choice_size);
   const long begin = (long)blockIdx.x * a.plan.at.chunk, end = min(begin + a.plan.at.chunk, a.plan.tokens);
   for (long t0 = begin; t0 < end; t0 += TOKENS) {
     const long t = min(t0 + slot, end - 1);
@@ -407,13 +404,16 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       const float v = e < experts ? (float)row[e] : NONE;
       c[i] = v > NONE ? v : NONE;  // (NaN too)
     }
-    float sum = 1.0f;
+    // How far a score may be off, in halves of a step of 1: of a logistic function 4 of its exponential, at most
+    // a quarter of which reaches it, a step of the reciprocal and two roundings; of a softmax 0.4 of the argument
+    // (d e^-d of its rounding), and of the largest score 4 of the exponential, as much of the sum's, 7 of their
+    // arguments, 21 of the additions and 2 of the quotient.
+    float off = 5.0f;
     if (a.softmax) {
-      float m = NONE;
+      float m = NONE, sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; i++) m = fmaxf(m, c[i]);
       m = largest<L>(m);
-      sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; i++) {
         s[i] = c[i] == NONE ? 0.0f : c[i] == m ? 1.0f : exp_f(c[i] - m);  // (infinite ones share all)
@@ -421,6 +421,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       }
       sum = group_sum<L>(sum);
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+      off = 0.4f + 38.0f * inv;
 #pragma unroll
       for (int i = 0; i < V; i++) s[i] *= inv;
     } else {
@@ -437,6 +438,9 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
 #pragma unroll
       for (int i = 0; i < V; i++) c[i] = c[i] == NONE ? NONE : s[i];
     }
+    // Two choices that are nearer than this may be in the other order (each is off by its score's error and its own
+    // rounding), and two ranks that are nearer than twice this and their own roundings.
+    const float near = 0x1p-23f * (off + choice_size), near_ranks = 2.0f * near + 0x1p-22f * choice_size;
     bool unclear = false;
     if (a.kept < a.groups) {
       float *mine = ranks + (L == 16 ? 1 : 2) * slot * a.groups;
@@ -487,7 +491,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
           high = fmaxf(high, rank);
       }
       over_lanes<L>([&](auto other) { low = fminf(low, other(low)), high = fmaxf(high, other(high)); });
-      unclear = !a.by_logit && high > NONE && low - high < margin(low);
+      unclear = high > NONE && low - high < near_ranks;
       wave_fence();
       for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = keep >> j & 1 ? 1.0f : 0.0f;
       wave_fence();
@@ -505,7 +509,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
 #pragma unroll
       for (int i = 0; i < V; i++) best = fmaxf(best, c[i]);
       best = largest<L>(best);
-      if (best > NONE && last - best < margin(best)) unclear = true;
+      if (best > NONE && last - best < near) unclear = true;
       last = best;
       any = any || best > NONE;
       if (k == top) break;
@@ -526,10 +530,17 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     float weight = (!a.renormalise ? score : total > 0.0f ? score / total : 0.0f) * a.scale;
     // (f32 scores that vanish: their shares need not.)
     unclear = (unclear && !a.by_logit) || (a.renormalise && total < 1e-30f && any);
-    if (__ballot(unclear)) {
-      for (int k = 0; k < 64 / L; k++)
-        if (unclear && slot % (64 / L) == k)
-          choose_f64<X, L, V>(a, row, lane, (double *)(ranks + (L == 16 ? slot / 4 * 4 : 2 * slot) * a.groups), chosen, weight);
+    for (unsigned long long left = __ballot(unclear); left != 0;) {
+      const int first = __ffsll(left) - 1, token = first / L;  // (the wave's)
+      left &= ~((L == 64 ? ~0ull : (1ull << (L & 63)) - 1) << token * L);
+      const long there = __shfl(t, first);
+      int c64 = __shfl(chosen, token * L + lane);
+      float w64;
+      choose_f64<X, (L * V + 63) / 64>(a, (const X *)a.logits + there * a.stride,
+                                       (double *)(ranks + (L == 16 ? slot / 4 * 4 : 2 * slot) * a.groups), c64, w64);
+      c64 = __shfl(c64, lane);
+      w64 = __shfl(w64, lane);
+      if (slot % (64 / L) == token) chosen = c64, weight = w64;
     }
     if (some && lane < top) {
       const long pair = t * top + lane;

@@ -128,6 +128,7 @@ __device__ __forceinline__ void into_rows8(const Args8 &a, floatx16 (&acc)[T::FM
   float *maxima = (float *)(lds + MAX0);
   const long out0 = (GATED ? n0 / 2 : n0) + wn * OUTS;  // this wave's first output
   float largest[T::FM];
+  const bool ragged = out0 + OUTS > a.n;
   with_act8(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < T::FM; i++) {
@@ -144,14 +145,36 @@ __device__ __forceinline__ void into_rows8(const Args8 &a, floatx16 (&acc)[T::FM
             const int r = 4 * q + e;
             float v = act8<decltype(act)::value>(acc[i][GATED ? 2 * j : j][r] + b[e]);
             if constexpr (GATED) v *= acc[i][2 * j + 1][r] + u[e];
-            if (out0 + 32 * j + 8 * q + 4 * hi + e >= a.n) v = 0.0f;
             acc[i][j][r] = v;
-            m = fmaxf(m, finite_magnitude(v));
+            m = fmaxf(m, fabsf(v));  // (a NaN is passed over)
           }
         }
-      largest[i] = fmaxf(m, __shfl_xor(m, 32));
+      largest[i] = m;
     }
   });
+  // What is rare: outputs past the last one, which are zeros, and infinities, which are NaN and no largest magnitude.
+  bool infinite = false;
+#pragma unroll
+  for (int i = 0; i < T::FM; i++) infinite = infinite || !finite8(largest[i]);
+  if (ragged || __ballot(infinite)) {
+#pragma unroll
+    for (int i = 0; i < T::FM; i++) {
+      float m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < JS; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float v = acc[i][j][r];
+          if (out0 + 32 * j + 8 * (r / 4) + 4 * hi + r % 4 >= a.n) v = 0.0f;
+          if (!finite8(v)) v = __uint_as_float(0x7fc00000);
+          acc[i][j][r] = v;
+          m = fmaxf(m, fabsf(v));
+        }
+      largest[i] = m;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < T::FM; i++) largest[i] = fmaxf(largest[i], __shfl_xor(largest[i], 32));
   if constexpr (SHARED) {
 #pragma unroll
     for (int i = 0; i < T::FM; i++)
@@ -172,13 +195,10 @@ __device__ __forceinline__ void into_rows8(const Args8 &a, floatx16 (&acc)[T::FM
 #pragma unroll
     for (int j = 0; j < JS; j++)
 #pragma unroll
-      for (int q = 0; q < 4; q += 2) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = acc[i][j][4 * q + e];
-        const int2v p = pack8(v, inv);
-        *(int *)(st + l32 * PITCH + 32 * j + 8 * q + 4 * hi) = p.x;
-        *(int *)(st + l32 * PITCH + 32 * j + 8 * q + 8 + 4 * hi) = p.y;
+      for (int q = 0; q < 4; q++) {
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(acc[i][j][4 * q] * inv, acc[i][j][4 * q + 1] * inv, 0, false);
+        p = __builtin_amdgcn_cvt_pk_fp8_f32(acc[i][j][4 * q + 2] * inv, acc[i][j][4 * q + 3] * inv, p, true);
+        *(int *)(st + l32 * PITCH + 32 * j + 8 * q + 4 * hi) = p;
       }
     __builtin_amdgcn_wave_barrier();
     if (hi == 0 && (!SHARED || wn % 2 == 0) && r0 + l32 < rows)
