@@ -58,7 +58,9 @@ struct PlaceShared {
       : bins(p), before(bins + PLACE_WAVES * n), total(before + n), offsets(total + n), firsts(offsets + n),
         sums(firsts + TILE_SIZES * n) {}
 };
-constexpr size_t place_ints(size_t n) { return (PLACE_WAVES + 3 + TILE_SIZES) * n + PLACE_WAVES * (TILE_SIZES + 1); }
+constexpr size_t place_ints(size_t n) {
+  return std::max((PLACE_WAVES + 3 + TILE_SIZES) * n + PLACE_WAVES * (TILE_SIZES + 1), (size_t)512);
+}
 
 __device__ __forceinline__ int bin_of(int expert, int experts) {
   return (unsigned)expert < (unsigned)experts ? expert : experts;
@@ -203,6 +205,70 @@ __device__ void place_pairs(const PlanArgs &a, const PlaceShared &s, F expert) {
   }
 }
 
+// All of it for up to FEW_PAIRS pairs, a thread a pair: how many come before it is
+// counted pair by pair.  expert: their experts in LDS (as many as the next multiple of
+// sixteen), begin: room for as many.  (8 pairs of 64 experts with their choice: 7.6 us, the general
+// way 10.4; 128 pairs 13.0 and 11.3.)
+constexpr int FEW_PAIRS = 64;
+__device__ void place_few(const PlanArgs &a, int *expert, int *begin) {
+  const int pairs = (int)a.tokens * a.top, fours = (pairs + 15) / 16 * 4, p = threadIdx.x;
+  if (p >= pairs && p < 4 * fours) expert[p] = 1 << 30;  // (none's, after all others)
+  __syncthreads();
+  const int e = p < pairs ? expert[p] : 0;
+  int at = 0, row = 0, all = 0;
+  if (p < pairs) {
+#pragma unroll 4
+    for (int q = 0; q < fours; q++) {
+      const int4v v = *(const int4v *)(expert + 4 * q);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        at += v[i] < e;
+        all += v[i] == e;
+        row += v[i] == e && 4 * q + i < p;
+      }
+    }
+    at += row;
+    a.plan[a.at.order + at] = p;
+    a.plan[a.at.place + p] = e < a.experts ? at : -1;
+  }
+  // Whether a tile of each size begins at the pair, a byte each.
+  static_assert(TILE_SIZES == 4 && FEW_PAIRS < 256, "counts in bytes");
+  unsigned begins = 0;
+#pragma unroll
+  for (int k = 0; k < TILE_SIZES; k++)
+    if (p < pairs && e < a.experts && (row & (TILE_ROWS[k] - 1)) == 0) begins |= 1u << 8 * k;
+  if (p < 4 * fours) begin[p] = (int)begins;
+  for (int g = threadIdx.x; g <= a.experts; g += blockDim.x) {
+    int offset = 0;
+#pragma unroll 4
+    for (int q = 0; q < fours; q++) {
+      const int4v v = *(const int4v *)(expert + 4 * q);
+#pragma unroll
+      for (int i = 0; i < 4; i++) offset += v[i] < g;
+    }
+    a.plan[a.at.offsets + g] = offset;
+  }
+  __syncthreads();
+  if (p >= pairs) return;
+  unsigned before = 0, total = 0;  // tiles of smaller experts, of all
+#pragma unroll 4
+  for (int q = 0; q < fours; q++) {
+    const int4v v = *(const int4v *)(expert + 4 * q), b = *(const int4v *)(begin + 4 * q);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      total += (unsigned)b[i];
+      before += v[i] < e ? (unsigned)b[i] : 0;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < TILE_SIZES; k++) {
+    if (p == 0) a.plan[a.at.totals + k] = (int)(total >> 8 * k & 255);
+    if (begins >> 8 * k & 1)
+      *(int4v *)(a.plan + a.at.tiles[k] + 4l * ((before >> 8 * k & 255) + row / TILE_ROWS[k])) =
+          int4v{e, at, min(at + TILE_ROWS[k], at - row + all), 0};
+  }
+}
+
 __global__ __launch_bounds__(256) void k_plan_count(PlanArgs a) {
   __shared__ int bins[MAX_EXPERTS + 4];
   for (int e = threadIdx.x; e < (int)a.at.pitch; e += 256) bins[e] = 0;
@@ -217,6 +283,11 @@ template <bool ONE>
 __global__ __launch_bounds__(PLACE_LANES) void k_plan_place(PlanArgs a) {
   extern __shared__ int lds[];
   const int *index = a.index + (long)blockIdx.x * a.at.chunk * a.top;
+  if (ONE && a.tokens * a.top <= FEW_PAIRS) {
+    if (threadIdx.x < a.tokens * a.top) lds[threadIdx.x] = bin_of(index[threadIdx.x], a.experts);
+    place_few(a, lds, lds + FEW_PAIRS);
+    return;
+  }
   place_pairs<ONE>(a, PlaceShared(lds, a.experts + 1), [&](int p) { return bin_of(index[p], a.experts); });
 }
 
@@ -237,17 +308,35 @@ struct RouteArgs {
 
 constexpr float NONE = -__builtin_inff();
 
-// f(v, v of lane xor 1, 2, 4, ..) over each group of L lanes.
+// A DPP move of any 4 or 8 bytes.
+template <int CTRL, typename T>
+__device__ __forceinline__ T moved(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const long b = __builtin_bit_cast(long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(T, (unsigned long)hi << 32 | lo);
+  } else {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+  }
+}
+// f(other) for the moves that bring a value over each group of L lanes in halves.
 template <int L, typename F>
 __device__ __forceinline__ void over_lanes(F f) {
-  f([](float v) { return dpp_from<0xB1>(v); });
-  f([](float v) { return dpp_from<0x4E>(v); });
-  f([](float v) { return dpp_from<0x141>(v); });
-  f([](float v) { return dpp_from<0x140>(v); });
+  f([](auto v) { return moved<0xB1>(v); });
+  f([](auto v) { return moved<0x4E>(v); });
+  f([](auto v) { return moved<0x141>(v); });
+  f([](auto v) { return moved<0x140>(v); });
   if constexpr (L == 64) {
-    f([](float v) { return __shfl_xor(v, 16); });
-    f([](float v) { return __shfl_xor(v, 32); });
+    f([](auto v) { return __shfl_xor(v, 16); });
+    f([](auto v) { return __shfl_xor(v, 32); });
   }
+}
+// f(other) for the moves that bring each of 16 lanes the 15 others' values.
+template <int N = 1, typename F>
+__device__ __forceinline__ void round_lanes(F f) {
+  f([](auto v) { return moved<0x120 + N>(v); });  // (row_ror)
+  if constexpr (N < 15) round_lanes<N + 1>(f);
 }
 template <int L>
 __device__ __forceinline__ float largest(float v) {
@@ -256,7 +345,7 @@ __device__ __forceinline__ float largest(float v) {
 }
 template <int L>
 __device__ __forceinline__ int least(int v) {
-  over_lanes<L>([&](auto other) { v = min(v, __float_as_int(other(__int_as_float(v)))); });
+  over_lanes<L>([&](auto other) { v = min(v, other(v)); });
   return v;
 }
 
@@ -274,8 +363,8 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// One token's choice in f64 (by_logit: as it is, in `chosen`) and its weights, by a
-// whole wave, V experts a lane: lane k's is slot k's expert and weight.
+// One token's choice in f64 by a whole wave, V experts a lane: lane k's is slot k's
+// expert and weight.  by_logit: the weights of the experts that lanes hold in `chosen`.
 template <typename X, int V>
 __device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, double *ranks, int &chosen, float &weight) {
   constexpr int L = 64;
@@ -289,8 +378,7 @@ __device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, dou
   double m = none, sum = 0.0;
   if (a.softmax) {
     for (int e = lane; e < experts; e += L) m = fmax(m, logit(e));
-#pragma unroll
-    for (int k = 1; k < L; k *= 2) m = fmax(m, __shfl_xor(m, k));
+    over_lanes<L>([&](auto other) { m = fmax(m, other(m)); });
   }
   auto score = [&](double v) {
     if (v == none) return 0.0;
@@ -304,8 +392,7 @@ __device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, dou
     sum += c[i];
   }
   if (a.softmax) {
-#pragma unroll
-    for (int k = 1; k < L; k *= 2) sum += __shfl_xor(sum, k);
+    over_lanes<L>([&](auto other) { sum += other(sum); });
   } else {
     sum = 1.0;
   }
@@ -321,12 +408,11 @@ __device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, dou
 #pragma unroll
       for (int i = 0; i < V; i++)
         if (((lane + L * i) * a.magic) >> 22 == (unsigned)g) next = fmax(next, fmin(best, c[i])), best = fmax(best, c[i]);
-#pragma unroll
-      for (int k = 1; k < L; k *= 2) {
-        const double b = __shfl_xor(best, k), n = __shfl_xor(next, k);
+      over_lanes<L>([&](auto other) {
+        const double b = other(best), n = other(next);
         next = fmax(fmax(next, n), fmin(best, b));
         best = fmax(best, b);
-      }
+      });
       if (lane == 0) ranks[g] = a.group_top == 2 && next > none ? best + next : best;
     }
     wave_fence();
@@ -348,21 +434,19 @@ __device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, dou
 #pragma unroll
     for (int i = 0; i < V; i++)
       if (c[i] > best) best = c[i], at = lane + L * i;
-#pragma unroll
-    for (int n = 1; n < L; n *= 2) {
-      const double other = __shfl_xor(best, n);
-      const int there = __shfl_xor(at, n);
-      if (before(other, there, best, at)) best = other, at = there;
-    }
+    over_lanes<L>([&](auto other) {
+      const double that = other(best);
+      const int there = other(at);
+      if (before(that, there, best, at)) best = that, at = there;
+    });
 #pragma unroll
     for (int i = 0; i < V; i++)
       if (lane + L * i == at) c[i] = none;
     if (lane == k && best > none) chosen = at;
   }
-  const double s = lane < top && chosen >= 0 ? score(logit(chosen)) / sum : 0.0;
+  const double s = chosen >= 0 ? score(logit(chosen)) / sum : 0.0;
   double total = s;
-#pragma unroll
-  for (int k = 1; k < L; k *= 2) total += __shfl_xor(total, k);
+  over_lanes<L>([&](auto other) { total += other(total); });
   const double w = !a.renormalise ? s : total > 0.0 ? s / total : 0.0;
   weight = (float)(w * (double)a.scale);
 }
@@ -375,21 +459,26 @@ template <typename X, int L, int V, bool ONE>
 __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   constexpr int LANES = route_lanes(L), TOKENS = LANES / L;
   extern __shared__ int lds[];
+  __shared__ float4v candidates[L == 16 ? TOKENS * 16 : 1];  // a choice, its score, its expert
+  __shared__ float biases[L * V];
   const int experts = a.plan.experts, top = a.plan.top, n = experts + 1;
   const int lane = threadIdx.x % L, slot = threadIdx.x / L;
   int *bins = lds;                                      // the chunk's counts; ONE: its pairs' experts
-  const int held = ONE ? 64 * top : (int)a.plan.at.pitch;
-  float *ranks = (float *)(lds + (held + 3) / 4 * 4);  // [token][groups]; f64 of one token a wave
+  const int held = ONE ? 64 * top : (int)a.plan.at.pitch;  // (whole fours)
+  float *ranks = (float *)(lds + held);                   // [token][groups]; f64 of one token a wave
   if constexpr (!ONE) {
     for (int e = threadIdx.x; e < held; e += LANES) bins[e] = 0;
-    __syncthreads();
   }
-  float b[V], choice_size = 1.0f;  // (no choice is larger)
+  float choice_size = 1.0f;  // (no choice is larger)
+  for (int e = threadIdx.x; e < L * V; e += LANES) {
+    const float b = a.bias && e < experts ? a.bias[e] : 0.0f;
+    biases[e] = b > NONE ? b : NONE;  // (NaN too)
+  }
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    b[i] = a.bias && lane + L * i < experts ? a.bias[lane + L * i] : 0.0f;
-    if (!(b[i] > NONE)) b[i] = NONE;
-    if (fabsf(b[i]) < __builtin_inff()) choice_size = fmaxf(choice_size, 1.0f + fabsf(b[i]));
+    const float b = fabsf(biases[lane + L * i]);
+    if (b < __builtin_inff()) choice_size = fmaxf(choice_size, 1.0f + b);
   }
   choice_size = largest<L>(choice_size);
   const long begin = (long)blockIdx.x * a.plan.at.chunk, end = min(begin + a.plan.at.chunk, a.plan.tokens);
@@ -433,7 +522,10 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     }
     if (a.bias) {
 #pragma unroll
-      for (int i = 0; i < V; i++) c[i] = c[i] == NONE || b[i] == NONE ? NONE : s[i] + b[i];
+      for (int i = 0; i < V; i++) {
+        const float b = biases[lane + L * i];
+        c[i] = c[i] == NONE || b == NONE ? NONE : s[i] + b;
+      }
     } else if (!a.by_logit) {
 #pragma unroll
       for (int i = 0; i < V; i++) c[i] = c[i] == NONE ? NONE : s[i];
@@ -443,29 +535,51 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     const float near = 0x1p-23f * (off + choice_size), near_ranks = 2.0f * near + 0x1p-22f * choice_size;
     bool unclear = false;
     if (a.kept < a.groups) {
-      float *mine = ranks + (L == 16 ? 1 : 2) * slot * a.groups;
       const int per = experts / a.groups;
-      auto rank_of = [&](int g, float best, float next) {
+      auto rank_of = [&](float best, float next) {
         over_lanes<L>([&](auto other) {
           const float b2 = other(best), n2 = other(next);
           next = fmaxf(fmaxf(next, n2), fminf(best, b2));
           best = fmaxf(best, b2);
         });
-        if (lane == 0) mine[g] = a.group_top == 2 && next > NONE ? best + next : best;
+        return a.group_top == 2 && next > NONE ? best + next : best;
       };
-      if (per % L == 0) {  // a group is some of every lane's experts, one after another
-        float best = NONE, next = NONE;
+      float low = __builtin_inff(), high = NONE;  // the last group kept, the first one not
+      if (per % L == 0) {  // a group is some of every lane's experts, one after another: lane g has group g's rank
+        float best = NONE, next = NONE, own = NONE;
         int g = 0;
 #pragma unroll
         for (int i = 0; i < V; i++) {
           next = fmaxf(next, fminf(best, c[i]));
           best = fmaxf(best, c[i]);
           if ((i + 1) * L == (g + 1) * per) {
-            rank_of(g++, best, next);
+            const float rank = rank_of(best, next);
+            if (lane == g) own = rank;
+            g++;
             best = next = NONE;
           }
         }
+        int ahead = 0;
+        if constexpr (L == 16) {
+          round_lanes([&](auto other) {
+            const float rank = other(own);
+            const int at = other(lane);
+            ahead += rank > own || (rank == own && at < lane);
+          });
+        } else {
+          for (int k = 0; k < a.groups; k++) {
+            const float rank = __shfl(own, k);
+            ahead += rank > own || (rank == own && k < lane);
+          }
+        }
+        const bool keep = ahead < a.kept && lane < a.groups;
+        if (lane < a.groups) (keep ? low : high) = own;
+        const unsigned long long kept = __ballot(keep) >> (L == 16 ? slot % 4 * 16 : 0);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (!(kept >> (L * i * a.magic >> 22) & 1)) c[i] = NONE;
       } else {
+        float *mine = ranks + (L == 16 ? 1 : 2) * slot * a.groups;
         for (int g = 0; g < a.groups; g++) {
           float best = NONE, next = NONE;
 #pragma unroll
@@ -474,58 +588,106 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
             next = fmaxf(next, fminf(best, v));
             best = fmaxf(best, v);
           }
-          rank_of(g, best, next);
+          const float rank = rank_of(best, next);
+          if (lane == 0) mine[g] = rank;
         }
-      }
-      wave_fence();
-      // The groups kept, and how near the last of them and the first of the others are.
-      unsigned long long keep = 0;  // of this lane's groups lane + L j
-      float low = __builtin_inff(), high = NONE;
-      for (int j = 0; lane + L * j < a.groups; j++) {
-        const float rank = mine[lane + L * j];
-        int ahead = 0;
-        for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
-        if (ahead < a.kept)
-          keep |= 1ull << j, low = fminf(low, rank);
-        else
-          high = fmaxf(high, rank);
+        wave_fence();
+        unsigned long long keep = 0;  // of this lane's groups lane + L j
+        for (int j = 0; lane + L * j < a.groups; j++) {
+          const float rank = mine[lane + L * j];
+          int ahead = 0;
+          for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
+          if (ahead < a.kept)
+            keep |= 1ull << j, low = fminf(low, rank);
+          else
+            high = fmaxf(high, rank);
+        }
+        wave_fence();
+        for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = keep >> j & 1 ? 1.0f : 0.0f;
+        wave_fence();
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (lane + L * i < experts && mine[(lane + L * i) * a.magic >> 22] == 0.0f) c[i] = NONE;
+        wave_fence();
       }
       over_lanes<L>([&](auto other) { low = fminf(low, other(low)), high = fmaxf(high, other(high)); });
       unclear = high > NONE && low - high < near_ranks;
-      wave_fence();
-      for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = keep >> j & 1 ? 1.0f : 0.0f;
-      wave_fence();
-#pragma unroll
-      for (int i = 0; i < V; i++)
-        if (lane + L * i < experts && mine[(lane + L * i) * a.magic >> 22] == 0.0f) c[i] = NONE;
-      wave_fence();
     }
-    // Slot k's expert and score stay with lane k.
-    int chosen = -1;
-    bool any = false;
-    float score = 0.0f, total = 0.0f, last = __builtin_inff();
-    for (int k = 0; k <= top; k++) {
-      float best = NONE;
+    // A lane's expert and score, and which slot they are for: the slots' are the first `top`.
+    int chosen = -1, place = lane;
+    bool any = false, choose = true;
+    float score = 0.0f, total = 0.0f;
+    if constexpr (L == 16) {
+      // By counting.  At least top + 1 choices are as large as the (top + 1)-th of the lanes' largest; where they
+      // are 16 at most, as they mostly are, every lane takes one and counts those before it.
+      float mine = NONE;
 #pragma unroll
-      for (int i = 0; i < V; i++) best = fmaxf(best, c[i]);
-      best = largest<L>(best);
-      if (best > NONE && last - best < near) unclear = true;
-      last = best;
-      any = any || best > NONE;
-      if (k == top) break;
-      int at = 1 << 30;
-      float its = 0.0f;
+      for (int i = 0; i < V; i++) mine = fmaxf(mine, c[i]);
+      int ahead = 0;
+      round_lanes([&](auto other) { ahead += other(mine) > mine; });
+      float least_of = ahead <= top ? mine : __builtin_inff();
+      over_lanes<L>([&](auto other) { least_of = fminf(least_of, other(least_of)); });
+      int upto = 0, own;
 #pragma unroll
-      for (int i = V - 1; i >= 0; i--)
-        if (c[i] == best) at = lane + L * i, its = s[i];
-      const int first = least<L>(at);
-      const bool owner = first == at;
+      for (int i = 0; i < V; i++) upto += c[i] >= least_of && c[i] > NONE;
+      own = upto;
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xF, 0xF, true);  // (row_shr 1, 2, 4, 8: sums from lane 0 on)
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xF, 0xF, true);
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, true);
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, true);
+      if (top < 16 && !__ballot(upto > 16)) {
+        float4v *list = candidates + slot * 16;
+        list[lane] = float4v{NONE, 0.0f, __int_as_float((int)MAX_EXPERTS + lane), 0.0f};
+        wave_fence();
+        int at = upto - own;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (first == lane + L * i) c[i] = NONE;
-      its = group_sum<L>(owner && best > NONE ? its : 0.0f);
-      total += its;
-      if (lane == k && best > NONE) chosen = first, score = its;
+        for (int i = 0; i < V; i++)
+          if (c[i] >= least_of && c[i] > NONE) list[at++] = float4v{c[i], s[i], __int_as_float(lane + L * i), 0.0f};
+        wave_fence();
+        const float4v one = list[lane];
+        const float value = one[0];
+        const int expert = __float_as_int(one[2]);
+        place = 0;
+        bool close = false;
+        round_lanes([&](auto other) {
+          const float that = other(value);
+          const int there = other(expert);
+          place += that > value || (that == value && there < expert);
+          close = close || fabsf(value - that) < near;
+        });
+        const bool taken = place < top && value > NONE;
+        if (taken) chosen = expert, score = one[1];
+        unclear = unclear || (taken && close);
+        total = group_sum<L>(score);
+        any = largest<L>(value) > NONE;
+        choose = false;
+      }
+    }
+    if (choose) {  // slot k's stay with lane k
+      float last = __builtin_inff();
+      for (int k = 0; k <= top; k++) {
+        float best = NONE;
+#pragma unroll
+        for (int i = 0; i < V; i++) best = fmaxf(best, c[i]);
+        best = largest<L>(best);
+        if (best > NONE && last - best < near) unclear = true;
+        last = best;
+        any = any || best > NONE;
+        if (k == top) break;
+        int at = 1 << 30;
+        float its = 0.0f;
+#pragma unroll
+        for (int i = V - 1; i >= 0; i--)
+          if (c[i] == best) at = lane + L * i, its = s[i];
+        const int first = least<L>(at);
+        const bool owner = first == at;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (first == lane + L * i) c[i] = NONE;
+        its = group_sum<L>(owner && best > NONE ? its : 0.0f);
+        total += its;
+        if (lane == k && best > NONE) chosen = first, score = its;
+      }
     }
     float weight = (!a.renormalise ? score : total > 0.0f ? score / total : 0.0f) * a.scale;
     // (f32 scores that vanish: their shares need not.)
@@ -534,16 +696,20 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       const int first = __ffsll(left) - 1, token = first / L;  // (the wave's)
       left &= ~((L == 64 ? ~0ull : (1ull << (L & 63)) - 1) << token * L);
       const long there = __shfl(t, first);
-      int c64 = __shfl(chosen, token * L + lane);
+      const bool mine = slot % (64 / L) == token;
+      int c64 = mine ? chosen : -1;
       float w64;
       choose_f64<X, (L * V + 63) / 64>(a, (const X *)a.logits + there * a.stride,
                                        (double *)(ranks + (L == 16 ? slot / 4 * 4 : 2 * slot) * a.groups), c64, w64);
-      c64 = __shfl(c64, lane);
-      w64 = __shfl(w64, lane);
-      if (slot % (64 / L) == token) chosen = c64, weight = w64;
+      if (!a.by_logit) {
+        c64 = __shfl(c64, lane);
+        w64 = __shfl(w64, lane);
+        if (mine) chosen = c64, place = lane;
+      }
+      if (mine) weight = w64;
     }
-    if (some && lane < top) {
-      const long pair = t * top + lane;
+    if (some && place < top) {
+      const long pair = t * top + place;
       a.index[pair] = chosen;
       a.weight[pair] = weight;
       if constexpr (ONE)
@@ -554,8 +720,10 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     wave_fence();  // (the ranks' next token)
   }
   __syncthreads();
-  if constexpr (ONE)
-    place_pairs<true>(a.plan, PlaceShared(lds + (held + 3) / 4 * 4, n), [&](int p) { return bins[p]; });
+  if (ONE && a.plan.tokens * top <= FEW_PAIRS)
+    place_few(a.plan, bins, lds + held);
+  else if constexpr (ONE)
+    place_pairs<true>(a.plan, PlaceShared(lds + held, n), [&](int p) { return bins[p]; });
   else
     for (int e = threadIdx.x; e < held; e += LANES) a.plan.plan[a.plan.at.parts + blockIdx.x * a.plan.at.pitch + e] = bins[e];
 }
@@ -575,7 +743,7 @@ void launch_route(ien_ctx *ctx, const RouteArgs &a) {
   const size_t held = one ? 64 * (size_t)p.top : (size_t)p.at.pitch;
   size_t ints = a.kept < a.groups ? (size_t)(route_lanes(L) / L) * a.groups * (L == 16 ? 1 : 2) : 0;
   if (one) ints = std::max(ints, place_ints((size_t)p.experts + 1));
-  const size_t lds = ((held + 3) / 4 * 4 + ints) * 4;
+  const size_t lds = (held + ints) * 4;
   if (one)
     hipLaunchKernelGGL((k_route<X, L, V, true>), dim3(1), dim3(route_lanes(L)), lds, ctx->stream, a);
   else
