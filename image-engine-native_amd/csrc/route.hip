@@ -133,9 +133,12 @@ __device__ void place_pairs(const PlanArgs &a, const PlaceShared &s, F expert) {
   const int pairs = (int)(min((blockIdx.x + 1) * a.at.chunk, a.tokens) * a.top - begin);
   const int part = (pairs + 64 * PLACE_WAVES - 1) / (64 * PLACE_WAVES) * 64;
   const int from = min(wave * part, pairs), to = wave < PLACE_WAVES ? min(from + part, pairs) : from;
+  constexpr int HELD = 4;  // a lane's first pairs' experts stay in registers: their loads are under way beside the counts'
+  int held[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; k++) held[k] = from + 64 * k + lane < to ? expert(from + 64 * k + lane) : 0;
   for (int i = tid; i < (PLACE_WAVES + 2) * n; i += blockDim.x) s.bins[i] = 0;  // (before and total too)
   __syncthreads();
-  for (int p = from + lane; p < to; p += 64) atomicAdd(s.bins + wave * n + expert(p), 1);
   if constexpr (!ONE) {
     // Four bins a thread, chunks side by side.
     const int fours = (int)a.at.pitch / 4, groups = (int)blockDim.x / fours, four = tid % fours, group = tid / fours;
@@ -155,6 +158,10 @@ __device__ void place_pairs(const PlanArgs &a, const PlaceShared &s, F expert) {
         }
     }
   }
+#pragma unroll
+  for (int k = 0; k < HELD; k++)
+    if (from + 64 * k + lane < to) atomicAdd(s.bins + wave * n + held[k], 1);
+  for (int p = from + 64 * HELD + lane; p < to; p += 64) atomicAdd(s.bins + wave * n + expert(p), 1);
   __syncthreads();
   if constexpr (ONE) {
     for (int e = tid; e < n; e += blockDim.x) {
@@ -180,7 +187,10 @@ __device__ void place_pairs(const PlanArgs &a, const PlaceShared &s, F expert) {
   for (int p0 = from; p0 < to; p0 += 64) {
     const int p = p0 + lane;
     const bool some = p < to;
-    const int e = some ? expert(p) : 0;
+    int e = held[0];
+    if (p0 >= from + 64 * HELD) e = some ? expert(p) : 0;
+#pragma unroll
+    for (int k = 0; k + 1 < HELD; k++) held[k] = held[k + 1];
     unsigned long long same = __ballot(some);
     for (int bit = 0; bit < bits; bit++) {
       const unsigned long long set = __ballot(e >> bit & 1);
@@ -313,11 +323,11 @@ template <int CTRL, typename T>
 __device__ __forceinline__ T moved(T v) {
   if constexpr (sizeof(T) == 8) {
     const long b = __builtin_bit_cast(long, v);
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false);
-    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, true);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, true);
     return __builtin_bit_cast(T, (unsigned long)hi << 32 | lo);
   } else {
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
   }
 }
 // f(other) for the moves that bring a value over each group of L lanes in halves.
@@ -339,8 +349,8 @@ __device__ __forceinline__ void round_lanes(F f) {
   if constexpr (N < 15) round_lanes<N + 1>(f);
 }
 template <int L>
-__device__ __forceinline__ float largest(float v) {
-  over_lanes<L>([&](auto other) { v = fmaxf(v, other(v)); });
+__device__ __forceinline__ int largest(int v) {
+  over_lanes<L>([&](auto other) { v = max(v, other(v)); });
   return v;
 }
 template <int L>
@@ -348,6 +358,15 @@ __device__ __forceinline__ int least(int v) {
   over_lanes<L>([&](auto other) { v = min(v, other(v)); });
   return v;
 }
+
+// A float as an integer in the same order (both zeros as one), and back: integers are
+// compared and moved in one instruction, floats are made quiet first.
+__device__ __forceinline__ int key_of(float v) {
+  const int b = __float_as_int(v + 0.0f);
+  return b ^ (b >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ float value_of(int key) { return __int_as_float(key ^ (key >> 31 & 0x7fffffff)); }
+constexpr int NO_KEY = (int)0x807fffff;  // of NONE
 
 // e^x: the hardware's power of two of the rounded x log2(e), times what the rounding left (some 2 steps of f32).
 __device__ __forceinline__ float exp_f(float x) {
@@ -459,39 +478,52 @@ template <typename X, int L, int V, bool ONE>
 __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   constexpr int LANES = route_lanes(L), TOKENS = LANES / L;
   extern __shared__ int lds[];
-  __shared__ float4v candidates[L == 16 ? TOKENS * 16 : 1];  // a choice, its score, its expert
+  __shared__ int4v candidates[L == 16 ? TOKENS * 16 : 1];  // a choice's key, its score, its expert
+  __shared__ int taken_tokens;
   __shared__ float biases[L * V];
   const int experts = a.plan.experts, top = a.plan.top, n = experts + 1;
-  const int lane = threadIdx.x % L, slot = threadIdx.x / L;
+  int lane = threadIdx.x % L;
+  const int slot = threadIdx.x / L;
   int *bins = lds;                                      // the chunk's counts; ONE: its pairs' experts
   const int held = ONE ? 64 * top : (int)a.plan.at.pitch;  // (whole fours)
   float *ranks = (float *)(lds + held);                   // [token][groups]; f64 of one token a wave
   if constexpr (!ONE) {
     for (int e = threadIdx.x; e < held; e += LANES) bins[e] = 0;
   }
-  float choice_size = 1.0f;  // (no choice is larger)
+  int size_key = key_of(1.0f);  // of a choice that none is larger than
   for (int e = threadIdx.x; e < L * V; e += LANES) {
     const float b = a.bias && e < experts ? a.bias[e] : 0.0f;
     biases[e] = b > NONE ? b : NONE;  // (NaN too)
   }
+  if (threadIdx.x == 0) taken_tokens = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const float b = fabsf(biases[lane + L * i]);
-    if (b < __builtin_inff()) choice_size = fmaxf(choice_size, 1.0f + b);
+    if (b < __builtin_inff()) size_key = max(size_key, key_of(1.0f + b));
   }
-  choice_size = largest<L>(choice_size);
+  const float choice_size = value_of(largest<L>(size_key));
   const long begin = (long)blockIdx.x * a.plan.at.chunk, end = min(begin + a.plan.at.chunk, a.plan.tokens);
-  for (long t0 = begin; t0 < end; t0 += TOKENS) {
-    const long t = min(t0 + slot, end - 1);
-    const bool some = t0 + slot < end;
+  for (;;) {
+    asm volatile("" : "+v"(lane));  // (what follows from it is cheaper to compute again than to keep: 48 registers too many)
+    // The next of the chunk's tokens that no wave has (a wave may be held up by a choice in f64).
+    int next = 0;
+    if ((threadIdx.x & 63) == 0) next = atomicAdd(&taken_tokens, 64 / L);
+    const long t0 = begin + __builtin_amdgcn_readfirstlane(next);
+    if (t0 >= end) break;
+    const long t = min(t0 + slot % (64 / L), end - 1);
+    const bool some = t0 + slot % (64 / L) < end;
     const X *row = (const X *)a.logits + t * a.stride;
-    float s[V], c[V];
+    float s[V];
+    int c[V];  // the choices' keys
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int e = lane + L * i;
-      const float v = e < experts ? (float)row[e] : NONE;
-      c[i] = v > NONE ? v : NONE;  // (NaN too)
+      s[i] = (float)row[min(lane + L * i, experts - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      s[i] = s[i] > NONE && lane + L * i < experts ? s[i] : NONE;  // (NaN too)
+      c[i] = key_of(s[i]);
     }
     // How far a score may be off, in halves of a step of 1: of a logistic function 4 of its exponential, at most
     // a quarter of which reaches it, a step of the reciprocal and two roundings; of a softmax 0.4 of the argument
@@ -499,13 +531,14 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     // arguments, 21 of the additions and 2 of the quotient.
     float off = 5.0f;
     if (a.softmax) {
-      float m = NONE, sum = 0.0f;
+      int key = NO_KEY;
 #pragma unroll
-      for (int i = 0; i < V; i++) m = fmaxf(m, c[i]);
-      m = largest<L>(m);
+      for (int i = 0; i < V; i++) key = max(key, c[i]);
+      const float m = value_of(largest<L>(key));
+      float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        s[i] = c[i] == NONE ? 0.0f : c[i] == m ? 1.0f : exp_f(c[i] - m);  // (infinite ones share all)
+        s[i] = c[i] == NO_KEY ? 0.0f : s[i] == m ? 1.0f : exp_f(s[i] - m);  // (infinite ones share all)
         sum += s[i];
       }
       sum = group_sum<L>(sum);
@@ -516,19 +549,19 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float e = exp_f(-fabsf(c[i]));
-        s[i] = (c[i] < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
+        const float e = exp_f(-fabsf(s[i]));
+        s[i] = (s[i] < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
       }
     }
     if (a.bias) {
 #pragma unroll
       for (int i = 0; i < V; i++) {
         const float b = biases[lane + L * i];
-        c[i] = c[i] == NONE || b == NONE ? NONE : s[i] + b;
+        c[i] = c[i] == NO_KEY || b == NONE ? NO_KEY : key_of(s[i] + b);
       }
     } else if (!a.by_logit) {
 #pragma unroll
-      for (int i = 0; i < V; i++) c[i] = c[i] == NONE ? NONE : s[i];
+      for (int i = 0; i < V; i++) c[i] = c[i] == NO_KEY ? NO_KEY : key_of(s[i]);
     }
     // Two choices that are nearer than this may be in the other order (each is off by its score's error and its own
     // rounding), and two ranks that are nearer than twice this and their own roundings.
@@ -536,82 +569,81 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     bool unclear = false;
     if (a.kept < a.groups) {
       const int per = experts / a.groups;
-      auto rank_of = [&](float best, float next) {
+      auto rank_of = [&](int best, int next) {
         over_lanes<L>([&](auto other) {
-          const float b2 = other(best), n2 = other(next);
-          next = fmaxf(fmaxf(next, n2), fminf(best, b2));
-          best = fmaxf(best, b2);
+          next = max(max(next, other(next)), min(best, other(best)));
+          best = max(best, other(best));
         });
-        return a.group_top == 2 && next > NONE ? best + next : best;
+        return a.group_top == 2 && next > NO_KEY ? key_of(value_of(best) + value_of(next)) : best;
       };
-      float low = __builtin_inff(), high = NONE;  // the last group kept, the first one not
+      int low = 0x7fffffff, high = NO_KEY;  // the last group kept, the first one not
       if (per % L == 0) {  // a group is some of every lane's experts, one after another: lane g has group g's rank
-        float best = NONE, next = NONE, own = NONE;
-        int g = 0;
+        int best = NO_KEY, next = NO_KEY, own = NO_KEY, g = 0;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          next = fmaxf(next, fminf(best, c[i]));
-          best = fmaxf(best, c[i]);
+          next = max(next, min(best, c[i]));
+          best = max(best, c[i]);
           if ((i + 1) * L == (g + 1) * per) {
-            const float rank = rank_of(best, next);
+            const int rank = rank_of(best, next);
             if (lane == g) own = rank;
             g++;
-            best = next = NONE;
+            best = next = NO_KEY;
           }
         }
         int ahead = 0;
         if constexpr (L == 16) {
           round_lanes([&](auto other) {
-            const float rank = other(own);
-            const int at = other(lane);
+            const int rank = other(own), at = other(lane);
             ahead += rank > own || (rank == own && at < lane);
           });
         } else {
           for (int k = 0; k < a.groups; k++) {
-            const float rank = __shfl(own, k);
+            const int rank = __shfl(own, k);
             ahead += rank > own || (rank == own && k < lane);
           }
         }
         const bool keep = ahead < a.kept && lane < a.groups;
         if (lane < a.groups) (keep ? low : high) = own;
-        const unsigned long long kept = __ballot(keep) >> (L == 16 ? slot % 4 * 16 : 0);
+        int kept = (int)(__ballot(keep) >> (L == 16 ? slot % 4 * 16 : 0)), edge = per;
 #pragma unroll
-        for (int i = 0; i < V; i++)
-          if (!(kept >> (L * i * a.magic >> 22) & 1)) c[i] = NONE;
+        for (int i = 0; i < V; i++) {
+          if (i * L == edge) kept >>= 1, edge += per;
+          if (!(kept & 1)) c[i] = NO_KEY;
+        }
       } else {
-        float *mine = ranks + (L == 16 ? 1 : 2) * slot * a.groups;
+        int *mine = (int *)ranks + (L == 16 ? 1 : 2) * slot * a.groups;
         for (int g = 0; g < a.groups; g++) {
-          float best = NONE, next = NONE;
+          int best = NO_KEY, next = NO_KEY;
 #pragma unroll
           for (int i = 0; i < V; i++) {
-            const float v = (lane + L * i) * a.magic >> 22 == (unsigned)g ? c[i] : NONE;
-            next = fmaxf(next, fminf(best, v));
-            best = fmaxf(best, v);
+            const int v = (lane + L * i) * a.magic >> 22 == (unsigned)g ? c[i] : NO_KEY;
+            next = max(next, min(best, v));
+            best = max(best, v);
           }
-          const float rank = rank_of(best, next);
+          const int rank = rank_of(best, next);
           if (lane == 0) mine[g] = rank;
         }
         wave_fence();
         unsigned long long keep = 0;  // of this lane's groups lane + L j
         for (int j = 0; lane + L * j < a.groups; j++) {
-          const float rank = mine[lane + L * j];
+          const int rank = mine[lane + L * j];
           int ahead = 0;
           for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
           if (ahead < a.kept)
-            keep |= 1ull << j, low = fminf(low, rank);
+            keep |= 1ull << j, low = min(low, rank);
           else
-            high = fmaxf(high, rank);
+            high = max(high, rank);
         }
         wave_fence();
-        for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = keep >> j & 1 ? 1.0f : 0.0f;
+        for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = (int)(keep >> j & 1);
         wave_fence();
 #pragma unroll
         for (int i = 0; i < V; i++)
-          if (lane + L * i < experts && mine[(lane + L * i) * a.magic >> 22] == 0.0f) c[i] = NONE;
+          if (lane + L * i < experts && mine[(lane + L * i) * a.magic >> 22] == 0) c[i] = NO_KEY;
         wave_fence();
       }
-      over_lanes<L>([&](auto other) { low = fminf(low, other(low)), high = fmaxf(high, other(high)); });
-      unclear = high > NONE && low - high < near_ranks;
+      low = least<L>(low), high = largest<L>(high);
+      unclear = high > NO_KEY && value_of(low) - value_of(high) < near_ranks;
     }
     // A lane's expert and score, and which slot they are for: the slots' are the first `top`.
     int chosen = -1, place = lane;
@@ -620,73 +652,72 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     if constexpr (L == 16) {
       // By counting.  At least top + 1 choices are as large as the (top + 1)-th of the lanes' largest; where they
       // are 16 at most, as they mostly are, every lane takes one and counts those before it.
-      float mine = NONE;
+      int mine = NO_KEY;
 #pragma unroll
-      for (int i = 0; i < V; i++) mine = fmaxf(mine, c[i]);
+      for (int i = 0; i < V; i++) mine = max(mine, c[i]);
       int ahead = 0;
       round_lanes([&](auto other) { ahead += other(mine) > mine; });
-      float least_of = ahead <= top ? mine : __builtin_inff();
-      over_lanes<L>([&](auto other) { least_of = fminf(least_of, other(least_of)); });
+      const int from = max(least<L>(ahead <= top ? mine : 0x7fffffff), NO_KEY + 1);
       int upto = 0, own;
 #pragma unroll
-      for (int i = 0; i < V; i++) upto += c[i] >= least_of && c[i] > NONE;
+      for (int i = 0; i < V; i++) upto += c[i] >= from;
       own = upto;
       upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xF, 0xF, true);  // (row_shr 1, 2, 4, 8: sums from lane 0 on)
       upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xF, 0xF, true);
       upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, true);
       upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, true);
       if (top < 16 && !__ballot(upto > 16)) {
-        float4v *list = candidates + slot * 16;
-        list[lane] = float4v{NONE, 0.0f, __int_as_float((int)MAX_EXPERTS + lane), 0.0f};
+        int4v *list = candidates + slot * 16;
+        list[lane] = int4v{NO_KEY, 0, (int)MAX_EXPERTS + lane, 0};
         wave_fence();
         int at = upto - own;
 #pragma unroll
         for (int i = 0; i < V; i++)
-          if (c[i] >= least_of && c[i] > NONE) list[at++] = float4v{c[i], s[i], __int_as_float(lane + L * i), 0.0f};
+          if (c[i] >= from) list[at++] = int4v{c[i], __float_as_int(s[i]), lane + L * i, 0};
         wave_fence();
-        const float4v one = list[lane];
-        const float value = one[0];
-        const int expert = __float_as_int(one[2]);
+        const int4v one = list[lane];
+        const int key = one[0], expert = one[2];
+        const float value = value_of(key);
         place = 0;
-        bool close = false;
+        int close = 0;
         round_lanes([&](auto other) {
-          const float that = other(value);
-          const int there = other(expert);
-          place += that > value || (that == value && there < expert);
-          close = close || fabsf(value - that) < near;
+          const int that = other(key), there = other(expert);
+          place += that > key || (that == key && there < expert);
+          close |= fabsf(value - other(value)) < near;
         });
-        const bool taken = place < top && value > NONE;
-        if (taken) chosen = expert, score = one[1];
-        unclear = unclear || (taken && close);
+        const bool taken = place < top && key > NO_KEY;
+        if (taken) chosen = expert, score = __int_as_float(one[1]);
+        unclear = unclear || largest<L>(taken ? close : 0);
         total = group_sum<L>(score);
-        any = largest<L>(value) > NONE;
+        any = largest<L>(key) > NO_KEY;
         choose = false;
       }
     }
     if (choose) {  // slot k's stay with lane k
       float last = __builtin_inff();
       for (int k = 0; k <= top; k++) {
-        float best = NONE;
+        int key = NO_KEY;
 #pragma unroll
-        for (int i = 0; i < V; i++) best = fmaxf(best, c[i]);
-        best = largest<L>(best);
-        if (best > NONE && last - best < near) unclear = true;
+        for (int i = 0; i < V; i++) key = max(key, c[i]);
+        key = largest<L>(key);
+        const float best = value_of(key);
+        if (key > NO_KEY && last - best < near) unclear = true;
         last = best;
-        any = any || best > NONE;
+        any = any || key > NO_KEY;
         if (k == top) break;
         int at = 1 << 30;
         float its = 0.0f;
 #pragma unroll
         for (int i = V - 1; i >= 0; i--)
-          if (c[i] == best) at = lane + L * i, its = s[i];
+          if (c[i] == key) at = lane + L * i, its = s[i];
         const int first = least<L>(at);
         const bool owner = first == at;
 #pragma unroll
         for (int i = 0; i < V; i++)
-          if (first == lane + L * i) c[i] = NONE;
-        its = group_sum<L>(owner && best > NONE ? its : 0.0f);
+          if (first == lane + L * i) c[i] = NO_KEY;
+        its = group_sum<L>(owner && key > NO_KEY ? its : 0.0f);
         total += its;
-        if (lane == k && best > NONE) chosen = first, score = its;
+        if (lane == k && key > NO_KEY) chosen = first, score = its;
       }
     }
     float weight = (!a.renormalise ? score : total > 0.0f ? score / total : 0.0f) * a.scale;
