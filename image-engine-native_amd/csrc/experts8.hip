@@ -55,7 +55,8 @@ ien_status ien_experts8_new(ien_ctx *ctx, const void *d_w, ien_wtype wtype, size
             IEN_ERR_INPUT, "%s weights of %zu experts x %zu x %zu", gated ? "gated" : "plain", experts, c, n);
   const long npad = gated ? 2 * (long)((n / 2 + 127) / 128 * 128) : (long)((n + 127) / 128 * 128);
   const size_t panels = experts * blocks8(c);
-  IEN_CHECK(panels * (size_t)npad < (1ull << 36), IEN_ERR_INPUT, "too many weights: %zu x %zu x %zu", experts, c, n);
+  // (A tile addresses an expert's scales by 31-bit offsets.)
+  IEN_CHECK(blocks8(c) * (size_t)npad < (1ull << 28), IEN_ERR_INPUT, "too many weights an expert: %zu x %zu", c, n);
   ien_experts8 *m = new (std::nothrow) ien_experts8;
   IEN_CHECK(m, IEN_ERR_GPU, "experts' weights: out of host memory");
   m->ctx = ctx;

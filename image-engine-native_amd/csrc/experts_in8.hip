@@ -12,15 +12,17 @@ namespace ien {
 namespace {
 
 template <typename T, Kind8 KIND>
-void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, int size) {
+bool launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, int size) {
   a.tiles_n = (int)((a.npad + T::TN - 1) / T::TN);
   a.list = (const ExpertTile *)(r->d_plan + p.tiles[size]);
   a.total = r->d_plan + p.totals + size;
+  if (!launches(p.most[size], a.tiles_n, T::THREADS)) return false;
   const dim3 grid((unsigned)(p.most[size] * a.tiles_n));
   if (a.exact)
     hipLaunchKernelGGL((k_tile8<T, true, _Float16, KIND>), grid, dim3(T::THREADS), 0, ctx->stream, a);
   else
     hipLaunchKernelGGL((k_tile8<T, false, _Float16, KIND>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  return true;
 }
 
 }  // namespace
@@ -97,21 +99,23 @@ extern "C" ien_status ien_experts_in8(ien_ctx *ctx, const ien_rows8 *x, const ie
   a.qs = out->scales;
   a.qsstride = (long)out->scale_stride;
   const long pairs = (long)(routes->tokens * routes->top);
+  bool done = false;
   switch (experts_in_choice(ctx->cus, pairs, (long)routes->experts, a.npad, a.cb, w->gated)) {
     case 0:
-      w->gated ? launch_few<EXPERTS_GATED8, float, 8, 1>(ctx, a, routes, p)
-               : launch_few<EXPERTS_ACT8, float, 8, 1>(ctx, a, routes, p);
+      done = w->gated ? launch_few<EXPERTS_GATED8, float, 8, 1>(ctx, a, routes, p)
+                      : launch_few<EXPERTS_ACT8, float, 8, 1>(ctx, a, routes, p);
       break;
     case 1:
-      w->gated ? launch<Tile8<1, 4, 2, 2, 3>, EXPERTS_GATED8>(ctx, a, routes, p, 1)
-               : launch<Tile8<1, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 1);
+      done = w->gated ? launch<Tile8<1, 4, 2, 2, 3>, EXPERTS_GATED8>(ctx, a, routes, p, 1)
+                      : launch<Tile8<1, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 1);
       break;
     case 2:
-      w->gated ? launch<Tile8<1, 4, 4, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 2)
-               : launch<Tile8<2, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 2);
+      done = w->gated ? launch<Tile8<1, 4, 4, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 2)
+                      : launch<Tile8<2, 2, 2, 2, 2>, EXPERTS_ACT8>(ctx, a, routes, p, 2);
       break;
-    default: launch<Tile8<2, 4, 4, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 3); break;
+    default: done = launch<Tile8<2, 4, 4, 2, 2>, EXPERTS_GATED8>(ctx, a, routes, p, 3); break;
   }
+  IEN_CHECK(done, IEN_ERR_INPUT, "experts_in8: %ld pairs by %ld columns are too many tiles", pairs, a.npad);
   IEN_HIP(hipGetLastError());
   return IEN_OK;
 }

@@ -12,10 +12,11 @@ namespace ien {
 namespace {
 
 template <typename T>
-void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, int size) {
+bool launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, int size) {
   a.tiles_n = (int)((a.n + T::TN - 1) / T::TN);
   a.list = (const ExpertTile *)(r->d_plan + p.tiles[size]);
   a.total = r->d_plan + p.totals + size;
+  if (!launches(p.most[size], a.tiles_n, T::THREADS)) return false;
   const dim3 grid((unsigned)(p.most[size] * a.tiles_n));
   if (a.f32)
     hipLaunchKernelGGL((k_tile8<T, true, float, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
@@ -23,14 +24,13 @@ void launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, in
     hipLaunchKernelGGL((k_tile8<T, true, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
   else
     hipLaunchKernelGGL((k_tile8<T, false, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  return true;
 }
 
 template <int WN, int WK>
-void few(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p) {
-  if (a.f32)
-    launch_few<EXPERTS_ROWS8, float, WN, WK>(ctx, a, r, p);
-  else
-    launch_few<EXPERTS_ROWS8, _Float16, WN, WK>(ctx, a, r, p);
+bool few(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p) {
+  return a.f32 ? launch_few<EXPERTS_ROWS8, float, WN, WK>(ctx, a, r, p)
+               : launch_few<EXPERTS_ROWS8, _Float16, WN, WK>(ctx, a, r, p);
 }
 
 struct CombineArgs {
@@ -146,12 +146,14 @@ ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *
   a.ksplit = 1;
   a.kchunks = w->cb;
   const long pairs = (long)(routes->tokens * routes->top);
+  bool done = false;
   switch (experts_out_choice(pairs, (long)routes->experts, a.cb)) {
-    case 0: few<4, 2>(ctx, a, routes, p); break;
-    case 1: launch<Tile8<1, 2, 2, 2, 2>>(ctx, a, routes, p, 1); break;
-    case 2: launch<Tile8<2, 2, 2, 2, 2>>(ctx, a, routes, p, 2); break;
-    default: few<2, 4>(ctx, a, routes, p); break;
+    case 0: done = few<4, 2>(ctx, a, routes, p); break;
+    case 1: done = launch<Tile8<1, 2, 2, 2, 2>>(ctx, a, routes, p, 1); break;
+    case 2: done = launch<Tile8<2, 2, 2, 2, 2>>(ctx, a, routes, p, 2); break;
+    default: done = few<2, 4>(ctx, a, routes, p); break;
   }
+  IEN_CHECK(done, IEN_ERR_INPUT, "experts_out8: %ld pairs by %ld columns are too many tiles", pairs, a.n);
   IEN_HIP(hipGetLastError());
   CombineArgs c{d_parts, a.ys, routes->d_plan + p.place, routes->d_weight, d_add, (long)add_stride, out->data,
                 (long)out->stride, (long)routes->tokens, a.n, (int)routes->top};

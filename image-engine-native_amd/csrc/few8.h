@@ -132,13 +132,18 @@ __global__ __launch_bounds__(64 * WN * WK) void k_few8(Args8 a) {
   }
 }
 
+// A launch counts its lanes in 32 bits.
+inline bool launches(long tiles_m, int tiles_n, int threads) { return tiles_m * tiles_n < (1L << 32) / threads; }
+
 template <Kind8 KIND, typename Y, int WN, int WK>
-void launch_few(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p) {
+bool launch_few(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p) {
   a.tiles_n = (int)((a.n + 16 * WN - 1) / (16 * WN));
   a.list = (const ExpertTile *)(r->d_plan + p.tiles[0]);
   a.total = r->d_plan + p.totals;
+  if (!launches(p.most[0], a.tiles_n, 64 * WN * WK)) return false;
   hipLaunchKernelGGL((k_few8<KIND, Y, WN, WK>), dim3((unsigned)(p.most[0] * a.tiles_n)), dim3(64 * WN * WK), 0,
                      ctx->stream, a);
+  return true;
 }
 
 }  // namespace

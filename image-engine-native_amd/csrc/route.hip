@@ -806,7 +806,7 @@ extern "C" {
 size_t ien_routes_order(size_t experts) { return 4 * ((experts + 4) / 4); }
 
 size_t ien_routes_ints(size_t tokens, size_t experts, size_t top) {
-  if (experts < 1 || experts > MAX_EXPERTS || top < 1 || top > MAX_TOP || tokens > MAX_PAIRS / top) return 0;
+  if (experts < 1 || experts > MAX_EXPERTS || top < 1 || top > MAX_TOP || top > experts || tokens > MAX_PAIRS / top) return 0;
   return (size_t)plan_layout(tokens, experts, top).ints;
 }
 

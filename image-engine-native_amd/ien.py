@@ -887,6 +887,8 @@ class Routes:
             if t.shape != (tokens, top) or t.dtype != dtype or not t.is_contiguous() or t.device != index.device:
                 raise ValueError(f"the experts and weights are contiguous int32 and f32 tensors of {tokens} x {top} on one device")
         plan = torch.zeros(ints, dtype=torch.int32, device=index.device)  # (zeros: a plan of no pairs)
+        if plan.is_cuda:
+            torch.cuda.current_stream(plan.device).synchronize()  # (whatever stream the context runs on)
         self.tokens, self.experts, self.top = tokens, experts, top
         self._index, self._weight, self._plan = index, weight, plan
         first = L.ien_routes_order(experts)

@@ -394,7 +394,7 @@ ien_status ien_routes_plan(ien_ctx *ctx, const ien_routes *routes);
  * weights, f32 biases; read before the call returns).  Quantised once, with a
  * scale for each 128 channels of an output, as ien_quantize8 does.  gated: n
  * is even and the outputs are n / 2, act(first half) x second half.
- * experts ceil(c / 128) under 65536, c and n under 2^22. */
+ * experts ceil(c / 128) under 65536, ceil(c / 128) n under 2^28, c and n under 2^22. */
 typedef struct ien_experts8 ien_experts8;
 ien_status ien_experts8_new(ien_ctx *ctx, const void *d_w, ien_wtype wtype, size_t experts, size_t c,
                             size_t n, int gated, const float *d_bias, ien_experts8 **out);
