@@ -66,6 +66,17 @@ __device__ __forceinline__ int bin_of(int expert, int experts) {
   return (unsigned)expert < (unsigned)experts ? expert : experts;
 }
 
+// The sum of v over lanes 0 .. this one: within rows of 16 lanes, then the last lane
+// of rows 0 and 2 (row_bcast 15) to 1 and 3, of row 1 (31) to 2 and 3.
+__device__ __forceinline__ int sums_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+
 // The offsets and each size's first tiles from the total counts, by the first
 // PLACE_LANES threads; into the plan too where `write`.
 __device__ void lay_out(const PlanArgs &a, const PlaceShared &s, bool write) {
@@ -85,11 +96,7 @@ __device__ void lay_out(const PlanArgs &a, const PlaceShared &s, bool write) {
 #pragma unroll
     for (int k = 0; k < SUMS; k++) {
       own[k] = run[k];
-#pragma unroll
-      for (int m = 1; m < 64; m *= 2) {
-        const int o = __shfl_up(run[k], m);
-        if (lane >= m) run[k] += o;
-      }
+      run[k] = sums_upto(run[k]);
       if (lane == 63) s.sums[tid / 64 * SUMS + k] = run[k];
     }
   }
