@@ -67,7 +67,7 @@ inline PlanLayout plan_layout(size_t tokens, size_t experts, size_t top) {
   return p;
 }
 
-// experts_in8.hip, experts_out8.hip: the tile of a product.
+// experts_in8.hip, experts_out8.hip: the tile of a product (gated 2: with the coarser sums).
 int experts_in_choice(int cus, long pairs, long experts, long npad, int chunks, int gated);
 int experts_out_choice(long pairs, long experts, int chunks);
 
