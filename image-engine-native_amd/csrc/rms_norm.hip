@@ -48,14 +48,16 @@ struct Raw<float> {
   typedef float8_any type;
 };
 
-// Eight channels of a row as they are; past the last one that one again.  (No branch
-// between one load and the next but for the row's end, and nothing uses them yet.)
-template <typename T>
+// Eight channels of a row as they are, past the last one anything.  EIGHTS: the row is
+// whole eights; else its end is read one by one, that last one again past it (no branch
+// between one load and the next, and nothing uses them yet).
+template <bool EIGHTS, typename T>
 __device__ __forceinline__ typename Raw<T>::type raw8(const T *row, int at, int c) {
   typename Raw<T>::type v;
+  if constexpr (EIGHTS) v = (T)0.0f;
   if (at + 8 <= c) {
     v = *(const typename Raw<T>::type *)(row + at);
-  } else {
+  } else if constexpr (!EIGHTS) {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = row[min(at + i, c - 1)];
   }
@@ -64,8 +66,9 @@ __device__ __forceinline__ typename Raw<T>::type raw8(const T *row, int at, int 
 
 // L lanes a row, N eights of channels a lane: eight n of lane l is n L + l.  gamma is
 // read first, for the rows that the workgroup takes one after another (behind them
-// 16384 x 1536 takes 50 us in place of 42).
-template <typename X, int ADD, int L, int N>
+// 16384 x 1536 takes 50 us in place of 42).  Rows of whole eights need no choice a
+// channel: with one, vector instructions were 88 % of the cycles.
+template <typename X, int ADD, int L, int N, bool EIGHTS>
 __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
   typedef std::conditional_t<ADD == ADD_F16, _Float16, float> A;
   constexpr int ROWS = 256 / L;
@@ -77,7 +80,7 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
   for (int n = 0; n < N; n++) {
     const int at = 8 * (n * L + lane);
     float8_any v = 1.0f;
-    if (a.gamma) v = raw8(a.gamma, at, c);
+    if (a.gamma) v = raw8<EIGHTS>(a.gamma, at, c);
 #pragma unroll
     for (int i = 0; i < 8; i++) g[n][i] = v[i];
   }
@@ -88,8 +91,8 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
     typename Raw<A>::type as[N];
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      xs[n] = raw8((const X *)a.x + r * a.stride, 8 * (n * L + lane), c);
-      if constexpr (ADD != NO_ADD) as[n] = raw8((const A *)a.add + r * a.add_stride, 8 * (n * L + lane), c);
+      xs[n] = raw8<EIGHTS>((const X *)a.x + r * a.stride, 8 * (n * L + lane), c);
+      if constexpr (ADD != NO_ADD) as[n] = raw8<EIGHTS>((const A *)a.add + r * a.add_stride, 8 * (n * L + lane), c);
     }
     float v[N][8];
     double squares = 0.0;
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
       for (int i = 0; i < 8; i++) {
         v[n][i] = (float)xs[n][i];
         if constexpr (ADD != NO_ADD) v[n][i] += (float)as[n][i];
-        if (8 * (n * L + lane) + i >= c) v[n][i] = 0.0f;
+        if (!EIGHTS && 8 * (n * L + lane) + i >= c) v[n][i] = 0.0f;
         squares = fma((double)v[n][i], (double)v[n][i], squares);
       }
     if constexpr (L == 16) {
@@ -116,7 +119,7 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
     }
     const float inv = (float)(1.0 / sqrt(squares / c + (double)a.eps));
     auto store = [&](auto *row, int at, const float *w) {
-      if (at + 8 <= c)
+      if (EIGHTS || at + 8 <= c)
         stream8(row + at, w);
       else
         store8<std::remove_reference_t<decltype(*row)>, false>(row, at, c, w);
@@ -124,22 +127,40 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
       const int at = 8 * (n * L + lane);
-      if (some && a.sum && at < c) store((X *)a.sum + r * a.sum_stride, at, v[n]);
+      if (a.sum && some && at < c) store((X *)a.sum + r * a.sum_stride, at, v[n]);
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[n][i] = at + i < c ? v[n][i] * inv * g[n][i] : 0.0f;
-      if (some && a.y && at < c) {
+      for (int i = 0; i < 8; i++) v[n][i] = v[n][i] * inv * g[n][i];
+      if (a.y && some && at < c) {
         if (a.y_f32)
           store((float *)a.y + r * a.y_stride, at, v[n]);
         else
           store((_Float16 *)a.y + r * a.y_stride, at, v[n]);
       }
       if (a.data) {
+        if constexpr (!EIGHTS) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[n][i] = at + i < c ? v[n][i] : 0.0f;
+        }
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, finite_magnitude(v[n][i]));
-        const int e = exponent8(max16(m));
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[n][i]));  // (a NaN is passed over)
+        if (__ballot(!finite8(m))) {  // infinities, which are NaN and no largest magnitude
+          m = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            m = fmaxf(m, finite_magnitude(v[n][i]));
+            if (!finite8(v[n][i])) v[n][i] = __uint_as_float(0x7fc00000);
+          }
+        }
+        const int e = exponent8(max16(at < c ? m : 0.0f));
+        const float unit = inverse_power(e);
+        int2v p;
+        p.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[n][0] * unit, v[n][1] * unit, 0, false);
+        p.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[n][2] * unit, v[n][3] * unit, p.x, true);
+        p.y = __builtin_amdgcn_cvt_pk_fp8_f32(v[n][4] * unit, v[n][5] * unit, 0, false);
+        p.y = __builtin_amdgcn_cvt_pk_fp8_f32(v[n][6] * unit, v[n][7] * unit, p.y, true);
         if (some && at < padded) {
-          *(int2v *)(a.data + r * a.data_stride + at) = pack8(v[n], inverse_power(e));
+          *(int2v *)(a.data + r * a.data_stride + at) = at < c ? p : int2v{};
           if (at % BLOCK8 == 0) a.scales[r * a.scale_stride + at / BLOCK8] = (uint8_t)(e + 127);
         }
       }
@@ -147,8 +168,8 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
   }
 }
 
-template <typename X, int ADD>
-void launch(ien_ctx *ctx, const RmsArgs &a) {
+template <typename X, int ADD, bool EIGHTS>
+void launch_rows(ien_ctx *ctx, const RmsArgs &a) {
   // Workgroups take rows in turns, so many of them a CU (us, 8, 16, 32 and one for every four rows: 65536 x 1024
   // 98.0, 95.9, 93.0, 93.7; 100000 x 96 16.5, 15.8, 17.6, 17.8; 4000 x 8192 57.1, 60.5, 60.2, 60.1).  A wave a row up to
   // 2048 channels: a workgroup's barriers cost more than its lanes save (16384 x 1536 42.3 and 45.8 at best).
@@ -156,13 +177,18 @@ void launch(ien_ctx *ctx, const RmsArgs &a) {
     const dim3 grid((unsigned)std::min((a.rows + rows - 1) / rows, (long)many * ctx->cus));
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, a);
   };
-  if (a.c <= 128) go(k_rms_norm<X, ADD, 16, 1>, 16, 16);
-  else if (a.c <= 512) go(k_rms_norm<X, ADD, 64, 1>, 4, 32);
-  else if (a.c <= 1024) go(k_rms_norm<X, ADD, 64, 2>, 4, 32);
-  else if (a.c <= 1536) go(k_rms_norm<X, ADD, 64, 3>, 4, 32);
-  else if (a.c <= 2048) go(k_rms_norm<X, ADD, 64, 4>, 4, 32);
-  else if (a.c <= 4096) go(k_rms_norm<X, ADD, 256, 2>, 1, 8);
-  else go(k_rms_norm<X, ADD, 256, 4>, 1, 8);
+  if (a.c <= 128) go(k_rms_norm<X, ADD, 16, 1, EIGHTS>, 16, 16);
+  else if (a.c <= 512) go(k_rms_norm<X, ADD, 64, 1, EIGHTS>, 4, 32);
+  else if (a.c <= 1024) go(k_rms_norm<X, ADD, 64, 2, EIGHTS>, 4, 32);
+  else if (a.c <= 1536) go(k_rms_norm<X, ADD, 64, 3, EIGHTS>, 4, 32);
+  else if (a.c <= 2048) go(k_rms_norm<X, ADD, 64, 4, EIGHTS>, 4, 32);
+  else if (a.c <= 4096) go(k_rms_norm<X, ADD, 256, 2, EIGHTS>, 1, 8);
+  else go(k_rms_norm<X, ADD, 256, 4, EIGHTS>, 1, 8);
+}
+
+template <typename X, int ADD>
+void launch(ien_ctx *ctx, const RmsArgs &a) {
+  a.c % 8 == 0 ? launch_rows<X, ADD, true>(ctx, a) : launch_rows<X, ADD, false>(ctx, a);
 }
 
 bool known(ien_out_type t) { return t == IEN_OUT_F16 || t == IEN_OUT_F32; }
