@@ -793,12 +793,12 @@ def conv8(ctx, x, images, height, width, matrix, out, step=1, act=ACT_NONE, add=
     _multiply8(ctx, x, (INPUT_IMAGE, images, height, width, step), row0, matrix, out, act, add, exact)
 
 
-def _channels_of(ctx, t, c):
+def _channels_of(ctx, t, c, what="gamma and beta"):
     """The address of c f32 values on the context's GPU, or None."""
     if t is None:
         return None
     if t.shape != (c,) or not t.is_cuda or not t.is_contiguous() or _out_type(t.dtype) != OUT_F32:
-        raise ValueError(f"gamma and beta are {c} contiguous f32 values on the GPU")
+        raise ValueError(f"{what} are {c} contiguous f32 values on the GPU")
     if t.get_device() != ctx.device:
         raise _elsewhere(ctx, t.device)
     return t.data_ptr()
@@ -923,7 +923,7 @@ def route(ctx, logits, routes, score=SCORE_SOFTMAX, bias=None, groups=1, kept=No
         raise _elsewhere(ctx, routes.index.device)
     if groups < 1 or group_top < 1 or (kept is not None and kept < 1):
         raise ValueError(f"{kept} of {groups} groups by their {group_top} best")
-    how = _ROUTER(score, _channels_of(ctx, bias, experts) or 0, groups, groups if kept is None else kept, group_top,
+    how = _ROUTER(score, _channels_of(ctx, bias, experts, "biases") or 0, groups, groups if kept is None else kept, group_top,
                   1 if renormalise else 0, scale)
     status = (_lib or load()).ien_route(ctx.h, at, kind, stride, how, routes._at)
     if status:

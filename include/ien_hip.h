@@ -337,7 +337,7 @@ ien_status ien_group_norm8(ien_ctx *ctx, const void *d_x, ien_out_type type, siz
  * (gamma device f32 or NULL for 1; the mean of squares in f64).  Written are,
  * where not NULL: the sum to d_sum, rows of `type` sum_stride elements apart;
  * y to d_y (f16 or f32 by y_type); and y in 8 bits to `out8`, as
- * ien_quantize8 of the f32 results.  The norm is of the f32 sum, not of what
+ * ien_quantize8 of the f32 results (a NaN may have either sign).  The norm is of the f32 sum, not of what
  * d_sum holds of it.  d_sum and d_y may each be d_x or d_add itself with its
  * type and stride. */
 ien_status ien_rms_norm(ien_ctx *ctx, const void *d_x, ien_out_type type, size_t rows, size_t c,
@@ -402,7 +402,8 @@ void ien_experts8_free(ien_experts8 *m);
 
 /* The experts' first product: for the pair at place p of the plan's order, of
  * token t and expert e, row p of `out` is act(x[t] . w[e] + bias[e]) (gated:
- * see above), in 8 bits as ien_quantize8 of the f32 results.  x: tokens rows of
+ * see above), in 8 bits as ien_quantize8 of the f32 results (a NaN may have
+ * either sign).  x: tokens rows of
  * c values, out: tokens x top rows of the outputs; rows of pairs without an
  * expert are left as they were.  Sums as in ien_multiply8, `fast` too.
  * x takes less than 2 GiB, its rows and out's are less than 1 MiB apart.

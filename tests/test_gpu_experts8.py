@@ -206,3 +206,59 @@ def test_an_unplanned_routing_does_nothing(ctx):
     assert bool((h.data == 99).all())
     torch.cuda.synchronize()
     m.free()
+
+
+@pytest.mark.parametrize("tokens,experts,top", [(3, 4, 1), (90, 3, 2), (1400, 2, 1), (5000, 2, 1)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_and_outputs_that_are_not_finite(ctx, tokens, experts, top, gated):
+    """A NaN in a token's row makes that token's rows NaN and no others; an infinite output is NaN and does not count
+    into its block's scale."""
+    import ien
+
+    rng = np.random.default_rng(tokens)
+    c, outs = 200, 300
+    n = outs * (2 if gated else 1)
+    data, scales = whole_rows(rng, tokens, c)
+    w, b = whole_weights(rng, experts, c, n), rng.integers(1, 9, (experts, n)).astype(np.float32)
+    b[:, 130] = np.inf
+    if gated:
+        w[:, :, outs + 130] = 0  # (the factor of that gate is its bias, 1 .. 8)
+    index = np.stack([(np.arange(tokens) + k) % experts for k in range(top)], 1).astype(np.int32)
+    bad = tokens // 2
+    m = ien.Experts8(ctx, w, b, gated=gated)
+    clean = hidden_rows(ctx, rows8_of(data, scales, c), index, experts, m, outs, ien.ACT_RELU)
+    v, _ = X.products(E.values(data, scales, c), index, w.astype(np.float64), np.where(np.isinf(b), 0, b).astype(np.float64), True)
+    v = X.gate(v, "relu", gated)
+    v[:, 130] = np.nan  # (infinite before its rounding)
+    want = E.quantize(v)
+    assert np.array_equal(clean[1], want[1])
+    got, ref = E.values(*clean, outs), E.values(*want, outs)
+    assert np.array_equal(np.isnan(got), np.isnan(ref)) and np.array_equal(got[~np.isnan(ref)], ref[~np.isnan(ref)])
+    broken = data.copy()
+    broken[bad, 7] = 127
+    again = hidden_rows(ctx, rows8_of(broken, scales, c), index, experts, m, outs, ien.ACT_RELU)
+    _, order = X.plan(index, experts)
+    its = order // top == bad
+    assert its.sum() == top and np.isnan(E.values(again[0][its], again[1][its], outs)).all()
+    assert np.array_equal(again[0][~its], clean[0][~its]) and np.array_equal(again[1][~its], clean[1][~its])
+    m.free()
+
+
+def test_an_expert_twice_and_far_values(ctx):
+    """The same expert in two of a token's slots; products past f16 in f32 results."""
+    import ien
+    import torch
+
+    rng = np.random.default_rng(7)
+    index = np.array([[1, 1], [0, 1], [1, 0]], np.int32)
+    v = rng.integers(-2, 3, (6, 64)).astype(np.float64) * 64
+    data, scales = E.to_bytes(np.concatenate([v, np.zeros((6, 64))], 1)), np.full((6, 1), 127, np.uint8)
+    w = whole_weights(rng, 2, 64, 24) * 4096
+    weight = np.array([[0.5, 0.25], [2, 1], [1, 4]])
+    m, routes = ien.Experts8(ctx, w), plan_of(ctx, index, weight, 2)
+    out = torch.empty(3, 24, device="cuda")
+    ien.experts_out8(ctx, rows8_of(data, scales, 64), routes, m, ien.expert_parts(routes, m, out.dtype), out)
+    y, size = X.products(v, index, w.astype(np.float64), None, False)
+    assert size.max() / (64 * 4096) < 2**24 and size.max() > 65504
+    assert np.array_equal(out.cpu().numpy(), X.combine(y, index, weight, 2).astype(np.float32))
+    m.free()
