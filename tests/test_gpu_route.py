@@ -138,3 +138,22 @@ def test_no_tokens(ctx):
 
     ien.route(ctx, torch.empty(0, 8, device="cuda"), ien.Routes(0, 8, 2))
     ien.plan_routes(ctx, ien.Routes(0, 8, 2))
+
+
+@pytest.mark.parametrize("per,many", [(16, 2), (16, 4), (16, 8), (16, 13), (16, 16), (32, 2), (32, 3), (32, 8), (64, 2), (64, 3),
+                                      (64, 4), (128, 2), (64, 7), (64, 16), (128, 5), (256, 3), (512, 2), (48, 5)])
+@pytest.mark.parametrize("softmax,biased,group_top", [(True, False, 1), (False, True, 2), (False, False, 2)])
+def test_groups_of_whole_lanes(ctx, per, many, softmax, biased, group_top):
+    """Groups of some experts of every lane, with equal ones, and with experts and whole groups that are off."""
+    rng = np.random.default_rng(per + many)
+    experts = per * many
+    logits = rng.standard_normal((90, experts)).astype(np.float32)
+    logits[:30] = rng.integers(0, 3, (30, experts))
+    logits[30:60][rng.random((30, experts)) < 0.7] = -np.inf
+    for t in range(40, 60):
+        logits[t].reshape(many, per)[rng.integers(0, many)] = np.nan
+    bias = (0.2 * rng.standard_normal(experts)).astype(np.float32) if biased else None
+    if biased:
+        bias[rng.integers(0, experts, 5)] = -np.inf
+    for kept in {1, (many + 1) // 2, many - 1}:
+        check(ctx, logits, min(8, per * kept), softmax, bias=bias, groups=many, kept=kept, group_top=group_top)
