@@ -5,8 +5,8 @@
 // experts).  What is not below the (top + 1)-th of the lanes' largest choices, 16
 // at most as a rule, is handed a lane each and ordered by counting; else the
 // largest choice is found top times.  Equal ones: the lowest index.  Vector
-// instructions bound it (95 % of the cycles): 65536 tokens, 8 of 256 experts in
-// 4 of 8 groups, take 39 us.  Without a bias choices are in the
+// instructions bound it (over 90 % of the cycles): 65536 tokens, 8 of 256 experts in
+// 4 of 8 groups, take 38 us.  Without a bias choices are in the
 // order of the logits, which are compared themselves.  With one they are f32
 // sums that are off by some steps: where two that matter (neighbours among the
 // chosen, the last chosen and the next, the last group kept and the first not)
@@ -380,10 +380,10 @@ __device__ __forceinline__ int key_of(float v) { return key_of_sum(v + 0.0f); }
 __device__ __forceinline__ float value_of(int key) { return __int_as_float(key ^ (key >> 31 & 0x7fffffff)); }
 constexpr int NO_KEY = (int)0x807fffff;  // of NONE
 
-// e^x for x <= 0 (0 below -150): the hardware's power of two of the rounded x log2(e), times what the rounding left
-// (some 2 steps of f32).
+// e^x for x <= 88 (0 below -150, e^88 past 88): the hardware's power of two of the rounded x log2(e), times what the
+// rounding left (some 2 steps of f32).
 __device__ __forceinline__ float exp_f(float x) {
-  x = __builtin_amdgcn_fmed3f(x, -150.0f, 0.0f);
+  x = __builtin_amdgcn_fmed3f(x, -150.0f, 88.0f);
   const float hi = x * 1.44269502f, lo = fmaf(x, 1.44269502f, -hi) + x * 1.92596303e-8f;
   const float r = __builtin_amdgcn_exp2f(hi);
   return fmaf(r * lo, 0.693147181f, r);
@@ -520,8 +520,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   constexpr int LANES = route_lanes(L), TOKENS = LANES / L;
   extern __shared__ int lds[];
   constexpr int LISTS = L == 16 ? TOKENS * 16 : 1;
-  __shared__ int keys[LISTS], experts_of[LISTS];  // of a token's candidates
-  __shared__ float scores[LISTS];
+  __shared__ int candidates[3 * LISTS];  // the keys of a token's, their scores, their experts
   __shared__ int taken_tokens;
   __shared__ float biases[L * V];
   const int experts = a.plan.experts, top = a.plan.top, n = experts + 1;
@@ -576,13 +575,13 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       s[i] = s[i] > NONE ? s[i] : NONE;  // (NaN too)
       most = max(most, __float_as_uint(s[i]));
     }
-    if (a.softmax || a.by_logit) {
-#pragma unroll
-      for (int i = 0; i < V; i++) c[i] = key_of(s[i]);
-    }
     if (!a.by_logit && __ballot(most == __float_as_uint(NONE))) {  // (it is the last of them as an integer)
 #pragma unroll
       for (int i = 0; i < V; i++) gone |= (s[i] == NONE ? 1u : 0u) << i;
+    }
+    if (a.softmax || a.by_logit) {
+#pragma unroll
+      for (int i = 0; i < V; i++) c[i] = key_of(s[i]);
     }
     // How far a score may be off, in halves of a step of 1: of a logistic function 4 of its exponential, at most
     // a quarter of which reaches it, a step of the reciprocal and two roundings; of a softmax 0.4 of the argument
@@ -608,8 +607,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float e = exp_f(-fabsf(s[i]));
-        s[i] = (s[i] < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
+        s[i] = __builtin_amdgcn_rcpf(1.0f + exp_f(-s[i]));  // (under 1e-30, also where it is less than that still)
       }
     }
     if (a.bias) {
@@ -730,20 +728,19 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, true);
       upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, true);
       if (top < 16 && !__ballot(upto > 16)) {
-        const int first = slot * 16;
-        keys[first + lane] = NO_KEY;
-        experts_of[first + lane] = (int)MAX_EXPERTS + lane;
+        int *const first = candidates + slot * 16, *at = first + upto - own;
+        first[lane] = NO_KEY;
+        first[lane + 2 * LISTS] = (int)MAX_EXPERTS + lane;
         wave_fence();
-        int at = first + upto - own;
 #pragma unroll
         for (int i = 0; i < V; i++)
           if (c[i] >= from) {
-            keys[at] = c[i], scores[at] = s[i], experts_of[at] = lane + L * i;
+            at[0] = c[i], at[LISTS] = __float_as_int(s[i]), at[2 * LISTS] = lane + L * i;
             at++;
           }
         wave_fence();
-        const int key = keys[first + lane], expert = experts_of[first + lane];
-        const float its = scores[first + lane];  // (past the candidates: not used)
+        const int key = first[lane], expert = first[lane + 2 * LISTS];
+        const float its = __int_as_float(first[lane + LISTS]);  // (past the candidates: not used)
         const long mine = ordered(key, expert);
         place = 0;
         round_lanes([&](auto other) { place += other(mine) > mine; });
@@ -751,9 +748,9 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
         if (taken) chosen = expert, score = its;
         if (!a.by_logit) {  // (in their order each is compared with the next one)
           wave_fence();
-          keys[first + place] = key;
+          first[place] = key;
           wave_fence();
-          const int close = taken && value_of(key) - value_of(keys[first + place + 1]) < near;
+          const int close = taken && value_of(key) - value_of(first[place + 1]) < near;
           unclear = unclear || largest<L>(close);
         }
         total = group_sum<L>(score);
