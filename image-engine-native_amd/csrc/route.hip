@@ -6,7 +6,7 @@
 // at most as a rule, is handed a lane each and ordered by counting; else the
 // largest choice is found top times.  Equal ones: the lowest index.  Vector
 // instructions bound it (over 90 % of the cycles): 65536 tokens, 8 of 256 experts in
-// 4 of 8 groups, take 38 us.  Without a bias choices are in the
+// 4 of 8 groups, take 39 us.  Without a bias choices are in the
 // order of the logits, which are compared themselves.  With one they are f32
 // sums that are off by some steps: where two that matter (neighbours among the
 // chosen, the last chosen and the next, the last group kept and the first not)
@@ -426,9 +426,8 @@ __device__ __forceinline__ void wave_fence() {
 // One token's choice in f64 by a whole wave, V experts a lane: lane k's is slot k's
 // expert and weight.  by_logit: the weights of the experts that lanes hold in `chosen`.
 template <typename X, int V>
-__device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, double *ranks, int &chosen, float &weight) {
+__device__ __forceinline__ void choose_f64(const RouteArgs &a, const X *row, double *ranks, int lane, int &chosen, float &weight) {
   constexpr int L = 64;
-  const int lane = threadIdx.x & 63;
   const int experts = a.plan.experts, top = a.plan.top;
   const double none = -__builtin_inf();
   auto logit = [&](int e) {
@@ -521,11 +520,11 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   extern __shared__ int lds[];
   constexpr int LISTS = L == 16 ? TOKENS * 16 : 1;
   __shared__ int candidates[3 * LISTS];  // the keys of a token's, their scores, their experts
+  __shared__ int boards[TOKENS * (L * V + 16)];  // a token's keys (16 more: a wave's four then write to different banks)
   __shared__ int taken_tokens;
-  __shared__ float biases[L * V];
+  __shared__ float biases[L * V], size_shared;
   const int experts = a.plan.experts, top = a.plan.top, n = experts + 1;
-  int lane = threadIdx.x % L;
-  const int slot = threadIdx.x / L;
+  int tid = threadIdx.x;
   int *bins = lds;                                      // the chunk's counts; ONE: its pairs' experts
   const int held = ONE ? 64 * top : (int)a.plan.at.pitch;  // (whole fours)
   float *ranks = (float *)(lds + held);                   // [token][groups]; f64 of one token a wave
@@ -541,16 +540,24 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const float b = fabsf(biases[lane + L * i]);
+    const float b = fabsf(biases[tid % L + L * i]);
     if (b < __builtin_inff()) size_key = max(size_key, key_of(1.0f + b));
   }
-  const float choice_size = value_of(largest<L>(size_key));
+  const float size_kept = value_of(largest<L>(size_key));  // (the same in all lanes)
+  if constexpr (V == 16) {  // (no register is left for it)
+    if (tid == 0) size_shared = size_kept;
+    __syncthreads();
+  }
   const long begin = (long)blockIdx.x * a.plan.at.chunk, end = min(begin + a.plan.at.chunk, a.plan.tokens);
   for (;;) {
-    asm volatile("" : "+v"(lane));  // (what follows from it is cheaper to compute again than to keep: 48 registers too many)
+    // (What follows from it is cheaper to compute again than to keep: 48 registers too many.)
+    if constexpr (V == 16) asm volatile("" : "+v"(tid));
+    int lane = tid % L;
+    if constexpr (V < 16) asm volatile("" : "+v"(lane));
+    const int slot = tid / L;
     // The next of the chunk's tokens that no wave has (a wave may be held up by a choice in f64).
     int next = 0;
-    if ((threadIdx.x & 63) == 0) next = atomicAdd(&taken_tokens, 64 / L);
+    if ((tid & 63) == 0) next = atomicAdd(&taken_tokens, 64 / L);
     const long t0 = begin + __builtin_amdgcn_readfirstlane(next);
     if (t0 >= end) break;
     const long t = min(t0 + slot % (64 / L), end - 1);
@@ -623,6 +630,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     }
     // Two choices that are nearer than this may be in the other order (each is off by its score's error and its own
     // rounding), and two ranks that are nearer than twice this and their own roundings.
+    const float choice_size = V == 16 ? size_shared : size_kept;
     const float near = 0x1p-23f * (off + choice_size), near_ranks = 2.0f * near + 0x1p-22f * choice_size;
     bool unclear = false;
     if (a.kept < a.groups) {
@@ -671,32 +679,60 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       } else if (V >= 16 && per == 8 * L) {
         if constexpr (V >= 16) in_lanes(std::integral_constant<int, 8>{});
       } else {
-        int *mine = (int *)ranks + (L == 16 ? 1 : 2) * slot * a.groups;
-        for (int g = 0; g < a.groups; g++) {
-          int best = NO_KEY, next = NO_KEY;
+        // Through LDS: a group's experts are read by `share` lanes beside each other (65536 tokens, with their plan: 32
+        // groups of 8 experts 88 us, 10 of 20 66; every group looked for among all lanes' experts 157 and 82).
+        int *mine = (int *)ranks + (L == 16 ? 1 : 2) * slot * a.groups, *board = boards + slot * (L * V + 16);
 #pragma unroll
-          for (int i = 0; i < V; i++) {
-            const int v = (lane + L * i) * a.magic >> 22 == (unsigned)g ? c[i] : NO_KEY;
+        for (int i = 0; i < V; i++) board[lane + L * i] = c[i];
+        wave_fence();
+        const int share_bits = max(0, (L == 16 ? 4 : 6) - (32 - __clz(a.groups - 1))), share = 1 << share_bits;
+        const int part = lane & (share - 1), group = lane >> share_bits;
+        auto rank_in = [&](int g) {
+          int best = NO_KEY, next = NO_KEY;
+          for (int e = g < a.groups ? part : per; e < per; e += share) {
+            const int v = board[g * per + e];
             next = max(next, min(best, v));
             best = max(best, v);
           }
-          over_lanes<L>([&](auto other) { merge(best, next, other(best), other(next)); });
-          const int rank = rank_of(best, next);
-          if (lane == 0) mine[g] = rank;
-        }
-        wave_fence();
-        unsigned long long keep = 0;  // of this lane's groups lane + L j
-        for (int j = 0; lane + L * j < a.groups; j++) {
-          const int rank = mine[lane + L * j];
+          int steps = share_bits;
+          over_lanes<L>([&](auto other) {
+            if (steps-- > 0) merge(best, next, other(best), other(next));
+          });
+          return rank_of(best, next);
+        };
+        if (a.groups <= L) {
+          const int own = rank_in(group);
+          const bool its = part == 0 && group < a.groups;
           int ahead = 0;
-          for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
-          if (ahead < a.kept)
-            keep |= 1ull << j, low = min(low, rank);
-          else
-            high = max(high, rank);
+          if constexpr (L == 16) {
+            const long rank = its ? ordered(own, group) : (long)(1ull << 63);
+            round_lanes([&](auto other) { ahead += other(rank) > rank; });
+          } else {
+            for (int g = 0; g < a.groups; g++) {
+              const int rank = __shfl(own, g << share_bits);
+              ahead += rank > own || (rank == own && g < group);
+            }
+          }
+          if (its) {
+            (ahead < a.kept ? low : high) = own;
+            mine[group] = ahead < a.kept;
+          }
+        } else {
+          for (int g = lane; g < a.groups; g += L) mine[g] = rank_in(g);
+          wave_fence();
+          unsigned long long keep = 0;  // of this lane's groups lane + L j
+          for (int j = 0; lane + L * j < a.groups; j++) {
+            const int rank = mine[lane + L * j];
+            int ahead = 0;
+            for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
+            if (ahead < a.kept)
+              keep |= 1ull << j, low = min(low, rank);
+            else
+              high = max(high, rank);
+          }
+          wave_fence();
+          for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = (int)(keep >> j & 1);
         }
-        wave_fence();
-        for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = (int)(keep >> j & 1);
         wave_fence();
 #pragma unroll
         for (int i = 0; i < V; i++)
@@ -796,7 +832,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
       int c64 = mine ? chosen : -1;
       float w64;
       choose_f64<X, (L * V + 63) / 64>(a, (const X *)a.logits + there * a.stride,
-                                       (double *)(ranks + (L == 16 ? slot / 4 * 4 : 2 * slot) * a.groups), c64, w64);
+                                       (double *)(ranks + (L == 16 ? slot / 4 * 4 : 2 * slot) * a.groups), tid & 63, c64, w64);
       if (!a.by_logit) {
         c64 = __shfl(c64, lane);
         w64 = __shfl(w64, lane);
