@@ -157,3 +157,16 @@ def test_groups_of_whole_lanes(ctx, per, many, softmax, biased, group_top):
         bias[rng.integers(0, experts, 5)] = -np.inf
     for kept in {1, (many + 1) // 2, many - 1}:
         check(ctx, logits, min(8, per * kept), softmax, bias=bias, groups=many, kept=kept, group_top=group_top)
+
+
+@pytest.mark.parametrize("tokens", [1, 64, 65])
+@pytest.mark.parametrize("experts,groups", [(16, 8), (60, 30), (128, 128), (256, 256), (250, 125), (1024, 1024), (1000, 40), (999, 3)])
+def test_many_groups_in_one_launch_and_in_two(ctx, tokens, experts, groups):
+    """The most that a workgroup keeps: a rank a group and, of one chunk, its pairs."""
+    rng = np.random.default_rng(tokens + groups)
+    logits = rng.standard_normal((tokens, experts)).astype(np.float32)
+    bias = (0.2 * rng.standard_normal(experts)).astype(np.float32)
+    per = experts // groups
+    for kept in {1, groups // 2, groups - 1}:
+        check(ctx, logits, min(16, per * kept), False, bias=bias, groups=groups, kept=kept, group_top=2)
+        check(ctx, np.round(logits), min(16, per * kept), True, groups=groups, kept=kept)
