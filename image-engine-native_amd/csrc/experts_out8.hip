@@ -5,6 +5,7 @@
 // takes the slots in order: what arrives first decides nothing.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "few8.h"
 
@@ -18,12 +19,11 @@ bool launch(ien_ctx *ctx, Args8 &a, const ien_routes *r, const PlanLayout &p, in
   a.total = r->d_plan + p.totals + size;
   if (!launches(p.most[size], a.tiles_n, T::THREADS)) return false;
   const dim3 grid((unsigned)(p.most[size] * a.tiles_n));
-  if (a.f32)
-    hipLaunchKernelGGL((k_tile8<T, true, float, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
-  else if (a.exact)
-    hipLaunchKernelGGL((k_tile8<T, true, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(T::THREADS), 0, ctx->stream, a); };
+  if (a.exact)
+    a.f32 ? go(k_tile8<T, true, float, EXPERTS_ROWS8>) : go(k_tile8<T, true, _Float16, EXPERTS_ROWS8>);
   else
-    hipLaunchKernelGGL((k_tile8<T, false, _Float16, EXPERTS_ROWS8>), grid, dim3(T::THREADS), 0, ctx->stream, a);
+    a.f32 ? go(k_tile8<T, false, float, EXPERTS_ROWS8>) : go(k_tile8<T, false, _Float16, EXPERTS_ROWS8>);
   return true;
 }
 
@@ -38,16 +38,20 @@ struct CombineArgs {
   long pitch;
   const int *place;
   const float *weight;
-  const void *add;
+  const void *add;  // of the result's type
   long as;
+  const void *branch;
+  long bs;
+  int branch_f32;
   void *y;
   long ys;
   long tokens, n;
   int top;
 };
 
-// A lane eight outputs of a token; rows of parts are whole eights.
-template <typename Y>
+// A lane eight outputs of a token (Y) from rows of parts (P), which are whole eights.  All
+// sums are in f32: an f16 result of f32 parts is rounded once.
+template <typename Y, typename P>
 __global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
   const long eights = (a.n + 7) / 8, total = a.tokens * eights;
   for (long item = (long)blockIdx.x * 256 + threadIdx.x; item < total; item += (long)gridDim.x * 256) {
@@ -59,18 +63,20 @@ __global__ __launch_bounds__(256) void k_combine(CombineArgs a) {
       if (place < 0) continue;
       const float w = a.weight[t * a.top + k];
       float part[8];
-      load8<Y, true>((const Y *)a.parts + place * a.pitch, at, 0, part);
+      load8<P, true>((const P *)a.parts + place * a.pitch, at, 0, part);
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = fmaf(w, part[i], v[i]);
     }
-    if (a.add) {
-      float old[8];
-      if (whole)
-        load8<Y, true>((const Y *)a.add + t * a.as, at, 0, old);
-      else
-        load8<Y, false>((const Y *)a.add + t * a.as, at, a.n, old);
+    if (a.add || a.branch) {
+      float old[8] = {}, branch[8] = {};
+      auto load = [&](auto *row, float *v) {
+        typedef std::remove_cv_t<std::remove_pointer_t<decltype(row)>> T;
+        whole ? load8<T, true>(row, at, 0, v) : load8<T, false>(row, at, a.n, v);
+      };
+      if (a.add) load((const Y *)a.add + t * a.as, old);
+      if (a.branch) a.branch_f32 ? load((const float *)a.branch + t * a.bs, branch) : load((const _Float16 *)a.branch + t * a.bs, branch);
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] += old[i];
+      for (int i = 0; i < 8; i++) v[i] += old[i] + branch[i];
     }
     Y *y = (Y *)a.y + t * a.ys;
     if (whole)
@@ -108,9 +114,20 @@ size_t ien_experts_parts(const ien_routes *routes, const ien_experts8 *w) {
 
 ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *routes, const ien_experts8 *w,
                             int fast, void *d_parts, const void *d_add, size_t add_stride, const ien_output *out) {
+  IEN_CHECK(out, IEN_ERR_INPUT, "null argument");
+  return ien_experts_out8_ex(ctx, h, routes, w, fast, d_parts, out->type, d_add, add_stride, nullptr, out->type, 0, out);
+}
+
+ien_status ien_experts_out8_ex(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *routes, const ien_experts8 *w,
+                               int fast, void *d_parts, ien_out_type parts_type, const void *d_add, size_t add_stride,
+                               const void *d_branch, ien_out_type branch_type, size_t branch_stride,
+                               const ien_output *out) {
   IEN_CHECK(ctx && w && w->d_w && out, IEN_ERR_INPUT, "null argument");
   IEN_CHECK(!w->gated, IEN_ERR_INPUT, "experts_out8 takes no gated weights");
-  IEN_CHECK(out->type == IEN_OUT_F16 || out->type == IEN_OUT_F32, IEN_ERR_INPUT, "type %d", (int)out->type);
+  IEN_CHECK((out->type == IEN_OUT_F16 || out->type == IEN_OUT_F32) && (parts_type == IEN_OUT_F32 || parts_type == out->type) &&
+                (!d_branch || branch_type == IEN_OUT_F16 || branch_type == IEN_OUT_F32),
+            IEN_ERR_INPUT, "type %d from products of type %d, with a branch of type %d", (int)out->type, (int)parts_type,
+            (int)branch_type);
   IEN_CHECK(out->layout == IEN_LAYOUT_NHWC, IEN_ERR_INPUT, "experts_out8 writes NHWC rows");
   ien_status s = check_routes(routes, "experts_out8");
   if (s != IEN_OK) return s;
@@ -118,8 +135,9 @@ ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *
   if (routes->tokens == 0) return IEN_OK;
   s = check_rows8(h, w->c, "experts_out8");
   if (s != IEN_OK) return s;
-  IEN_CHECK(out->data && out->stride >= w->n && (!d_add || add_stride >= w->n), IEN_ERR_INPUT,
-            "no output, or rows %zu and %zu apart for n = %zu", out->stride, add_stride, w->n);
+  IEN_CHECK(out->data && out->stride >= w->n && (!d_add || add_stride >= w->n) && (!d_branch || branch_stride >= w->n),
+            IEN_ERR_INPUT, "no output, or rows %zu, %zu and %zu apart for n = %zu", out->stride, add_stride, branch_stride,
+            w->n);
   IEN_CHECK(d_parts && ((uintptr_t)d_parts & 15) == 0, IEN_ERR_INPUT, "experts_out8: no parts, or unaligned");
   IEN_CHECK(h->stride < (1u << 20) && h->scale_stride < (1u << 20), IEN_ERR_INPUT,
             "experts_out8: rows in 8 bits %zu and %zu bytes apart", h->stride, h->scale_stride);
@@ -140,8 +158,8 @@ ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *
   a.npad = w->npad;
   a.y = d_parts;
   a.ys = (long)((w->n + 7) / 8 * 8);
-  a.f32 = out->type == IEN_OUT_F32;
-  a.exact = a.f32 || !fast;
+  a.f32 = parts_type == IEN_OUT_F32;
+  a.exact = out->type == IEN_OUT_F32 || !fast;
   a.act = IEN_ACT_NONE;
   a.ksplit = 1;
   a.kchunks = w->cb;
@@ -155,14 +173,16 @@ ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *
   }
   IEN_CHECK(done, IEN_ERR_INPUT, "experts_out8: %ld pairs by %ld columns are too many tiles", pairs, a.n);
   IEN_HIP(hipGetLastError());
-  CombineArgs c{d_parts, a.ys, routes->d_plan + p.place, routes->d_weight, d_add, (long)add_stride, out->data,
-                (long)out->stride, (long)routes->tokens, a.n, (int)routes->top};
+  CombineArgs c{d_parts, a.ys, routes->d_plan + p.place, routes->d_weight, d_add, (long)add_stride, d_branch,
+                (long)branch_stride, branch_type == IEN_OUT_F32, out->data, (long)out->stride, (long)routes->tokens, a.n,
+                (int)routes->top};
   const long items = c.tokens * ((c.n + 7) / 8);
   const dim3 grid((unsigned)std::min((items + 255) / 256, 1L << 20));
-  if (a.f32)
-    hipLaunchKernelGGL(k_combine<float>, grid, dim3(256), 0, ctx->stream, c);
+  auto combine = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, c); };
+  if (out->type == IEN_OUT_F32)
+    combine(k_combine<float, float>);
   else
-    hipLaunchKernelGGL(k_combine<_Float16>, grid, dim3(256), 0, ctx->stream, c);
+    a.f32 ? combine(k_combine<_Float16, float>) : combine(k_combine<_Float16, _Float16>);
   IEN_HIP(hipGetLastError());
   return IEN_OK;
 }

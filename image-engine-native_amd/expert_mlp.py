@@ -60,13 +60,14 @@ class ExpertMlp8:
                                ien.Rows8(tokens, self.c, device=x.device),
                                torch.empty(tokens, self.router.n, dtype=torch.float32, device=x.device), routes,
                                ien.Rows8(tokens * self.top, self.first.n, device=x.device),
-                               ien.expert_parts(routes, self.second, x.dtype))
+                               ien.expert_parts(routes, self.second, torch.float32))
         norm, q, logits, routes, hidden, parts = self._work[key]
-        ien.rms_norm(self.ctx, x, self.gamma, norm[:, :self.c], q, add=add, total=out, eps=self.eps)
+        ien.rms_norm(self.ctx, x, self.gamma, norm[:, :self.c], q, add=add, eps=self.eps)
         ien.multiply_ex(self.ctx, ien.rows_input(norm, self.router.k), 0, tokens, self.router, logits, self.router.n, out_f32=True)
         ien.route(self.ctx, logits, routes, **self.how)
         ien.experts_in8(self.ctx, q, routes, self.first, hidden, act=self.act)
-        ien.experts_out8(self.ctx, hidden, routes, self.second, parts, out, add=out)
+        # (The two addends again, not their sum as x's type: an f16 stream is rounded once.)
+        ien.experts_out8(self.ctx, hidden, routes, self.second, parts, out, add=x, branch=add)
         return out
 
     def free(self):

@@ -48,6 +48,7 @@ EXPORTS = (
     "ien_matrix8_free", "ien_multiply8", "ien_group_norm", "ien_group_norm8",
     "ien_rms_norm", "ien_routes_ints", "ien_routes_order", "ien_route", "ien_routes_plan", "ien_experts8_new",
     "ien_experts8_free", "ien_experts_in8", "ien_experts_parts", "ien_experts_out8",
+    "ien_experts_out8_ex",
 )
 
 
@@ -258,6 +259,7 @@ def load():
         L.ien_experts_parts.argtypes = [vp, vp]
         L.ien_experts_parts.restype = sz
         L.ien_experts_out8.argtypes = [vp, vp, vp, vp, i, vp, vp, sz, vp]
+        L.ien_experts_out8_ex.argtypes = [vp, vp, vp, vp, i, vp, i, vp, sz, vp, i, sz, vp]
         for name in EXPORTS:
             getattr(L, name)
         _lib = L
@@ -996,31 +998,39 @@ def experts_in8(ctx, x, routes, matrix, out, act=ACT_NONE, exact=True):
 
 
 def expert_parts(routes, matrix, dtype):
-    """What experts_out8 writes its products to, of the result's type."""
+    """What experts_out8 writes its products to: of the result's type, or f32."""
     import torch
 
     return torch.empty(load().ien_experts_parts(routes._at, matrix.h), dtype=dtype, device=routes.index.device)
 
 
-def experts_out8(ctx, h, routes, matrix, parts, out, add=None, exact=True):
-    """out (tokens x n, f16 or f32) = add + each token's sum of weight x (h . w +
-    bias) over its pairs' rows of the Rows8 h (as experts_in8 leaves them);
-    `add` like out, or out itself; parts: expert_parts(routes, matrix, out's type)."""
+def experts_out8(ctx, h, routes, matrix, parts, out, add=None, exact=True, branch=None):
+    """out (tokens x n, f16 or f32) = (add + branch) + each token's sum of weight x
+    (h . w + bias) over its pairs' rows of the Rows8 h (as experts_in8 leaves
+    them); `add` like out, or out itself; `branch` f16 or f32, or out itself;
+    parts: expert_parts(routes, matrix, out's type or f32).  Products are rounded
+    to the parts' type (in f16 those past 65504 are infinite), sums are in f32."""
     _experts_of(ctx, h, routes.tokens * routes.top, routes, matrix)
     rows, n, at, kind, stride = _rows_of(ctx, out)
     if rows != routes.tokens or n != matrix.n:
         raise ValueError(f"{routes.tokens} rows of {matrix.n} into {tuple(out.shape)}")
-    if parts.dtype != out.dtype or not parts.is_contiguous() or parts.get_device() != ctx.device \
-            or parts.numel() < rows * routes.top * (-(-n // 8) * 8):
-        raise ValueError("parts are what expert_parts makes for the result's type")
-    add_at = None
-    add_stride = 0
+    if not parts.is_contiguous() or parts.get_device() != ctx.device or parts.numel() < rows * routes.top * (-(-n // 8) * 8) \
+            or _out_type(parts.dtype) not in (kind, OUT_F32):
+        raise ValueError("parts are what expert_parts makes for the result's type or f32")
+    add_at = branch_at = None
+    add_stride = branch_stride = 0
+    branch_kind = kind
     if add is not None:
         add_rows, add_n, add_at, add_kind, add_stride = _rows_of(ctx, add)
         if add_rows != rows or add_n != n or add_kind != kind:
             raise ValueError("what is added has the output's shape and type")
-    status = (_lib or load()).ien_experts_out8(ctx.h, h._at, routes._at, matrix.h, 0 if exact else 1, parts.data_ptr(),
-                                               add_at, add_stride, _OUTPUT(at, stride, NHWC, kind))
+    if branch is not None:
+        add_rows, add_n, branch_at, branch_kind, branch_stride = _rows_of(ctx, branch)
+        if add_rows != rows or add_n != n:
+            raise ValueError("the branch has the output's shape")
+    status = (_lib or load()).ien_experts_out8_ex(ctx.h, h._at, routes._at, matrix.h, 0 if exact else 1, parts.data_ptr(),
+                                                  _out_type(parts.dtype), add_at, add_stride, branch_at, branch_kind,
+                                                  branch_stride, _OUTPUT(at, stride, NHWC, kind))
     if status:
         check(status)
 

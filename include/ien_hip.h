@@ -423,6 +423,17 @@ ien_status ien_experts_out8(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *
                             const ien_experts8 *w, int fast, void *d_parts, const void *d_add,
                             size_t add_stride, const ien_output *out);
 
+/* The same with the pairs' products in f32 for an f16 result too (parts_type
+ * F32: as many values, of f32), and with a second addend: rows of a branch
+ * (or NULL; f16 or f32), y[t] = (add[t] + branch[t]) + the sum, all of it in
+ * f32.  A result of f32 products is rounded once.  The branch may be
+ * out->data itself with its type and stride. */
+ien_status ien_experts_out8_ex(ien_ctx *ctx, const ien_rows8 *h, const ien_routes *routes,
+                               const ien_experts8 *w, int fast, void *d_parts,
+                               ien_out_type parts_type, const void *d_add, size_t add_stride,
+                               const void *d_branch, ien_out_type branch_type,
+                               size_t branch_stride, const ien_output *out);
+
 /* ---- resampling and padding ------------------------------------------- */
 
 /* birefnet-native decoder.rs:436-522 resize: bilinear with aligned corners
