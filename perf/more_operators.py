@@ -323,7 +323,7 @@ def prepare(case, seed):
             s["logits"] = _logits(g, tokens, experts)
             s["offset"] = 0.1 * torch.randn(experts, generator=g, device=DEVICE)
             if own:
-                s["sum"], s["q"] = torch.empty_like(s["x"]), _ien().Rows8(tokens, c)
+                s["q"] = _ien().Rows8(tokens, c)
                 s["routes"] = _ien().Routes(tokens, experts, top)
         else:
             rows, k = (tokens, c) if kind == "in8" else (tokens * top, hidden)
@@ -342,7 +342,7 @@ def prepare(case, seed):
         if own and kind == "in8":
             s["y"] = torch.empty(tokens * top, hidden, dtype=dtype, device=DEVICE)
         elif own:
-            s["parts"] = _ien().expert_parts(s["routes"], s["second"]["matrix"], dtype)
+            s["parts"] = _ien().expert_parts(s["routes"], s["second"]["matrix"], torch.float32)
             s["y"] = _held(torch.zeros(tokens, c, device=DEVICE), case.get("extra", 0), dtype)
     return s
 
@@ -378,10 +378,10 @@ def _run_own(s):
     elif kind == "out8":
         ien.experts_out8(ctx, s["q"], s["routes"], s["second"]["matrix"], s["parts"], s["y"], add=s["residual"])
     else:
-        ien.rms_norm(ctx, s["x"], s["gamma"], None, s["q"], add=s["branch"], total=s["sum"], eps=EPS)
+        ien.rms_norm(ctx, s["x"], s["gamma"], None, s["q"], add=s["branch"], eps=EPS)
         ien.route(ctx, s["logits"], s["routes"], **_how(s))
         ien.experts_in8(ctx, s["q"], s["routes"], s["first"]["matrix"], s["h"], act=acts[s["act"]])
-        ien.experts_out8(ctx, s["h"], s["routes"], s["second"]["matrix"], s["parts"], s["y"], add=s["sum"])
+        ien.experts_out8(ctx, s["h"], s["routes"], s["second"]["matrix"], s["parts"], s["y"], add=s["x"], branch=s["branch"])
     return s["y"]
 
 
