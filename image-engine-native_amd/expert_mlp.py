@@ -49,8 +49,8 @@ class ExpertMlp8:
         too)."""
         import torch
 
-        tokens = x.shape[0]
-        out = torch.empty_like(x) if out is None else out
+        tokens, made = x.shape[0], out is None
+        out = torch.empty_like(x) if made else out
         if tokens == 0:
             return out
         key = tokens, x.dtype
@@ -61,6 +61,9 @@ class ExpertMlp8:
                                torch.empty(tokens, self.router.n, dtype=torch.float32, device=x.device), routes,
                                ien.Rows8(tokens * self.top, self.first.n, device=x.device),
                                ien.expert_parts(routes, self.second, torch.float32))
+            made = True
+        if made:
+            ien.settle(self.ctx)
         norm, q, logits, routes, hidden, parts = self._work[key]
         ien.rms_norm(self.ctx, x, self.gamma, norm[:, :self.c], q, add=add, eps=self.eps)
         ien.multiply_ex(self.ctx, ien.rows_input(norm, self.router.k), 0, tokens, self.router, logits, self.router.n, out_f32=True)

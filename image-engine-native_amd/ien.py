@@ -316,6 +316,17 @@ class Context:
         check(load().ien_sync(self.h))
 
 
+def settle(ctx):
+    """Waits for torch's current stream unless it is the context's: of a tensor that
+    torch has just made, fills and what lay in its memory before may be under way
+    there, and the context's launches do not follow them."""
+    import torch
+
+    stream = torch.cuda.current_stream(ctx.device)
+    if stream.cuda_stream != load().ien_stream(ctx.h):
+        stream.synchronize()
+
+
 class Matrix:
     """gemm.rs Matrix::new: host weights k x n (numpy f32 or f16) + bias."""
 
