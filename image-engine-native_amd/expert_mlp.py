@@ -49,6 +49,8 @@ class ExpertMlp8:
         too)."""
         import torch
 
+        if x.dim() != 2 or x.shape[1] != self.c or x.get_device() != self.ctx.device:  # (before anything is kept for its size)
+            raise ValueError(f"rows of {self.c} channels on GPU {self.ctx.device} expected, not {tuple(x.shape)} on {x.device}")
         tokens, made = x.shape[0], out is None
         out = torch.empty_like(x) if made else out
         if tokens == 0:

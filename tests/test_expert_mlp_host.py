@@ -40,13 +40,24 @@ def seen(monkeypatch):
     return seen
 
 
+class OnGpu(torch.Tensor):
+    """A host tensor that says it is on GPU 0."""
+
+    def get_device(self):
+        return 0
+
+
+def rows(tokens, c=24):
+    return torch.zeros(tokens, c, dtype=torch.float16).as_subclass(OnGpu)
+
+
 def block(c=24):
     return expert_mlp.ExpertMlp8(CTX, c, 2, None, (torch.zeros(c, 4).numpy(), None), (4, c, 64), (4, 32, c))
 
 
 def test_nothing_made_is_used_before_torchs_stream_is_done_with_it(seen):
     """The first run of a size, a later one with a new result, and one that makes nothing."""
-    b, x = block(), torch.zeros(6, 24, dtype=torch.float16)
+    b, x = block(), rows(6)
     for out, makes in ((x, True), (None, True), (x, False)):
         seen.clear()
         b.run(x, out=out)
@@ -56,3 +67,15 @@ def test_nothing_made_is_used_before_torchs_stream_is_done_with_it(seen):
             assert "wait" in seen[last:seen.index("call")], seen
         else:
             assert "wait" not in seen
+
+
+def test_what_is_refused_leaves_nothing(seen):
+    """Rows that are not on the context's GPU, or not the block's: nothing of theirs is kept, and the same number of tokens
+    runs afterwards."""
+    b = block()
+    for x in (torch.zeros(6, 24, dtype=torch.float16), rows(6, 23), rows(6)[0], rows(6)[:, None]):
+        with pytest.raises(ValueError):
+            b.run(x)
+        assert not b._work and "call" not in seen
+    b.run(rows(6))
+    assert list(b._work) == [(6, torch.float16)] and "call" in seen
