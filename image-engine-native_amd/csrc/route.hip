@@ -635,8 +635,11 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
     bool unclear = false;
     if (a.kept < a.groups) {
       const int per = experts / a.groups;
+      // Of two choices half their sum, which f32 always holds (two of its lowest values sum to what is no expert's).
       auto rank_of = [&](int best, int next) {
-        return a.group_top == 2 && next > NO_KEY ? key_of(value_of(best) + value_of(next)) : best;
+        if (a.group_top == 1) return best;
+        const float half = 0.5f * value_of(best);
+        return key_of(next > NO_KEY ? half + 0.5f * value_of(next) : half);
       };
       int low = 0x7fffffff, high = NO_KEY;  // the last group kept, the first one not
       // A group is OF of every lane's experts, one after another: G groups, the last of them of no expert perhaps.
@@ -740,7 +743,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
         wave_fence();
       }
       low = least<L>(low), high = largest<L>(high);
-      unclear = high > NO_KEY && value_of(low) - value_of(high) < near_ranks;
+      unclear = high > NO_KEY && value_of(low) - value_of(high) < (a.group_top == 1 ? 1.0f : 0.5f) * near_ranks;
     }
     // A lane's expert and score, and which slot they are for: the slots' are the first `top`.
     int chosen = -1, place = lane;
