@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256) void k_plan_count(PlanArgs a) {
 
 template <bool ONE>
 __global__ __launch_bounds__(PLACE_LANES) void k_plan_place(PlanArgs a) {
-  extern __shared__ int lds[];
+  extern __shared__ __attribute__((aligned(16))) int lds[];  // (experts are read four at a time)
   const int *index = a.index + (long)blockIdx.x * a.at.chunk * a.top;
   if (ONE && a.tokens * a.top <= FEW_PAIRS) {
     if (threadIdx.x < a.tokens * a.top) lds[threadIdx.x] = bin_of(index[threadIdx.x], a.experts);
@@ -517,7 +517,7 @@ constexpr int route_lanes(int l) { return l == 16 ? 1024 : 512; }  // of a workg
 template <typename X, int L, int V, bool ONE>
 __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   constexpr int LANES = route_lanes(L), TOKENS = LANES / L;
-  extern __shared__ int lds[];
+  extern __shared__ __attribute__((aligned(16))) int lds[];  // (experts four at a time, ranks in f64; behind the arrays below)
   constexpr int LISTS = L == 16 ? TOKENS * 16 : 1;
   __shared__ int candidates[3 * LISTS];  // the keys of a token's, their scores, their experts
   __shared__ int boards[TOKENS * (L * V + 16)];  // a token's keys (16 more: a wave's four then write to different banks)
