@@ -522,7 +522,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   __shared__ int candidates[3 * LISTS];  // the keys of a token's, their scores, their experts
   __shared__ int boards[TOKENS * (L * V + 16)];  // a token's keys (16 more: a wave's four then write to different banks)
   __shared__ int taken_tokens;
-  __shared__ float biases[L * V], size_shared;
+  __shared__ float biases[L * V];
   const int experts = a.plan.experts, top = a.plan.top, n = experts + 1;
   int tid = threadIdx.x;
   int *bins = lds;                                      // the chunk's counts; ONE: its pairs' experts
@@ -531,23 +531,13 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
   if constexpr (!ONE) {
     for (int e = threadIdx.x; e < held; e += LANES) bins[e] = 0;
   }
-  int size_key = key_of(1.0f);  // of a choice that none is larger than
   for (int e = threadIdx.x; e < L * V; e += LANES) {
     const float b = a.bias && e < experts ? a.bias[e] : 0.0f;
     biases[e] = b > NONE ? b : NONE;  // (NaN too)
   }
   if (threadIdx.x == 0) taken_tokens = 0;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const float b = fabsf(biases[tid % L + L * i]);
-    if (b < __builtin_inff()) size_key = max(size_key, key_of(1.0f + b));
-  }
-  const float size_kept = value_of(largest<L>(size_key));  // (the same in all lanes)
-  if constexpr (V == 16) {  // (no register is left for it)
-    if (tid == 0) size_shared = size_kept;
-    __syncthreads();
-  }
+  __builtin_amdgcn_sched_barrier(0);  // (else the barrier waits for what every wave computes below: a token 5.8 us, so 5.3)
   const long begin = (long)blockIdx.x * a.plan.at.chunk, end = min(begin + a.plan.at.chunk, a.plan.tokens);
   for (;;) {
     // (What follows from it is cheaper to compute again than to keep: 48 registers too many.)
@@ -628,20 +618,32 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
 #pragma unroll
       for (int i = 0; i < V; i++) c[i] = gone >> i & 1 ? NO_KEY : c[i];
     }
-    // Two choices that are nearer than this may be in the other order (each is off by its score's error and its own
-    // rounding), and two ranks that are nearer than twice this and their own roundings.
-    const float choice_size = V == 16 ? size_shared : size_kept;
-    const float near = 0x1p-23f * (off + choice_size), near_ranks = 2.0f * near + 0x1p-22f * choice_size;
+    // Two choices that are nearer than this may be in the other order: each is off by its score's error and its own
+    // rounding, half a step of its size.  (That bound grows with a choice, so what is clear between neighbours in
+    // order is clear between all.  The factor is a step and what the comparison's own roundings come to.)
+    auto close = [&](float larger, float smaller) {
+      return larger - smaller < 0x1.0001p-23f * (off + fmaxf(fabsf(larger), fabsf(smaller)));
+    };
     bool unclear = false;
     if (a.kept < a.groups) {
       const int per = experts / a.groups;
       // Of two choices half their sum, which f32 always holds (two of its lowest values sum to what is no expert's).
+      float cancelled = 0.0f;  // the part of two choices that is not in their sum's size
       auto rank_of = [&](int best, int next) {
         if (a.group_top == 1) return best;
-        const float half = 0.5f * value_of(best);
-        return key_of(next > NO_KEY ? half + 0.5f * value_of(next) : half);
+        const float b = 0.5f * value_of(best), n = next > NO_KEY ? 0.5f * value_of(next) : 0.0f;
+        cancelled = fmaxf(cancelled, fminf(b, -n));
+        return key_of(b + n);
       };
-      int low = 0x7fffffff, high = NO_KEY;  // the last group kept, the first one not
+      // The least that a kept group's rank may be, the most that another's: it is off by the choices' errors, half a step
+      // of their sizes for the choices' roundings and another for the sum's, and the bound's own.  (An infinite
+      // one stays infinite.)
+      auto bound = [&](bool keep, int rank) {
+        const float r = value_of(rank);
+        const float by = 0x1.0001p-23f * (0.5f * off + 1.5f * fminf(fabsf(r), 0x1.fffffep127f) + 3.0f * cancelled);
+        return key_of(keep ? r - by : r + by);
+      };
+      int low = 0x7fffffff, high = NO_KEY;  // of the groups kept, and of the others
       // A group is OF of every lane's experts, one after another: G groups, the last of them of no expert perhaps.
       auto in_lanes = [&](auto of) {
         constexpr int OF = decltype(of)::value, G = V / OF, EVERY = 16 / G;
@@ -665,7 +667,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
         int ahead = 0;
         round_lanes<EVERY>([&](auto other) { ahead += other(mine) > mine; });
         const bool keep = ahead < a.kept && group < a.groups;
-        if (group < a.groups) (keep ? low : high) = own;
+        if (group < a.groups) (keep ? low : high) = bound(keep, own);
         const unsigned kept = (unsigned)(__ballot(keep) >> (L == 16 ? slot % 4 * 16 : 0));
 #pragma unroll
         for (int i = 0; i < V; i++) {
@@ -717,7 +719,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
             }
           }
           if (its) {
-            (ahead < a.kept ? low : high) = own;
+            (ahead < a.kept ? low : high) = bound(ahead < a.kept, own);
             mine[group] = ahead < a.kept;
           }
         } else {
@@ -729,9 +731,9 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
             int ahead = 0;
             for (int g = 0; g < a.groups; g++) ahead += mine[g] > rank || (mine[g] == rank && g < lane + L * j);
             if (ahead < a.kept)
-              keep |= 1ull << j, low = min(low, rank);
+              keep |= 1ull << j, low = min(low, bound(true, rank));
             else
-              high = max(high, rank);
+              high = max(high, bound(false, rank));
           }
           wave_fence();
           for (int j = 0; lane + L * j < a.groups; j++) mine[lane + L * j] = (int)(keep >> j & 1);
@@ -743,7 +745,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
         wave_fence();
       }
       low = least<L>(low), high = largest<L>(high);
-      unclear = high > NO_KEY && value_of(low) - value_of(high) < (a.group_top == 1 ? 1.0f : 0.5f) * near_ranks;
+      unclear = high > NO_KEY && low < high;
     }
     // A lane's expert and score, and which slot they are for: the slots' are the first `top`.
     int chosen = -1, place = lane;
@@ -789,8 +791,8 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
           wave_fence();
           first[place] = key;
           wave_fence();
-          const int close = taken && value_of(key) - value_of(first[place + 1]) < near;
-          unclear = unclear || largest<L>(close);
+          const int near = taken && close(value_of(key), value_of(first[place + 1]));
+          unclear = unclear || largest<L>(near);
         }
         total = group_sum<L>(score);
         any = largest<L>(key) > NO_KEY;
@@ -805,7 +807,7 @@ __global__ __launch_bounds__(route_lanes(L)) void k_route(RouteArgs a) {
         for (int i = 0; i < V; i++) key = max(key, c[i]);
         key = largest<L>(key);
         const float best = value_of(key);
-        if (key > NO_KEY && last - best < near) unclear = true;
+        if (key > NO_KEY && close(last, best)) unclear = true;
         last = best;
         any = any || key > NO_KEY;
         if (k == top) break;
