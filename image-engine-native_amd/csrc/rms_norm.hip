@@ -117,7 +117,12 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
         squares = (part[0] + part[1]) + (part[2] + part[3]);
       }
     }
-    const float inv = (float)(1.0 / sqrt(squares / c + (double)a.eps));
+    // A root that is past what has a normal reciprocal in f32 (of f32 rows, and where it is small without an epsilon) is
+    // taken towards 1 by a power of two, and so are the values that it divides.
+    const double root = sqrt(squares / c + (double)a.eps);
+    const float power = root < 0x1p-126 ? 0x1p64f : root > 0x1p126 ? 0x1p-64f : 1.0f;
+    const float inv = (float)(1.0 / (root * (double)power));
+    const bool far = (sizeof(X) == 4 || ADD == ADD_F32) && __ballot(power != 1.0f);
     auto store = [&](auto *row, int at, const float *w) {
       if (EIGHTS || at + 8 <= c)
         stream8(row + at, w);
@@ -128,6 +133,10 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsArgs a) {
     for (int n = 0; n < N; n++) {
       const int at = 8 * (n * L + lane);
       if (a.sum && some && at < c) store((X *)a.sum + r * a.sum_stride, at, v[n]);
+      if (far) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[n][i] *= power;
+      }
 #pragma unroll
       for (int i = 0; i < 8; i++) v[n][i] = v[n][i] * inv * g[n][i];
       if (a.y && some && at < c) {
