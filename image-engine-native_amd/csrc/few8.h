@@ -8,7 +8,8 @@
 // the weights' addresses wait for the tile's expert alone, not for its rows.  Products
 // are those of ien_multiply8's default (bf16 operands, sums in f32), whatever the
 // caller asks for: the matrix pipe has nothing else to do.  32 tokens, four of 64 experts
-// each, 1024 -> 2 x 1024 gated: 24.1 us, 4.8 TB/s of the weights of the 56 experts chosen.
+// each, 1024 -> 2 x 1024 gated: 24.1 us, 4.8 TB/s of the weights of the 56 experts that
+// have a token; 15.3 us where the tokens share 10 to 14 of them.
 #pragma once
 
 #include "tile8.h"

@@ -6,11 +6,17 @@
 // at most as a rule, is handed a lane each and ordered by counting; else the
 // largest choice is found top times.  Equal ones: the lowest index.  Vector
 // instructions bound it (over 90 % of the cycles): 65536 tokens, 8 of 256 experts in
-// 4 of 8 groups, take 39 us.  Without a bias choices are in the
+// 4 of 8 groups, take 38 us.  Without a bias choices are in the
 // order of the logits, which are compared themselves.  With one they are f32
 // sums that are off by some steps: where two that matter (neighbours among the
 // chosen, the last chosen and the next, the last group kept and the first not)
-// are nearer than that, the token is chosen again in f64.
+// are nearer than that, the token is chosen again in f64, by a whole wave: rare but for
+// choices that are equal to the last bit (a router of zeros under a bias: 65536 tokens of
+// 256 experts 171 us in place of 45, of 8 groups 279 in place of 50).
+//
+// More than 256 experts go by 64 lanes a token and top + 1 rounds of a maximum over
+// them: 65536 tokens, 8 of 300, 512 and 1024 experts 225, 232 and 240 us, of 1024 in
+// 32 groups 407.
 //
 // Planning is a counting sort that keeps the order of equal experts and adds
 // nothing atomically across workgroups, so it is the same every time.  The
@@ -228,8 +234,8 @@ __device__ void place_pairs(const PlanArgs &a, const PlaceShared &s, F expert) {
 
 // All of it for up to FEW_PAIRS pairs, a thread a pair: how many come before it is
 // counted pair by pair.  expert: their experts in LDS (as many as the next multiple of
-// sixteen), begin: room for as many.  (8 pairs of 64 experts with their choice: 7.6 us, the general
-// way 10.4; 128 pairs 13.0 and 11.3.)
+// sixteen), begin: room for as many.  (With their choice, of 64 experts: 8 pairs 5.4 us, the general
+// way 6.8; 64 pairs 7.6 and 6.9, 128 pairs 10.6 and 6.9.)
 constexpr int FEW_PAIRS = 64;
 __device__ void place_few(const PlanArgs &a, int *expert, int *begin) {
   const int pairs = (int)a.tokens * a.top, fours = (pairs + 15) / 16 * 4, p = threadIdx.x;

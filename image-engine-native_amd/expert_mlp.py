@@ -21,13 +21,15 @@ import ien
 class ExpertMlp8:
     """gamma: the norm's f32 gains (torch, on the GPU; or None).  router: c x
     experts weights and biases of the logits (numpy, kept in f16 and f32; biases
-    or None).  first, second: the experts' weights and biases, as Experts8 takes
+    or None; its product is of the norm in f16).  first, second: the experts' weights and biases, as Experts8 takes
     them (gated: first has 2 hidden columns).  how: the choice, as keywords of
     ien.route.
 
-    The first run of each number of tokens makes what lies between its steps; it
-    stays the block's until free(), so a captured run has it for as long as the
-    block lives.  Runs of a number of tokens share it: they follow each other, a
+    The first run of each number of tokens, which is not a captured one, makes
+    what lies between its steps; it stays the block's until free(), so a captured
+    run has it for as long as the block lives.  A program of many sizes keeps to
+    a few, by parts or padding, or frees the block.  An f16 stream is rounded once,
+    at its end.  Runs of a number of tokens share it: they follow each other, a
     graph's replays among them."""
 
     def __init__(self, ctx, c, top, gamma, router, first, second, gated=True, act=ien.ACT_SILU, eps=1e-6, how=None):
